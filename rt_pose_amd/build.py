@@ -19,7 +19,10 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-u
          "-Wno-int-to-pointer-cast",
          # no SLP vectoriser: it packs the epilogues' fp32 adds / multiplies into v_pk_add_f32 / v_pk_fma_f32, which cost more issue
          # time beside the matrix pipe than the scalar pairs they replace (fused data gradient of conv_tiled: 77.6 -> 72.8 us)
-         "-fno-slp-vectorize"] + os.environ.get("RTP_HIPCC_EXTRA", "").split()
+         "-fno-slp-vectorize",
+         # no packed fp32 at all (hipcc also forms v_pk_add / mul / fma_f32 from plain float code): some of their forms have given
+         # wrong results now and then.  The host pass does not know the feature and says so; harmless.
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("RTP_HIPCC_EXTRA", "").split()
 LIB = os.environ.get("RTP_BUILD_LIB", LIB)   # A/B builds: another output library (load it with RTP_LIB)
 OBJ = os.environ.get("RTP_BUILD_OBJ", OBJ)
 
