@@ -270,31 +270,31 @@ def _plain_attn(s):
 
 # ---------------------------------------------------------------------------------------------------------------- runs
 def _own(s):
-    from rt_pose_amd.attention import cross_attention
-    from rt_pose_amd.fp8 import matmul_fp8, quantize_fp8
-    from rt_pose_amd.rmsnorm import add_rms_norm, add_rms_norm_fp8, rms_norm
     c = s["case"]
-    if c["op"] == "norm" and c["mode"] == "fp8":
-        q, scale, stream = add_rms_norm_fp8(s["x"], s["r"], s["w"], EPS)
-        return {"q": q, "scale": scale, "stream": stream} if c["residual"] else {"q": q, "scale": scale}
-    if c["op"] == "norm" and c["residual"]:
-        y, stream = add_rms_norm(s["x"], s["r"], s["w"], EPS)
-        dx, dr, dw = torch.autograd.grad((y, stream), (s["x"], s["r"], s["w"]), (s["dy"], s["dh"]))
-        return {"y": y, "stream": stream, "dx": dx, "dr": dr, "dw": dw}
     if c["op"] == "norm":
-        y = rms_norm(s["x"], s["w"], EPS)
+        from rt_pose_amd import rmsnorm
+        if c["mode"] == "fp8":
+            q, scale, stream = rmsnorm.add_rms_norm_fp8(s["x"], s["r"], s["w"], EPS)
+            return {"q": q, "scale": scale, "stream": stream} if c["residual"] else {"q": q, "scale": scale}
+        if c["residual"]:
+            y, stream = rmsnorm.add_rms_norm(s["x"], s["r"], s["w"], EPS)
+            dx, dr, dw = torch.autograd.grad((y, stream), (s["x"], s["r"], s["w"]), (s["dy"], s["dh"]))
+            return {"y": y, "stream": stream, "dx": dx, "dr": dr, "dw": dw}
+        y = rmsnorm.rms_norm(s["x"], s["w"], EPS)
         dx, dw = torch.autograd.grad(y, (s["x"], s["w"]), s["dy"])
         return {"y": y, "dx": dx, "dw": dw}
+    if c["op"] == "attn":
+        from rt_pose_amd import attention
+        o = attention.cross_attention(s["q"], s["k"], s["v"], key_lens=s["lens"], key_mask=s["mask"])
+        if c["mode"] == "infer":
+            return o
+        dq, dk, dv = torch.autograd.grad(o, (s["q"], s["k"], s["v"]), s["do"])
+        return {"o": o, "dq": dq, "dk": dk, "dv": dv}
+    from rt_pose_amd import fp8
     if c["op"] == "quant":
-        q, scale = quantize_fp8(s["x"], (128, 128) if c["square"] else (1, 128))
+        q, scale = fp8.quantize_fp8(s["x"], (128, 128) if c["square"] else (1, 128))
         return {"q": q, "scale": scale}
-    if c["op"] == "matmul":
-        return matmul_fp8(s["a"], s["sa"], s["b"], s["sb"], out_dtype=TYPES[c["out"]])
-    o = cross_attention(s["q"], s["k"], s["v"], key_lens=s["lens"], key_mask=s["mask"])
-    if c["mode"] == "infer":
-        return o
-    dq, dk, dv = torch.autograd.grad(o, (s["q"], s["k"], s["v"]), s["do"])
-    return {"o": o, "dq": dq, "dk": dk, "dv": dv}
+    return fp8.matmul_fp8(s["a"], s["sa"], s["b"], s["sb"], out_dtype=TYPES[c["out"]])
 
 
 def run(s):
