@@ -550,6 +550,38 @@ int rtp_modulated_deform_conv_backward(const float* input, const float* weight, 
                                        int c, int h, int w, int co, int kh, int kw, int sh, int sw, int ph, int pw,
                                        int dh, int dw, int group, int deformable_group, int with_bias, void* stream);
 
+/* ---------------------------------------------------------------- F. token operators --- */
+/* Rows of tokens beside the volumes: norm, 8-bit quantising and product, cross attention.  Value types: */
+#define RTP_DT_F32 0
+#define RTP_DT_F16 1
+#define RTP_DT_BF16 2
+/* "8 bits" is OCP e4m3 (largest value 448), held in rows of at least the length rounded up to 16 bytes, 16-byte aligned.  Row strides
+ * (`*_rs`) are in elements; rows of the other types need no alignment.  An operand is q * scale with one fp32 scale for each 128 columns
+ * of a row (scale[rows][ceil(cols / 128)]) or for each 128 x 128 block ([ceil(rows / 128)][ceil(cols / 128)]).
+ *
+ * Root-mean-square norm (csrc/token_norm.hip): s = round(x + res), y = s / sqrt(mean(s^2) + eps) * w.  res may be NULL (s = x); s may be
+ * NULL when res is.  w_dtype: the values' type or RTP_DT_F32.  h <= 16384.  s, y, dx: contiguous rows of h.
+ * Backward: dx (= the residual's gradient too) = rho (g - xhat mean(g xhat)) + ds with g = dy w; ds may be NULL; dw of w's type.
+ * part: rtp_rmsnorm_backward_slots(rows, h) * h floats of scratch.  Deterministic. */
+int rtp_rmsnorm_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* y, void* s, long rows, int h,
+                        int dtype, float eps, void* stream);
+int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* q, long q_rs,
+                            float* scale, void* s, long rows, int h, int dtype, float eps, void* stream);
+int rtp_rmsnorm_backward_slots(long rows, int h);
+int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int w_dtype, const void* dy, long dy_rs, const void* ds, long ds_rs, void* dx,
+                         void* dw, float* part, long rows, int h, int dtype, float eps, void* stream);
+/* x -> q, scale with blocks of 1 x 128 (square = 0) or 128 x 128 (square = 1): a = max(largest magnitude, 2^-100), q = e4m3(x * (448 / a)),
+ * scale = a / 448.  turned = 1: x is given by columns, x[r][c] at c * x_rs + r (a transpose that is never written out).  The bytes between
+ * cols and cols rounded up to 8 are written too. */
+int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, float* scale, long rows, int cols, int square, int dtype,
+                     void* stream);
+
+/* out[m][n] = the product of a [m][k] and the transpose of b [n][k], both in 8 bits with scales (csrc/matmul_fp8.hip).  sa: [m][ceil(k / 128)];
+ * sb: [ceil(n / 128)][ceil(k / 128)] (b_square = 1) or [n][ceil(k / 128)].  Rows of a and b are readable up to k rounded up to 16; what stands
+ * there does not count.  out: row stride n, out_dtype any of the three. */
+int rtp_matmul_fp8(const void* a, long lda, const float* sa, const void* b, long ldb, const float* sb, int b_square, void* out, int m, int n,
+                   int k, int out_dtype, void* stream);
+
 /* ---------------------------------------------------------------- E. diagnostics --- */
 /* Per-kernel-family HIP-event timing on the launch stream (bench.py roofline leg). */
 int rtp_prof_enable(int family, int on);

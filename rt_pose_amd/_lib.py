@@ -152,6 +152,12 @@ PROTOTYPES = {
     "rtp_deform_conv_backward_overwrite": [_P] * 8 + [_I] * 15 + [_F, _I, _P],
     "rtp_modulated_deform_conv_forward": [_P, _P, _P, _P, _P, _P, _P] + [_I] * 16 + [_P],
     "rtp_modulated_deform_conv_backward": [_P] * 12 + [_I] * 16 + [_P],
+    "rtp_rmsnorm_forward": [_P, _L, _P, _L, _P, _I, _P, _P, _L, _I, _I, _F, _P],
+    "rtp_rmsnorm_fp8_forward": [_P, _L, _P, _L, _P, _I, _P, _L, _P, _P, _L, _I, _I, _F, _P],
+    "rtp_rmsnorm_backward_slots": [_L, _I],
+    "rtp_rmsnorm_backward": [_P, _L, _P, _I, _P, _L, _P, _L, _P, _P, _P, _L, _I, _I, _F, _P],
+    "rtp_quantize_fp8": [_P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _P],
+    "rtp_matmul_fp8": [_P, _L, _P, _P, _L, _P, _I, _P, _I, _I, _I, _I, _P],
     "rtp_prof_enable": [_I, _I],
     "rtp_prof_collect": [_I, C.POINTER(_F), C.POINTER(_I)],
     "rtp_version": [],

@@ -1,0 +1,432 @@
+// Root-mean-square norm of token rows with the residual's addition, in values or in 8 bits with scales, its backward pass, and the
+// step into 8 bits by itself.
+//
+//   s = round(x + r)        y = s * rho * w        rho = 1 / sqrt(mean(s^2) + eps)
+//   backward, g = dy * w, xhat = s * rho:   dx = dr = rho * (g - xhat * mean(g * xhat)) + ds        dw = sum over rows of dy * xhat
+//   8 bits: each 128 columns of a row share a = max(max|y|, 2^-100); q = e4m3(y * (448 / a)), scale = a / 448
+//
+// All of it is bound by HBM: 4 streams forward (x, r in; y, s out), 4 backward (dy, ds, s in; dx out), 16-64 operations per chunk of
+// eight.  A row is read ONCE: a group of LPR lanes holds it in registers (NV chunks of eight per lane) between the sum of squares and
+// the output, and the backward pass forms both of its row sums (s^2 and g * s) from one reading, so nothing but s is kept for it.
+// Sums are fp32, in an order that depends on the row's length alone.
+#include <type_traits>
+
+#include "rtp_prof.h"
+#include "token_common.h"
+
+// sum over the LPR lanes of a row; every lane gets it.  `red` holds one float per wave of the workgroup and is used twice in a row by
+// callers: the closing barrier keeps the second use off the first one's reads.
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if constexpr (LPR > 64) {
+    constexpr int NW = LPR / 64;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += red[i];
+    __syncthreads();
+  }
+  return v;
+}
+
+struct NormParams {
+  const void *x, *res, *w;
+  void *y, *s;
+  uint8_t* q;
+  float* scale;
+  long x_rs, res_rs, q_rs, rows;
+  int h;
+  float eps;
+};
+
+template <typename T, typename W, int LPR, int NV, bool OUT8>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(NormParams p) {
+  constexpr int THREADS = LPR > 256 ? LPR : 256;
+  __shared__ float red[THREADS / 64];
+  const int lane = threadIdx.x % LPR;
+  const long row = (long)blockIdx.x * (THREADS / LPR) + threadIdx.x / LPR;
+  if (LPR <= 64 && row >= p.rows) return;   // wider groups: one row per workgroup, the grid is exact
+  const T* x = (const T*)p.x + row * p.x_rs;
+  const T* r = p.res ? (const T*)p.res + row * p.res_rs : nullptr;
+  T* so = p.s ? (T*)p.s + row * p.h : nullptr;
+  float v[NV][8], wv[NV][8];
+  float sq = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) load8(v[i], x + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+  if (r) {
+    float rv[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load8(rv[i], r + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + rv[i][j]);   // the stream as it is written is what is normed
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) load8(wv[i], (const W*)p.w + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+  if (so) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store8(so + (lane + i * LPR) * 8, v[i], p.h - (lane + i * LPR) * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sq += v[i][j] * v[i][j];
+  const float rho = 1.f / sqrtf(row_sum<LPR>(sq, red) / (float)p.h + p.eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (lane + i * LPR) * 8, n = p.h - c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rho * wv[i][j];
+    if constexpr (!OUT8) {
+      store8((T*)p.y + row * p.h + c, v[i], n);
+    } else {
+      // a block of 128 columns = 16 neighbouring lanes; columns behind the row's end are zeros and change nothing
+      float a = amax8(v[i]);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+      a = fmaxf(a, RTP_FP8_AMAX_FLOOR);
+      if (n > 0) {
+        *(i32x2*)(p.q + row * p.q_rs + c) = to_fp8x8(v[i], RTP_FP8_MAX / a);   // up to the row's end rounded up to 8: inside its padding
+        if ((lane & 15) == 0) p.scale[row * ((p.h + 127) >> 7) + (c >> 7)] = a / RTP_FP8_MAX;
+      }
+    }
+  }
+}
+
+struct NormBwdParams {
+  const void *s, *w, *dy, *ds;
+  void* dx;
+  float* part;   // [gridDim.x][h]
+  long s_rs, dy_rs, ds_rs, rows;
+  int h;
+  float eps;
+};
+
+// Workgroups walk the rows with a stride; each lane keeps its columns' share of dw in registers over all its rows, a workgroup leaves one
+// partial row, and rmsnorm_dw_kernel adds those in fixed order: no atomics.
+template <typename T, typename W, int LPR, int NV>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(NormBwdParams p) {
+  constexpr int THREADS = LPR > 256 ? LPR : 256, GROUPS = THREADS / LPR;
+  __shared__ float red[THREADS / 64];
+  __shared__ float comb[GROUPS > 1 ? GROUPS * LPR * NV * 8 : 1];
+  const int lane = threadIdx.x % LPR, grp = threadIdx.x / LPR;
+  float wv[NV][8], dw[NV][8];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    load8(wv[i], (const W*)p.w + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+  }
+  for (long row = (long)blockIdx.x * GROUPS + grp; row < p.rows; row += (long)gridDim.x * GROUPS) {
+    float s[NV][8], g[NV][8];
+    float sq = 0.f, gs = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (lane + i * LPR) * 8;
+      load8(s[i], (const T*)p.s + row * p.s_rs + c, p.h - c);
+      load8(g[i], (const T*)p.dy + row * p.dy_rs + c, p.h - c);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sq += s[i][j] * s[i][j];
+        gs += g[i][j] * wv[i][j] * s[i][j];
+      }
+    const float rho = 1.f / sqrtf(row_sum<LPR>(sq, red) / (float)p.h + p.eps);
+    const float back = row_sum<LPR>(gs, red) / (float)p.h * rho * rho;   // mean(g * xhat) * rho: xhat * mean = s * back
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (lane + i * LPR) * 8, n = p.h - c;
+      float d[8];
+      if (p.ds) load8(d, (const T*)p.ds + row * p.ds_rs + c, n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dw[i][j] += g[i][j] * s[i][j] * rho;
+        const float own = rho * (g[i][j] * wv[i][j] - s[i][j] * back);
+        d[j] = p.ds ? own + d[j] : own;
+      }
+      store8((T*)p.dx + row * p.h + c, d, n);
+    }
+  }
+  if constexpr (GROUPS > 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) comb[grp * (LPR * NV * 8) + (lane + i * LPR) * 8 + j] = dw[i][j];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.h; c += THREADS) {
+      float t = 0.f;
+      for (int k = 0; k < GROUPS; ++k) t += comb[k * (LPR * NV * 8) + c];
+      p.part[(long)blockIdx.x * p.h + c] = t;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (lane + i * LPR) * 8;
+      store8(p.part + (long)blockIdx.x * p.h + c, dw[i], p.h - c);
+    }
+  }
+}
+
+// dw[c] = sum of the partial rows: 16 columns (one 64-byte line) x 64 row slots per workgroup, so that few columns still make enough loads
+template <typename W>
+__global__ __launch_bounds__(1024) void rmsnorm_dw_kernel(const float* part, int slots, int h, W* dw) {
+  __shared__ float red[64][17];
+  const int cl = threadIdx.x & 15, k = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
+  float t = 0.f;
+  if (c < h)
+    for (int i = k; i < slots; i += 64) t += part[(long)i * h + c];
+  red[k][cl] = t;
+  __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (k < o) red[k][cl] += red[k + o][cl];
+    __syncthreads();
+  }
+  if (k == 0 && c < h) dw[c] = (W)red[0][cl];
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+// lanes per row and chunks per lane by the row's length: 16 lanes up to 128 columns (four rows a wave), a wave up to 2048, a workgroup of
+// 256 up to 8192, of 1024 up to 16384 (its 128 registers a lane end there)
+#define NORM_MAX_H 16384
+
+template <typename F>
+static int norm_shape(int h, F f) {
+  if (h <= 128) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+  if (h <= 512) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+  if (h <= 1024) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  if (h <= 2048) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  if (h <= 4096) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+  if (h <= 8192) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+}
+
+// value type x weight type (fp32 weights beside half values, or the values' own type)
+template <typename F>
+static int norm_types(int dtype, int w_dtype, F f) {
+  if (dtype == RTP_DT_F32 && w_dtype == RTP_DT_F32) return f(float{}, float{});
+  if (dtype == RTP_DT_F16 && w_dtype == RTP_DT_F16) return f(_Float16{}, _Float16{});
+  if (dtype == RTP_DT_F16 && w_dtype == RTP_DT_F32) return f(_Float16{}, float{});
+  if (dtype == RTP_DT_BF16 && w_dtype == RTP_DT_BF16) return f(bf16_t{}, bf16_t{});
+  if (dtype == RTP_DT_BF16 && w_dtype == RTP_DT_F32) return f(bf16_t{}, float{});
+  return RTP_ERR_UNSUPPORTED;
+}
+
+template <bool OUT8>
+static int norm_forward(const NormParams& p, int dtype, int w_dtype, hipStream_t st) {
+  if (p.rows < 0 || p.h < 1 || p.rows >= (1L << 31)) return RTP_ERR_SHAPE;
+  if (p.h > NORM_MAX_H) return RTP_ERR_UNSUPPORTED;
+  if (p.rows == 0) return RTP_OK;
+  if (!p.x || !p.w || (p.res && !p.s)) return RTP_ERR_SHAPE;
+  RtpProfScope prof(RTP_FAM_NORM, st);
+  return norm_types(dtype, w_dtype, [&](auto t, auto w) {
+    return norm_shape(p.h, [&](auto lpr, auto nv) {
+      constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, THREADS = LPR > 256 ? LPR : 256;
+      hipLaunchKernelGGL((rmsnorm_fwd_kernel<decltype(t), decltype(w), LPR, NV, OUT8>), dim3(rtp_div_up(p.rows, THREADS / LPR)), dim3(THREADS), 0,
+                         st, p);
+      RTP_CHECK_LAUNCH();
+      return RTP_OK;
+    });
+  });
+}
+
+extern "C" int rtp_rmsnorm_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* y, void* s,
+                                   long rows, int h, int dtype, float eps, void* stream) {
+  if (rows > 0 && !y) return RTP_ERR_SHAPE;
+  NormParams p{x, res, w, y, s, nullptr, nullptr, x_rs, res_rs, 0, rows, h, eps};
+  return norm_forward<false>(p, dtype, w_dtype, (hipStream_t)stream);
+}
+
+extern "C" int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* q, long q_rs,
+                                       float* scale, void* s, long rows, int h, int dtype, float eps, void* stream) {
+  if (rows > 0 && (!q || !scale)) return RTP_ERR_SHAPE;
+  if (q_rs < ((h + 15) & ~15)) return RTP_ERR_SHAPE;
+  if (((size_t)q & 15) || (q_rs & 15)) return RTP_ERR_ALIGN;
+  NormParams p{x, res, w, nullptr, s, (uint8_t*)q, scale, x_rs, res_rs, q_rs, rows, h, eps};
+  return norm_forward<true>(p, dtype, w_dtype, (hipStream_t)stream);
+}
+
+// partial rows of dw: two workgroups per CU walk the rows, fewer where there are fewer
+extern "C" int rtp_rmsnorm_backward_slots(long rows, int h) {
+  if (rows < 1 || h < 1 || h > NORM_MAX_H) return 0;
+  const int groups = h <= 128 ? 16 : h <= 2048 ? 4 : 1;
+  const long need = (rows + groups - 1) / groups;
+  return (int)(need < 512 ? need : 512);
+}
+
+extern "C" int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int w_dtype, const void* dy, long dy_rs, const void* ds, long ds_rs,
+                                    void* dx, void* dw, float* part, long rows, int h, int dtype, float eps, void* stream) {
+  if (rows < 1 || h < 1 || rows >= (1L << 31)) return RTP_ERR_SHAPE;
+  if (h > NORM_MAX_H) return RTP_ERR_UNSUPPORTED;
+  if (!s || !w || !dy || !dx || !dw || !part) return RTP_ERR_SHAPE;
+  hipStream_t st = (hipStream_t)stream;
+  RtpProfScope prof(RTP_FAM_NORM, st);
+  NormBwdParams p{s, w, dy, ds, dx, part, s_rs, dy_rs, ds_rs, rows, h, eps};
+  const int slots = rtp_rmsnorm_backward_slots(rows, h);
+  return norm_types(dtype, w_dtype, [&](auto t, auto wt) {
+    return norm_shape(h, [&](auto lpr, auto nv) {
+      constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, THREADS = LPR > 256 ? LPR : 256;
+      typedef decltype(wt) W;
+      hipLaunchKernelGGL((rmsnorm_bwd_kernel<decltype(t), W, LPR, NV>), dim3(slots), dim3(THREADS), 0, st, p);
+      RTP_CHECK_LAUNCH();
+      hipLaunchKernelGGL((rmsnorm_dw_kernel<W>), dim3(rtp_div_up(h, 16)), dim3(1024), 0, st, part, slots, h, (W*)dw);
+      RTP_CHECK_LAUNCH();
+      return RTP_OK;
+    });
+  });
+}
+
+// ------------------------------------------------------------------------------------------------ quantising by itself
+struct QuantParams {
+  const void* x;
+  uint8_t* q;
+  float* scale;
+  long x_rs, q_rs, rows;
+  int cols, kb;
+};
+
+// blocks of 1 x 128, rows in memory order: 16 lanes a block, four rows a lane so that four loads are in flight
+#define QUANT_ROWS 4
+template <typename T>
+__global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
+  const unsigned g = blockIdx.x * 16u + (threadIdx.x >> 4);
+  const int lane = threadIdx.x & 15;
+  const long row0 = (long)(g / (unsigned)p.kb) * QUANT_ROWS;
+  const int b = (int)(g % (unsigned)p.kb), c = b * 128 + lane * 8, n = p.cols - c;
+  float v[QUANT_ROWS][8];
+#pragma unroll
+  for (int u = 0; u < QUANT_ROWS; ++u)
+    load8(v[u], (const T*)p.x + (row0 + u) * p.x_rs + c, row0 + u < p.rows ? n : 0);
+#pragma unroll
+  for (int u = 0; u < QUANT_ROWS; ++u) {
+    float a = amax8(v[u]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+    a = fmaxf(a, RTP_FP8_AMAX_FLOOR);
+    if (row0 + u < p.rows && n > 0) {
+      *(i32x2*)(p.q + (row0 + u) * p.q_rs + c) = to_fp8x8(v[u], RTP_FP8_MAX / a);
+      if (lane == 0) p.scale[(row0 + u) * p.kb + b] = a / RTP_FP8_MAX;
+    }
+  }
+}
+
+// blocks of 128 x 128, rows in memory order: one workgroup a block, held in registers between its maximum and the output
+template <typename T>
+__global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
+  __shared__ float red[4];
+  const int lane = threadIdx.x & 15, b = blockIdx.x % (unsigned)p.kb;
+  const long row0 = (long)(blockIdx.x / (unsigned)p.kb) * 128 + (threadIdx.x >> 4);
+  const int c = b * 128 + lane * 8, n = p.cols - c;
+  float v[8][8];
+  float a = 0.f;
+#pragma unroll
+  for (int u = 0; u < 8; ++u) load8(v[u], (const T*)p.x + (row0 + u * 16) * p.x_rs + c, row0 + u * 16 < p.rows ? n : 0);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) a = fmaxf(a, amax8(v[u]));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+  __syncthreads();
+  a = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), RTP_FP8_AMAX_FLOOR);
+  const float up = RTP_FP8_MAX / a;
+#pragma unroll
+  for (int u = 0; u < 8; ++u)
+    if (row0 + u * 16 < p.rows && n > 0) *(i32x2*)(p.q + (row0 + u * 16) * p.q_rs + c) = to_fp8x8(v[u], up);
+  if (threadIdx.x == 0) p.scale[blockIdx.x] = a / RTP_FP8_MAX;
+}
+
+// Either block, x given by columns (a transpose's view: x[r][c] at c * x_rs + r).  A tile of 128 rows x 128 columns goes through LDS:
+// read along the columns' memory order, then each thread takes 64 columns of one row -- neighbouring lanes take neighbouring rows, so the
+// reads of a wave are consecutive halves -- and writes them as 64 bytes.  The pitch keeps the 16-byte stores aligned.
+template <typename T, bool SQUARE>
+__global__ __launch_bounds__(256) void quant_turned_kernel(QuantParams p) {
+  constexpr int PITCH = 128 + 16 / sizeof(T);
+  __shared__ __attribute__((aligned(16))) T tile[128 * PITCH];
+  __shared__ float red[256];
+  const int b = blockIdx.x % (unsigned)p.kb;
+  const long row0 = (long)(blockIdx.x / (unsigned)p.kb) * 128;
+  {
+    const int ch = (threadIdx.x & 15) * 8;
+    const long left = p.rows - row0 - ch;
+    const int n = left < 0 ? 0 : left > 8 ? 8 : (int)left;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int c = (threadIdx.x >> 4) + u * 16;
+      float v[8];
+      load8(v, (const T*)p.x + (long)(b * 128 + c) * p.x_rs + row0 + ch, b * 128 + c < p.cols ? n : 0);
+      store8(tile + c * PITCH + ch, v, 8);
+    }
+  }
+  __syncthreads();
+  const int r = threadIdx.x & 127, half = threadIdx.x >> 7;
+  float a = 0.f;
+#pragma unroll 16
+  for (int c = 0; c < 64; ++c) a = fmaxf(a, fabsf((float)tile[(half * 64 + c) * PITCH + r]));
+  if constexpr (SQUARE) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    a = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  } else {
+    red[threadIdx.x] = a;
+    __syncthreads();
+    a = fmaxf(red[r], red[r + 128]);
+  }
+  a = fmaxf(a, RTP_FP8_AMAX_FLOOR);
+  const float up = RTP_FP8_MAX / a;
+  if (row0 + r < p.rows) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = half * 64 + k * 16;
+      if (b * 128 + c < p.cols) {
+        float lo[8], hi[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          lo[j] = (float)tile[(c + j) * PITCH + r];
+          hi[j] = (float)tile[(c + 8 + j) * PITCH + r];
+        }
+        const i32x2 l = to_fp8x8(lo, up), h = to_fp8x8(hi, up);
+        *(i32x4*)(p.q + (row0 + r) * p.q_rs + b * 128 + c) = i32x4{l[0], l[1], h[0], h[1]};
+      }
+    }
+    if (!SQUARE && half == 0) p.scale[(row0 + r) * p.kb + b] = a / RTP_FP8_MAX;
+  }
+  if (SQUARE && threadIdx.x == 0) p.scale[blockIdx.x] = a / RTP_FP8_MAX;
+}
+
+extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, float* scale, long rows, int cols, int square, int dtype,
+                                void* stream) {
+  if (rows < 0 || cols < 1 || q_rs < ((cols + 15) & ~15)) return RTP_ERR_SHAPE;
+  if (rows == 0) return RTP_OK;
+  if (!x || !q || !scale) return RTP_ERR_SHAPE;
+  if (((size_t)q & 15) || (q_rs & 15)) return RTP_ERR_ALIGN;
+  hipStream_t st = (hipStream_t)stream;
+  RtpProfScope prof(RTP_FAM_NORM, st);
+  const int kb = (cols + 127) >> 7;
+  QuantParams p{x, (uint8_t*)q, scale, x_rs, q_rs, rows, cols, kb};
+  const long tiles = ((rows + 127) >> 7) * kb, groups = ((rows + QUANT_ROWS - 1) / QUANT_ROWS) * kb;
+  if (tiles >= (1L << 31) || groups >= (1L << 31)) return RTP_ERR_SHAPE;
+  auto go = [&](auto t) {
+    typedef decltype(t) T;
+    if (turned && square)
+      hipLaunchKernelGGL((quant_turned_kernel<T, true>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+    else if (turned)
+      hipLaunchKernelGGL((quant_turned_kernel<T, false>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+    else if (square)
+      hipLaunchKernelGGL((quant_square_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((quant_rows_kernel<T>), dim3(rtp_div_up(groups, 16)), dim3(256), 0, st, p);
+    RTP_CHECK_LAUNCH();
+    return RTP_OK;
+  };
+  if (dtype == RTP_DT_F32) return go(float{});
+  if (dtype == RTP_DT_F16) return go(_Float16{});
+  if (dtype == RTP_DT_BF16) return go(bf16_t{});
+  return RTP_ERR_UNSUPPORTED;
+}
