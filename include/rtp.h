@@ -582,6 +582,28 @@ int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, f
 int rtp_matmul_fp8(const void* a, long lda, const float* sa, const void* b, long ldb, const float* sb, int b_square, void* out, int m, int n,
                    int k, int out_dtype, void* stream);
 
+/* Cross attention (csrc/cross_attn.hip): o[b][i][h] = sum_j softmax_j(scale q[b][i][h] . k[b][j][h / (hq / hkv)]) v[b][j][...] over the keys j that
+ * count in batch entry b: j < key_lens[b] (clamped to 0 .. sk; NULL: all) and key_mask[b][j] (bytes, strides m_bs and m_ss; NULL: all).  Keys that
+ * do not count are not read, whatever they hold; a row without keys gives zeros and takes part in no gradient.  fp16 or bf16, d a multiple of 8
+ * up to 128, scale > 0.  Strides in elements, of batch, token and head; the columns of a head are contiguous; every row 16-byte aligned.
+ * o, dq: contiguous [b][sq][hq][d]; dk, dv: contiguous [b][sk][hkv][d], zeros at keys that do not count.  dq, or dk and dv, may be NULL.
+ * For a backward pass the forward pass also leaves o_lo (what o's rounding left over, o's type and shape) and lse ([b][hkv][sq * hq / hkv] fp32:
+ * base-2 logarithm of the sum of exponentials); both NULL otherwise.  o_bs, o_ss, o_hs: of d_o.  ws: rtp_xattn_workspace_bytes(a, backward) bytes,
+ * 256-byte aligned; -1 for what the entries refuse.  No atomics: results do not depend on scheduling. */
+typedef struct RtpXattn {
+  const void *q, *k, *v;
+  long q_bs, q_ss, q_hs, k_bs, k_ss, k_hs, v_bs, v_ss, v_hs;
+  const void* key_mask;
+  long m_bs, m_ss;
+  const int* key_lens;
+  int b, sq, sk, hq, hkv, d, dtype;
+  float scale;
+} RtpXattn;
+long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward);
+int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* lse, void* ws, long ws_bytes, void* stream);
+int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* o_lo, const float* lse, const void* d_o, long o_bs, long o_ss, long o_hs,
+                       void* dq, void* dk, void* dv, void* ws, long ws_bytes, void* stream);
+
 /* ---------------------------------------------------------------- E. diagnostics --- */
 /* Per-kernel-family HIP-event timing on the launch stream (bench.py roofline leg). */
 int rtp_prof_enable(int family, int on);

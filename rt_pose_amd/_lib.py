@@ -53,6 +53,14 @@ class RtpConv64(C.Structure):
                 ("relu", C.c_int), ("transposed", C.c_int)]
 
 
+class RtpXattn(C.Structure):
+    """include/rtp.h: operands of the cross-attention entries."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v")]
+                + [(n, C.c_long) for n in ("q_bs", "q_ss", "q_hs", "k_bs", "k_ss", "k_hs", "v_bs", "v_ss", "v_hs")]
+                + [("key_mask", C.c_void_p), ("m_bs", C.c_long), ("m_ss", C.c_long), ("key_lens", C.c_void_p)]
+                + [(n, C.c_int) for n in ("b", "sq", "sk", "hq", "hkv", "d", "dtype")] + [("scale", C.c_float)])
+
+
 class RtpGnLazy(C.Structure):
     _fields_ = [("pq", C.c_void_p), ("nsplit", C.c_int), ("mr", C.c_void_p), ("gamma", C.c_void_p), ("groups", C.c_int)]
 
@@ -158,6 +166,9 @@ PROTOTYPES = {
     "rtp_rmsnorm_backward": [_P, _L, _P, _I, _P, _L, _P, _L, _P, _P, _P, _L, _I, _I, _F, _P],
     "rtp_quantize_fp8": [_P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _P],
     "rtp_matmul_fp8": [_P, _L, _P, _P, _L, _P, _I, _P, _I, _I, _I, _I, _P],
+    "rtp_xattn_workspace_bytes": [C.POINTER(RtpXattn), _I],
+    "rtp_xattn_forward": [C.POINTER(RtpXattn), _P, _P, _P, _P, _L, _P],
+    "rtp_xattn_backward": [C.POINTER(RtpXattn), _P, _P, _P, _P, _L, _L, _L, _P, _P, _P, _P, _L, _P],
     "rtp_prof_enable": [_I, _I],
     "rtp_prof_collect": [_I, C.POINTER(_F), C.POINTER(_I)],
     "rtp_version": [],
@@ -165,7 +176,7 @@ PROTOTYPES = {
     "rtp_multi_begin": [], "rtp_multi_param_bytes": [], "rtp_multi_end": [_P, _L, C.POINTER(_I)], "rtp_multi_abort": [],
     "rtp_multi_launch": [_I, _P], "rtp_multi_free": [_I],
 }
-_RESTYPE = {"rtp_version": C.c_char_p, "rtp_multi_param_bytes": C.c_long, "rtp_dcn_workspace_bytes": C.c_long, "rtp_voxelize_workspace_bytes": C.c_long,
+_RESTYPE = {"rtp_version": C.c_char_p, "rtp_multi_param_bytes": C.c_long, "rtp_dcn_workspace_bytes": C.c_long, "rtp_xattn_workspace_bytes": C.c_long, "rtp_voxelize_workspace_bytes": C.c_long,
             "rtp_upsample_bwd_scratch_floats": C.c_long}
 
 _lib = None

@@ -1,23 +1,31 @@
-"""Marshalling shared by the token operators (rmsnorm.py, fp8.py, attention.py)."""
-import ctypes as C
-
+"""Marshalling shared by the token operators (rmsnorm.py, fp8.py, attention.py).  Small calls are bound by the host: one native call, no
+context manager and no stream object where the tensor's device is already the current one."""
 import torch
+
+from . import _lib
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # RTP_DT_* of include/rtp.h
 FP8 = torch.float8_e4m3fn
 
 
 def p(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else None
+    return None if t is None else t.data_ptr()
 
 
-def stream_of(t):
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+# the current stream's handle without a Stream object around it: 0.1 us instead of 1.2, and 15 us less in a backward pass, whose thread is another
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def on_device(t):
-    """Launches go to the tensor's device, whichever is current."""
-    return torch.cuda.device(t.device)
+def call(name, t, *args):
+    """The native entry `name` on the current stream of t's device, with that device current; RtpError if it fails."""
+    index = t.device.index
+    if index == _current_device():
+        rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def same_device(x, *others):
@@ -30,7 +38,8 @@ def same_device(x, *others):
 
 def rows_of(t):
     """[..., n] as [rows, n] with unit stride along the row: a view where there is one, a copy otherwise."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -38,6 +47,7 @@ def fp8_rows(shape, device, scale_rows=None):
     """An uninitialised 8-bit operand of `shape` (rows of a multiple of 16 bytes in memory) and its scales, one for 128 columns of each row
     (or of `scale_rows` rows)."""
     *lead, n = shape
-    q = torch.empty((*lead, -(-n // 16) * 16), dtype=torch.uint8, device=device).view(FP8)[..., :n]
+    wide = -(-n // 16) * 16
+    q = torch.empty((*lead, wide), dtype=FP8, device=device)
     scale = torch.empty((*lead, -(-n // 128)) if scale_rows is None else (scale_rows, -(-n // 128)), dtype=torch.float32, device=device)
-    return q, scale
+    return q if wide == n else q[..., :n], scale

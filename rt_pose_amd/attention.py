@@ -1,0 +1,114 @@
+"""Cross attention to an encoder's states of another length, on csrc/cross_attn.hip.
+
+    cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None)      [batch, queries, heads, dim]
+
+q: [b, sq, hq, d]; k, v: [b, sk, hkv, d] with hq a multiple of hkv (head h reads k and v of head h // (hq // hkv)).  Of batch entry i the keys j
+with j < key_lens[i] and key_mask[i, j] count.  Keys that do not count -- an encoder's padding -- are never multiplied, whatever they hold (NaN
+too), and get zero gradients; a row without keys gives zeros.  bf16 or fp16, d a multiple of 8 up to 128; any strides (a tensor whose rows
+are not 16-byte aligned is copied).  Sums and softmax are fp32; the result does not depend on scheduling.  Differentiable in q, k and v.
+With few queries (single tokens while serving, key-point queries) the keys are split over the GPU and joined.
+Errors as in rt_pose_amd.rmsnorm.
+"""
+import ctypes as C
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._tokens import DTYPES, call, p, same_device
+
+
+def _check(q, k, v, key_lens, key_mask, scale):
+    same_device(q, k, v, key_lens, key_mask)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError("cross_attention: bf16 or fp16 only (got %s)" % q.dtype)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("cross_attention: q, k and v of one type expected (got %s, %s, %s)" % (q.dtype, k.dtype, v.dtype))
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("cross_attention: [b, sq, hq, d] and twice [b, sk, hkv, d] expected (got %s, %s, %s)"
+                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if k.shape[2] < 1 or q.shape[2] < 1 or q.shape[2] % k.shape[2]:
+        raise ValueError("cross_attention: %d query heads are no multiple of %d key heads" % (q.shape[2], k.shape[2]))
+    if q.shape[3] < 8 or q.shape[3] % 8 or q.shape[3] > 128:
+        raise NotImplementedError("cross_attention: head widths of a multiple of 8 up to 128 (got %d)" % q.shape[3])
+    if key_lens is not None and (key_lens.shape != q.shape[:1] or key_lens.dtype not in (torch.int32, torch.int64)):
+        raise ValueError("cross_attention: key_lens of shape (%d,) and whole numbers expected (got %s %s)"
+                         % (q.shape[0], tuple(key_lens.shape), key_lens.dtype))
+    if key_mask is not None and key_mask.dtype != torch.bool:
+        raise NotImplementedError("cross_attention: key_mask of truth values only, True where a key counts (got %s)" % key_mask.dtype)
+    if key_mask is not None and key_mask.shape != k.shape[:2]:
+        raise ValueError("cross_attention: key_mask of shape %s expected (got %s)" % (tuple(k.shape[:2]), tuple(key_mask.shape)))
+    if not 0.0 < scale <= 3e38:
+        raise ValueError("cross_attention: a positive, finite scale expected (got %r)" % (scale,))
+
+
+def _aligned(t):
+    """t with contiguous heads in rows on 16-byte boundaries: itself, or a copy."""
+    st = t.stride()
+    if st[3] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 or n == 1 for s, n in zip(st[:3], t.shape)):
+        return t
+    return t.contiguous()
+
+
+def _strides(t):
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+
+
+def _operands(q, k, v, key_lens, key_mask, scale):
+    b, sq, hq, d = q.shape
+    return _lib.RtpXattn(p(q), p(k), p(v), *_strides(q), *_strides(k), *_strides(v), p(key_mask),
+                         *((0, 0) if key_mask is None else key_mask.stride()), p(key_lens), b, sq, k.shape[1], hq, k.shape[2], d, DTYPES[q.dtype], scale)
+
+
+def _workspace(a, backward, like):
+    n = _lib.load().rtp_xattn_workspace_bytes(C.byref(a), backward)
+    if n < 0:
+        raise _lib.RtpError("cross_attention: sizes beyond what the kernels index (%s)" % (tuple(like.shape),))
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None, n
+
+
+def _forward(q, k, v, key_lens, key_mask, scale, train):
+    a = _operands(q, k, v, key_lens, key_mask, scale)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o_lo, lse = (torch.empty_like(o), q.new_empty(o.shape[:3].numel(), dtype=torch.float32)) if train else (None, None)
+    if o.numel():
+        ws, n = _workspace(a, 0, q)
+        call("rtp_xattn_forward", q, C.byref(a), p(o), p(o_lo), p(lse), p(ws), n)
+    return o, o_lo, lse
+
+
+class CrossAttentionFunction(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, key_lens, key_mask, scale):
+        o, o_lo, lse = _forward(q, k, v, key_lens, key_mask, scale, True)
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, key_lens, key_mask, o, o_lo, lse)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, key_lens, key_mask, o, o_lo, lse = ctx.saved_tensors
+        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
+        dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if need_kv else None for t in (k, v))
+        if q.numel() == 0 or k.numel() == 0:
+            return tuple(None if t is None else t.zero_() for t in (dq, dk, dv)) + (None, None, None)
+        do = _aligned(do)
+        a = _operands(q, k, v, key_lens, key_mask, ctx.scale)
+        ws, n = _workspace(a, 1, q)
+        call("rtp_xattn_backward", q, C.byref(a), p(o), p(o_lo), p(lse), p(do), *_strides(do), p(dq), p(dk), p(dv), p(ws), n)
+        return dq, dk, dv, None, None, None
+
+
+def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
+    """scale: 1 / sqrt(d) by default.  key_lens: [b] int32 or int64 (taken between 0 and sk); key_mask: [b, sk], True where a key counts."""
+    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() == 4 and q.shape[-1] else 1.0 if scale is None else float(scale)
+    _check(q, k, v, key_lens, key_mask, scale)
+    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    if key_lens is not None:
+        key_lens = (key_lens if key_lens.dtype == torch.int32 else key_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return CrossAttentionFunction.apply(q, k, v, key_lens, key_mask, scale)
+    return _forward(q, k, v, key_lens, key_mask, scale, False)[0]

@@ -11,8 +11,7 @@ Neither function is differentiable.  Errors as in rt_pose_amd.rmsnorm.
 """
 import torch
 
-from . import _lib
-from ._tokens import DTYPES, FP8, fp8_rows, on_device, p, rows_of, same_device, stream_of
+from ._tokens import DTYPES, FP8, call, fp8_rows, p, rows_of, same_device
 
 
 @torch.no_grad()
@@ -32,9 +31,8 @@ def quantize_fp8(x, block=(1, 128)):
     x2 = x if turned else rows_of(x)
     rows, cols = x2.shape
     q, scale = fp8_rows(x.shape, x.device, -(-rows // 128) if square else None)
-    with on_device(x):
-        _lib.check(_lib.load().rtp_quantize_fp8(p(x2), x2.stride(1) if turned else x2.stride(0), int(turned), p(q), -(-cols // 16) * 16, p(scale),
-                                                rows, cols, int(square), DTYPES[x.dtype], stream_of(x)), "rtp_quantize_fp8")
+    call("rtp_quantize_fp8", x, p(x2), x2.stride(1) if turned else x2.stride(0), int(turned), p(q), -(-cols // 16) * 16, p(scale), rows, cols,
+         int(square), DTYPES[x.dtype])
     return q, scale
 
 
@@ -79,7 +77,5 @@ def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16):
     a2, lda = _operand(a.reshape(-1, k), "a")
     b2, ldb = _operand(b, "b")
     sa, sb = a_scale.reshape(-1, kb).contiguous(), b_scale.contiguous()
-    with on_device(a):
-        _lib.check(_lib.load().rtp_matmul_fp8(p(a2), lda, p(sa), p(b2), ldb, p(sb), int(b_scale.shape[0] == nb), p(out), a2.shape[0], n, k,
-                                              DTYPES[out_dtype], stream_of(a)), "rtp_matmul_fp8")
+    call("rtp_matmul_fp8", a, p(a2), lda, p(sa), p(b2), ldb, p(sb), int(b_scale.shape[0] == nb), p(out), a2.shape[0], n, k, DTYPES[out_dtype])
     return out

@@ -16,7 +16,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tokens import DTYPES, fp8_rows, on_device, p, rows_of, same_device, stream_of
+from ._tokens import DTYPES, call, fp8_rows, p, rows_of, same_device
 
 
 def _check(x, residual, weight):
@@ -37,27 +37,24 @@ def _check(x, residual, weight):
 def _forward(x, residual, weight, eps):
     x2, w = rows_of(x), weight.contiguous()
     r2 = rows_of(residual) if residual is not None else None
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    with on_device(x):
-        _lib.check(_lib.load().rtp_rmsnorm_forward(p(x2), x2.stride(0), p(r2), r2.stride(0) if r2 is not None else 0, p(w), DTYPES[w.dtype], p(y),
-                                                   p(s), x2.shape[0], x2.shape[1], DTYPES[x.dtype], eps, stream_of(x)), "rtp_rmsnorm_forward")
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    s = torch.empty_like(y) if residual is not None else None
+    call("rtp_rmsnorm_forward", x, p(x2), x2.stride(0), p(r2), 0 if r2 is None else r2.stride(0), p(w), DTYPES[w.dtype], p(y), p(s), *x2.shape,
+         DTYPES[x.dtype], eps)
     return y, s
 
 
 def _backward(s, weight, eps, dy, ds, need_w):
     """dx (also the residual's gradient) and dw of the rows `s` that were normed."""
     s2, w = rows_of(s), weight.contiguous()
-    dx, dw = torch.empty(s.shape, dtype=s.dtype, device=s.device), torch.empty_like(w)
-    if s2.shape[0] == 0:
+    rows, h = s2.shape
+    dx, dw = torch.empty_like(s, memory_format=torch.contiguous_format), torch.empty_like(w)
+    if rows == 0:
         return dx, dw.zero_() if need_w else None
     dy2, ds2 = rows_of(dy), rows_of(ds) if ds is not None else None
-    lib = _lib.load()
-    part = torch.empty(lib.rtp_rmsnorm_backward_slots(*s2.shape) * s2.shape[1], dtype=torch.float32, device=s.device)
-    with on_device(s):
-        _lib.check(lib.rtp_rmsnorm_backward(p(s2), s2.stride(0), p(w), DTYPES[w.dtype], p(dy2), dy2.stride(0), p(ds2),
-                                            ds2.stride(0) if ds2 is not None else 0, p(dx), p(dw), p(part), s2.shape[0], s2.shape[1],
-                                            DTYPES[s.dtype], eps, stream_of(s)), "rtp_rmsnorm_backward")
+    part = torch.empty(_lib.load().rtp_rmsnorm_backward_slots(rows, h) * h, dtype=torch.float32, device=s.device)
+    call("rtp_rmsnorm_backward", s, p(s2), s2.stride(0), p(w), DTYPES[w.dtype], p(dy2), dy2.stride(0), p(ds2), 0 if ds2 is None else ds2.stride(0),
+         p(dx), p(dw), p(part), rows, h, DTYPES[s.dtype], eps)
     return dx, dw if need_w else None
 
 
@@ -116,10 +113,8 @@ def add_rms_norm_fp8(x, residual, weight, eps=1e-6):
     r2 = rows_of(residual) if residual is not None else None
     q, scale = fp8_rows(x.shape, x.device)
     s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    with on_device(x):
-        _lib.check(_lib.load().rtp_rmsnorm_fp8_forward(p(x2), x2.stride(0), p(r2), r2.stride(0) if r2 is not None else 0, p(w), DTYPES[w.dtype],
-                                                       p(q), -(-x.shape[-1] // 16) * 16, p(scale), p(s), x2.shape[0],
-                                                       x2.shape[1], DTYPES[x.dtype], float(eps), stream_of(x)), "rtp_rmsnorm_fp8_forward")
+    call("rtp_rmsnorm_fp8_forward", x, p(x2), x2.stride(0), p(r2), 0 if r2 is None else r2.stride(0), p(w), DTYPES[w.dtype], p(q),
+         -(-x.shape[-1] // 16) * 16, p(scale), p(s), *x2.shape, DTYPES[x.dtype], float(eps))
     return q, scale, x if s is None else s
 
 

@@ -57,3 +57,53 @@ def test_8_bit_entries_check_before_they_launch():
     assert mm(k=0) == SHAPE and mm(m=-1) == SHAPE and mm(a=None) == SHAPE and mm(lda=112) == SHAPE and mm(k=129) == SHAPE
     assert mm(lda=136) == ALIGN and mm(b=P(4097)) == ALIGN and mm(t=3) == UNSUPPORTED
     assert mm(m=2 ** 31 - 1, n=2 ** 31 - 1) == SHAPE
+
+
+def test_cross_attention_has_no_cpu_path():
+    from rt_pose_amd.attention import cross_attention
+    q = torch.zeros(1, 2, 4, 32, dtype=torch.bfloat16)
+    with pytest.raises(NotImplementedError):
+        cross_attention(q, q, q)
+
+
+def attn(**k):
+    a = _lib.RtpXattn()
+    for n in ("q", "k", "v"):
+        setattr(a, n, 4096)
+    for n, v in dict(dict(b=2, sq=3, sk=5, hq=4, hkv=2, d=64, dtype=2, scale=0.125, q_bs=768, q_ss=256, q_hs=64, k_bs=640, k_ss=128, k_hs=64,
+                          v_bs=640, v_ss=128, v_hs=64), **k).items():
+        setattr(a, n, v)
+    return a
+
+
+def test_cross_attention_entries_check_before_they_launch():
+    lib = _lib.load()
+    o = P(4096)
+    size = lambda back=0, **k: lib.rtp_xattn_workspace_bytes(C.byref(attn(**k)), back)
+    fwd = lambda o_lo=None, lse=None, ws=None, n=0, **k: lib.rtp_xattn_forward(C.byref(attn(**k)), o, o_lo, lse, ws, n, None)
+    bwd = lambda dq=o, dk=o, dv=o, ws=o, n=1 << 40, os=64, **k: lib.rtp_xattn_backward(C.byref(attn(**k)), o, o, o, o, 768, 256, os, dq, dk, dv, ws, n, None)
+    assert size() == 0 and size(1) > 0
+    assert fwd(b=0) == 0 and fwd(sq=0) == 0
+    for bad in (dict(b=-1), dict(sq=-1), dict(sk=-1), dict(hq=3), dict(hkv=0), dict(d=0), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+                dict(scale=float("inf")), dict(sk=2 ** 30 + 1), dict(sq=2 ** 30, hq=64)):
+        assert fwd(**bad) == SHAPE and size(**bad) == -1 and bwd(**bad) == SHAPE
+    for bad in (dict(d=12), dict(d=136), dict(dtype=0), dict(dtype=3)):
+        assert fwd(**bad) == UNSUPPORTED and bwd(**bad) == UNSUPPORTED
+    for bad in (dict(q=4100), dict(q_hs=4), dict(k_ss=130), dict(v_bs=641)):
+        assert fwd(**bad) == ALIGN and bwd(**bad) == ALIGN
+    assert fwd(q=None) == SHAPE and fwd(k=None) == SHAPE and fwd(o_lo=o) == SHAPE and fwd(lse=o) == SHAPE
+    assert fwd(key_mask=4096, ws=None, n=0) == SHAPE                      # a mask needs a workspace
+    assert bwd(os=60) == ALIGN and bwd(ws=P(4112)) == ALIGN and bwd(n=8) == SHAPE and bwd(dk=None) == SHAPE and bwd(ws=None) == SHAPE
+    assert bwd(b=0) == SHAPE and bwd(sk=0) == SHAPE
+
+
+def test_workspace_is_sized_for_every_cut():
+    """The cut of the work depends on sizes alone; its partial results stay a fraction of what the pass reads and writes anyway or small."""
+    lib = _lib.load()
+    for b in (1, 3, 16):
+        for sq in (1, 15, 40, 700, 5000):
+            for sk in (0, 1, 64, 5000, 10 ** 6):
+                for hq, hkv in ((1, 1), (8, 2), (12, 12)):
+                    for back in (0, 1):
+                        n = lib.rtp_xattn_workspace_bytes(C.byref(attn(b=b, sq=sq, sk=sk, hq=hq, hkv=hkv)), back)
+                        assert 0 <= n < 2 ** 33
