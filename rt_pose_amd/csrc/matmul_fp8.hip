@@ -5,12 +5,14 @@
 // One v_mfma_f32_16x16x128_f8f6f4 contracts exactly one block of 128: its fp32 result, started from zero, is scaled by the block's factor and
 // added to the running fp32 sum, so the scales cost one multiply-add per result and block.  Rows of b are the instruction's rows and rows of
 // a its columns: a lane then holds four neighbouring n of one m.
-// Both operands of an instruction may take the 128 k in any common order, so a lane simply takes 32 consecutive bytes of its row.
+// Both operands of an instruction may take the 128 k in any common order: a lane takes two chunks of 16 bytes of its row, which ones is free.
 // The 8-bit matrix instructions (every shape alike) add groups of eight products at 14 bits: within a group a product loses what lies under
 // 2^-13 of the group's largest one; from there on sums are fp32.  On random operands that is 1.4e-5 of the result, below the rounding of a
 // bf16 (1.7e-3) or fp16 (2.1e-4) output.  An fp32 output takes the exact road instead: both operands widened to bf16 (every e4m3 value is one)
 // and the bf16 instruction, whose products are exact and whose sums are fp32, at half the rate.
 // Bytes from k on (a row's padding, or a whole chunk of the last block) may hold anything: they are masked to zero in BOTH operands.
+#include <type_traits>
+
 #include "rtp_prof.h"
 #include "token_common.h"
 
@@ -54,12 +56,12 @@ __device__ __forceinline__ f32x4 mfma128(const Frag16& a, const Frag16& b) {
   return r;
 }
 
-// this lane's 32 bytes of a block of 128 (k0 = first k of the block + 32 * (lane / 16)): zero from k on
-__device__ __forceinline__ i32x8 tail_mask(int k0, int k) {
+// this lane's 32 bytes of a block of 128, 16 from k0 on and 16 from k1 on: zero behind k
+__device__ __forceinline__ i32x8 tail_mask(int k0, int k1, int k) {
   i32x8 r;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int left = k - (k0 + 4 * i);
+    const int left = k - (i < 4 ? k0 + 4 * i : k1 + 4 * (i - 4));
     r[i] = left >= 4 ? -1 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1u);
   }
   return r;
@@ -79,78 +81,130 @@ __device__ __forceinline__ void store4(O* p, f32x4 v, int n) {
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// Waves of a workgroup share one tile of 16 n x 16 * MT m and split the blocks of k; their sums meet in LDS in wave order.  Operands go from
-// memory straight to registers: every byte of b is used by one wave alone.
-template <typename O, int MT, int W, bool SQUARE>
-__global__ __launch_bounds__(64 * W) void mm8_few_kernel(Mm8Params p) {
+// The eight waves of a workgroup share one tile of 16 * NT n x 16 * MT m and split the blocks of k; their sums meet in LDS in wave order.
+// Operands go from memory straight to registers, DEPTH blocks in flight.  Nothing is staged: a row of b is used by this workgroup alone, and the
+// rows of a are few enough to come from L2.
+#define MM8_FEW_WAVES 8
+template <typename O, int MT, int NT, int DEPTH, bool SQUARE>
+__global__ __launch_bounds__(64 * MM8_FEW_WAVES) void mm8_few_kernel(Mm8Params p) {
+  constexpr int W = MM8_FEW_WAVES;
   typedef typename FragOf<(sizeof(O) == 4)>::type Frag;
-  __shared__ f32x4 red[W][MT][64];
+  __shared__ f32x4 red[W / 2][MT * NT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int n0 = (blockIdx.x % (unsigned)p.tiles_n) * 16, m0 = (blockIdx.x / (unsigned)p.tiles_n) * (16 * MT);
-  const int nr = n0 + col < p.n ? n0 + col : p.n - 1;
-  const uint8_t* bp = p.b + nr * p.ldb;
-  const uint8_t* ap[MT];
-  const float* sap[MT];
+  const int n0 = (blockIdx.x % (unsigned)p.tiles_n) * (16 * NT), m0 = (blockIdx.x / (unsigned)p.tiles_n) * (16 * MT);
+  const uint8_t *ap[MT], *bp[NT];
+  const float *sap[MT], *sbp[SQUARE ? 1 : NT * 4];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int mr = m0 + i * 16 + col < p.m ? m0 + i * 16 + col : p.m - 1;
     ap[i] = p.a + mr * p.lda;
     sap[i] = p.sa + (long)mr * p.kb;
   }
-  f32x4 acc[MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto block = [&](int kb, bool tail) {
-    const int k0 = kb * 128 + g * 32;
-    const int o0 = tail && k0 >= p.k ? 0 : k0, o1 = tail && k0 + 16 >= p.k ? 0 : k0 + 16;
-    auto frag = [&](const uint8_t* row) {
-      const i32x4 lo = *(const i32x4*)(row + o0), hi = *(const i32x4*)(row + o1);
-      i32x8 r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      if (tail) r &= tail_mask(k0, p.k);
-      Frag f;
-      make_frag(f, r);
-      return f;
-    };
-    const Frag bf = frag(bp);
-    f32x4 sb;
-    if constexpr (SQUARE) {
-      const float s = p.sb[(long)(n0 >> 7) * p.kb + kb];
-      sb = f32x4{s, s, s, s};
-    } else {
+  for (int i = 0; i < NT; ++i) {
+    bp[i] = p.b + (n0 + i * 16 + col < p.n ? n0 + i * 16 + col : p.n - 1) * p.ldb;
+    if constexpr (!SQUARE) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sb[j] = p.sb[(long)(n0 + g * 4 + j < p.n ? n0 + g * 4 + j : p.n - 1) * p.kb + kb];
+      for (int j = 0; j < 4; ++j) {
+        const int nr = n0 + i * 16 + g * 4 + j;
+        sbp[i * 4 + j] = p.sb + (long)(nr < p.n ? nr : p.n - 1) * p.kb;
+      }
     }
+  }
+  if constexpr (SQUARE) sbp[0] = p.sb + (long)(n0 >> 7) * p.kb;      // 16 * NT divides 128: one block of n
+  f32x4 acc[NT][MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] += mfma128(bf, frag(ap[i])) * (sb * sap[i][kb]);
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // the blocks kb, kb + W, ... kb + (D - 1) W; one that is none (from `end` on) repeats a readable one with the factor zero
+  auto blocks = [&](int kb, int end, bool tail, auto depth) {
+    constexpr int D = decltype(depth)::value;
+    i32x8 av[D][MT], bv[D][NT];
+    float f[D][MT];
+    f32x4 sb[D][NT];
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      const int k = kb + u * W < end ? kb + u * W : end - 1;
+      const int k0 = k * 128 + g * 32;
+      const int o0 = tail && k0 >= p.k ? 0 : k0, o1 = tail && k0 + 16 >= p.k ? 0 : k0 + 16;
+      auto raw = [&](const uint8_t* row) {
+        const i32x4 lo = *(const i32x4*)(row + o0), hi = *(const i32x4*)(row + o1);
+        return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+#pragma unroll
+      for (int i = 0; i < NT; ++i) bv[u][i] = raw(bp[i]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) av[u][j] = raw(ap[j]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) f[u][j] = kb + u * W < end ? sap[j][k] : 0.f;
+      if constexpr (SQUARE) {
+        const float x = sbp[0][k];
+        sb[u][0] = f32x4{x, x, x, x};
+      } else {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) sb[u][i] = f32x4{sbp[i * 4][k], sbp[i * 4 + 1][k], sbp[i * 4 + 2][k], sbp[i * 4 + 3][k]};
+      }
+    }
+    i32x8 mask;
+    if (tail) mask = tail_mask(kb * 128 + g * 32, kb * 128 + g * 32 + 16, p.k);
+#pragma unroll
+    for (int u = 0; u < D; ++u) {
+      Frag af[MT];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) make_frag(af[j], tail ? av[u][j] & mask : av[u][j]);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        Frag bf;
+        make_frag(bf, tail ? bv[u][i] & mask : bv[u][i]);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] += mfma128(bf, af[j]) * (sb[u][SQUARE ? 0 : i] * f[u][j]);
+      }
+    }
   };
   const int full = p.k >> 7;
-  for (int kb = wave; kb < full; kb += W) block(kb, false);
-  if (full < p.kb && full % W == wave) block(full, true);
+  for (int kb = wave; kb < full; kb += W * DEPTH) blocks(kb, full, false, std::integral_constant<int, DEPTH>{});
+  if (full < p.kb && full % W == wave) blocks(full, p.kb, true, std::integral_constant<int, 1>{});
+  // halves of the waves meet until one is left
 #pragma unroll
-  for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
-  __syncthreads();
-  for (int i = wave; i < MT; i += W) {
-    f32x4 t = red[0][i][lane];
+  for (int o = W / 2; o > 0; o >>= 1) {
+    if (wave >= o && wave < 2 * o) {
 #pragma unroll
-    for (int w = 1; w < W; ++w) t += red[w][i][lane];
-    const int mr = m0 + i * 16 + col;
-    if (mr < p.m) store4((O*)p.out + mr * p.ldo + n0 + g * 4, t, p.n - n0 - g * 4);
+      for (int i = 0; i < NT * MT; ++i) red[wave - o][i][lane] = acc[i / MT][i % MT];
+    }
+    __syncthreads();
+    if (wave < o) {
+#pragma unroll
+      for (int i = 0; i < NT * MT; ++i) acc[i / MT][i % MT] += red[wave][i][lane];
+    }
+    __syncthreads();
+  }
+  if (wave > 0) return;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int mr = m0 + j * 16 + col;
+    if (mr < p.m) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) store4((O*)p.out + mr * p.ldo + n0 + i * 16 + g * 4, acc[i][j], p.n - (n0 + i * 16 + g * 4));
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
 // BM x BN per workgroup, WM x WN per wave.  Blocks of 128 k are staged by LDS-DMA (16 B a lane, no registers) into two buffers, the next
-// one while this one is multiplied: one barrier per block.  A row is 128 B in LDS, its 16-byte chunk c at slot c ^ ((row / 2) % 8): the 16
-// rows that a fragment read touches then lie in 16 different slots of the 256-byte bank row.
+// one while this one is multiplied: one barrier per block.  A row is 128 B in LDS, its 16-byte chunk c at slot c ^ ((row / 2) % 8), and lanes
+// of group g = lane / 16 read chunks g and g + 4.  A 16-byte LDS read goes by the lanes {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same of
+// the upper half: each of these sets then touches 16 different slots of the 256-byte bank row (chunks 2 g and 2 g + 1 instead: every read
+// two-way, half of the LDS cycles, 637 -> 621 us at 8192^3).
 template <typename O, int BM, int BN, int WM, int WN, bool SQUARE>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm8_tile_kernel(Mm8Params p) {
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel(Mm8Params p) {
   constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = WAVES * 64, MT = WM / 16, NT = WN / 16;
   constexpr int AI = BM * 8 / THREADS, BI = BN * 8 / THREADS;
-  typedef typename FragOf<(sizeof(O) == 4)>::type Frag;
-  constexpr int SCALES = BM + (SQUARE ? 0 : BN);          // floats per buffer
+  constexpr int SCALES = BM + (SQUARE ? 64 : BN);          // floats per buffer: sa of the rows; sb of the rows or of the tile's blocks of 128
   constexpr int BUF = (BM + BN) * 128 + SCALES * 4;
-  static_assert(SCALES % 64 == 0 && SCALES / 64 <= WAVES, "one wave instruction stages 64 scales");
+  typedef typename FragOf<(sizeof(O) == 4)>::type Frag;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -162,39 +216,46 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm8_tile_kernel(Mm
   const int m0 = (int)(s0 + in % sm) * BM, n0 = (int)(in / sm) * BN;
   const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
 
-  const uint8_t *src[AI + BI];
+  // staging: 32-bit offsets from the tile's first row; rows behind the last one repeat it
+  const uint8_t *ab = p.a + (long)m0 * p.lda, *bb = p.b + (long)n0 * p.ldb;
+  int src[AI + BI];
 #pragma unroll
   for (int i = 0; i < AI + BI; ++i) {
     const int item = (i < AI ? i : i - AI) * THREADS + threadIdx.x, row = item >> 3;
     const int chunk = (item & 7) ^ ((row >> 1) & 7);
     if (i < AI)
-      src[i] = p.a + (long)(m0 + row < p.m ? m0 + row : p.m - 1) * p.lda + chunk * 16;
+      src[i] = (m0 + row < p.m ? row : p.m - 1 - m0) * (int)p.lda + chunk * 16;
     else
-      src[i] = p.b + (long)(n0 + row < p.n ? n0 + row : p.n - 1) * p.ldb + chunk * 16;
+      src[i] = (n0 + row < p.n ? row : p.n - 1 - n0) * (int)p.ldb + chunk * 16;
   }
-  const float* ssrc = nullptr;
-  if (wave < SCALES / 64) {
-    const int i = threadIdx.x;   // < SCALES
+  const float* ssrc[(SCALES / 64 + WAVES - 1) / WAVES];
+#pragma unroll
+  for (int u = 0; u < (SCALES / 64 + WAVES - 1) / WAVES; ++u) {
+    const int i = u * THREADS + threadIdx.x, nb = (p.n - 1) >> 7;
     if (i < BM)
-      ssrc = p.sa + (long)(m0 + i < p.m ? m0 + i : p.m - 1) * p.kb;
+      ssrc[u] = p.sa + (long)(m0 + i < p.m ? m0 + i : p.m - 1) * p.kb;
+    else if (SQUARE)
+      ssrc[u] = p.sb + (long)((n0 >> 7) + i - BM < nb ? (n0 >> 7) + i - BM : nb) * p.kb;
     else
-      ssrc = p.sb + (long)(n0 + i - BM < p.n ? n0 + i - BM : p.n - 1) * p.kb;
+      ssrc[u] = p.sb + (long)(n0 + i - BM < p.n ? n0 + i - BM : p.n - 1) * p.kb;
   }
   typedef __attribute__((address_space(3))) void lds_void;
   typedef __attribute__((address_space(1))) void glb_void;
-  auto stage = [&](int kb, int buf) {
-    const bool tail = (kb + 1) * 128 > p.k;
-#pragma unroll
-    for (int i = 0; i < AI + BI; ++i) {
-      const int item = (i < AI ? i : i - AI) * THREADS + threadIdx.x;
-      const int chunk = (item & 7) ^ ((item >> 4) & 7);
+  constexpr int PIECES = AI + BI + 1;         // of a block's staging: 16-byte loads of the operands, and the scales
+  auto stage = [&](int kb, int buf, int i) {
+    if (i < AI + BI) {
+      const bool tail = (kb + 1) * 128 > p.k;
+      const int chunk = ((threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7)) * 16;   // THREADS is a multiple of 128: the same in every step
       // a chunk behind k: any readable one in its place, the fragment's mask makes it zero
-      const int off = tail && kb * 128 + chunk * 16 >= p.k ? -chunk * 16 : kb * 128;
-      __builtin_amdgcn_global_load_lds((const glb_void*)(src[i] + off),
+      const int off = tail && kb * 128 + chunk >= p.k ? src[i] - chunk - kb * 128 : src[i];
+      __builtin_amdgcn_global_load_lds((const glb_void*)((i < AI ? ab : bb) + (long)kb * 128 + off),
                                        (lds_void*)(lds + buf * BUF + (i < AI ? i * THREADS * 16 : BM * 128 + (i - AI) * THREADS * 16) + wave * 1024), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < (SCALES / 64 + WAVES - 1) / WAVES; ++u)
+        if (u * WAVES + wave < SCALES / 64)
+          __builtin_amdgcn_global_load_lds((const glb_void*)(ssrc[u] + kb), (lds_void*)(lds + buf * BUF + (BM + BN) * 128 + (u * WAVES + wave) * 256), 4, 0, 0);
     }
-    if (wave < SCALES / 64)
-      __builtin_amdgcn_global_load_lds((const glb_void*)(ssrc + kb), (lds_void*)(lds + buf * BUF + (BM + BN) * 128 + wave * 256), 4, 0, 0);
   };
 
   f32x4 acc[NT][MT];
@@ -203,13 +264,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm8_tile_kernel(Mm
 #pragma unroll
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int sw = (col >> 1) & 7;
-  const int off0 = col * 128 + ((2 * g) ^ sw) * 16, off1 = col * 128 + ((2 * g + 1) ^ sw) * 16;
-  auto compute = [&](int kb, int buf, bool tail) {
+  const int off0 = col * 128 + (g ^ sw) * 16, off1 = col * 128 + ((g + 4) ^ sw) * 16;
+  auto compute = [&](int kb, int buf, bool tail, bool more) {
     const uint8_t* la = lds + buf * BUF + wm * 128;
     const uint8_t* lb = lds + buf * BUF + BM * 128 + wn * 128;
     const float* ls = (const float*)(lds + buf * BUF + (BM + BN) * 128);
     i32x8 mask;
-    if (tail) mask = tail_mask(kb * 128 + g * 32, p.k);
+    if (tail) mask = tail_mask(kb * 128 + g * 16, kb * 128 + g * 16 + 64, p.k);
     auto frag = [&](const uint8_t* t) {
       const i32x4 lo = *(const i32x4*)(t + off0), hi = *(const i32x4*)(t + off1);
       i32x8 r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
@@ -220,37 +281,60 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm8_tile_kernel(Mm
     };
     Frag af[MT];
     float f[MT];
-    float sbu = 1.f;
-    if constexpr (SQUARE) sbu = p.sb[(long)((n0 + wn < p.n ? n0 + wn : p.n - 1) >> 7) * p.kb + kb];
+    const float sbu = SQUARE ? ls[BM + (wn >> 7)] : 1.f;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       af[j] = frag(la + j * 2048);
       f[j] = ls[wm + j * 16 + col] * sbu;
     }
+    // step i multiplies, while the results of step i - 1 are scaled and added and the fragment of step i + 2 is read
+    constexpr int PER = 4;
+    Frag bf = frag(lb), b1 = frag(lb + 2048);
+    f32x4 r[MT], sb4 = {1.f, 1.f, 1.f, 1.f};
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const Frag bf = frag(lb + i * 2048);
-      f32x4 sb4;
-      if constexpr (!SQUARE) sb4 = *(const f32x4*)(ls + BM + wn + i * 16 + g * 4);
+    for (int i = 0; i <= NT; ++i) {
+      if (more) {               // the next block's staging, spread over the first steps (at once in front of them: 565 us at 8192^3, so 510)
+#pragma unroll
+        for (int u = i * PER; u < (i + 1) * PER && u < PIECES; ++u) stage(kb + 1, (kb + 1) & 1, u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      Frag next = b1;
+      if (i + 2 < NT) next = frag(lb + (i + 2) * 2048);
+      f32x4 sn = sb4;
+      if (!SQUARE && i < NT) sn = *(const f32x4*)(ls + BM + wn + i * 16 + g * 4);
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const f32x4 r = mfma128(bf, af[j]);
-        if constexpr (SQUARE) acc[i][j] += r * f[j];
-        else acc[i][j] += r * (sb4 * f[j]);
+        f32x4 t = r[j];
+        if (i < NT) r[j] = mfma128(bf, af[j]);
+        if (i > 0) {
+          if constexpr (SQUARE) acc[i - 1][j] += t * f[j];
+          else acc[i - 1][j] += t * (sb4 * f[j]);
+        }
       }
+      bf = b1;
+      b1 = next;
+      sb4 = sn;
+      // the order of issue: the fragment's reads, then one matrix instruction and one earlier result's multiply-adds in turn
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x008, sizeof(O) == 4 ? 4 : 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, SQUARE ? 4 : 8, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  stage(0, 0);
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) stage(0, 0, i);
   int kb = 0;
   for (; kb + 1 < p.kb; ++kb) {
     __syncthreads();          // this block has landed (the barrier waits for the DMA), the other buffer has been read
-    stage(kb + 1, (kb + 1) & 1);
-    compute(kb, kb & 1, false);
+    compute(kb, kb & 1, false, true);
   }
   __syncthreads();
-  if (p.k & 127) compute(kb, kb & 1, true);
-  else compute(kb, kb & 1, false);
+  if (p.k & 127) compute(kb, kb & 1, true, false);
+  else compute(kb, kb & 1, false, false);
 
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
@@ -270,23 +354,27 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void mm8_tile_kernel(Mm
 template <typename O, bool SQUARE>
 static int mm8_launch(Mm8Params p, hipStream_t st) {
   const long tiles128 = (long)rtp_div_up(p.m, 128) * rtp_div_up(p.n, 128);
-  if (p.m <= 64 || tiles128 < 128) {
-    p.tiles_n = rtp_div_up(p.n, 16);
-#define MM8_FEW(MT)                                                                                                              \
-  do {                                                                                                                           \
-    p.tiles_m = rtp_div_up(p.m, 16 * MT);                                                                                        \
-    hipLaunchKernelGGL((mm8_few_kernel<O, MT, 8, SQUARE>), dim3((unsigned)(p.tiles_n * p.tiles_m)), dim3(512), 0, st, p);        \
-  } while (0)
-    if (p.m <= 16) MM8_FEW(1);
-    else if (p.m <= 32) MM8_FEW(2);
-    else MM8_FEW(4);
-#undef MM8_FEW
-    RTP_CHECK_LAUNCH();
-    return RTP_OK;
+  // Up to 64 rows, or where 128 x 128 tiles would leave most CUs without one.  m x 4096 x 4096: m = 128 (32 tiles) 17.9 us against 23.4 in tiles,
+  // m = 300 (96 tiles) 39.4 against 23.6; 64 x 8192 x 8192 32.5 against 46.
+  if (p.m <= 64 || tiles128 < 48) {
+    // as many n per workgroup as leave one for each CU: b is then read once, a from L2 less often
+    const int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
+    const long rows = rtp_div_up(p.m, 16 * mt);
+    const int nt = rows * rtp_div_up(p.n, 64) >= 256 ? 4 : rows * rtp_div_up(p.n, 32) >= 256 ? 2 : 1;
+    p.tiles_n = rtp_div_up(p.n, 16 * nt);
+    p.tiles_m = (int)rows;
+    auto few = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * p.tiles_n)), dim3(64 * MM8_FEW_WAVES), 0, st, p);
+      RTP_CHECK_LAUNCH();
+      return RTP_OK;
+    };
+    if (mt == 1) return nt == 4 ? few(mm8_few_kernel<O, 1, 4, 2, SQUARE>) : nt == 2 ? few(mm8_few_kernel<O, 1, 2, 4, SQUARE>) : few(mm8_few_kernel<O, 1, 1, 4, SQUARE>);
+    if (mt == 2) return nt == 4 ? few(mm8_few_kernel<O, 2, 4, 2, SQUARE>) : nt == 2 ? few(mm8_few_kernel<O, 2, 2, 2, SQUARE>) : few(mm8_few_kernel<O, 2, 1, 4, SQUARE>);
+    return nt == 4 ? few(mm8_few_kernel<O, 4, 4, 1, SQUARE>) : nt == 2 ? few(mm8_few_kernel<O, 4, 2, 2, SQUARE>) : few(mm8_few_kernel<O, 4, 1, 2, SQUARE>);
   }
   const long tiles256 = (long)rtp_div_up(p.m, 256) * rtp_div_up(p.n, 256);
   auto go = [&](auto kernel, int bm, int bn, int threads, bool* once) {
-    const int bytes = 2 * ((bm + bn) * 128 + (bm + (SQUARE ? 0 : bn)) * 4);
+    const int bytes = 2 * ((bm + bn) * 128 + (bm + (SQUARE ? 64 : bn)) * 4);
     if (rtp_once_per_device(once) && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
       return RTP_ERR_LAUNCH;
     p.tiles_m = rtp_div_up(p.m, bm);
@@ -296,7 +384,13 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     return RTP_OK;
   };
   static bool once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES];
-  if (tiles256 >= 200) return go(mm8_tile_kernel<O, 256, 256, 64, 128, SQUARE>, 256, 256, 512, once256);
+  // 256 x 256 halves what is staged per product and wins where the sum is long and its tiles fill whole rounds of the 256 CUs (8192^3: 505 us
+  // against 580, 4096^3: 72 against 77); 128 x 128, two workgroups to a CU, where one's start and end hide behind the other's sum
+  // (163840 x 256 x 384: 40 us against 57, x 1024: 71 against 87).  The exact road needs the registers of the small tile.
+  if constexpr (sizeof(O) == 2) {
+    const long rounds = (tiles256 + 255) / 256;
+    if (p.kb >= 16 && tiles256 >= 256 && tiles256 * 5 >= rounds * 256 * 4) return go(mm8_tile_kernel<O, 256, 256, 64, 128, SQUARE>, 256, 256, 512, once256);
+  }
   return go(mm8_tile_kernel<O, 128, 128, 64, 64, SQUARE>, 128, 128, 256, once128);
 }
 
@@ -306,7 +400,7 @@ extern "C" int rtp_matmul_fp8(const void* a, long lda, const float* sa, const vo
   if (m == 0 || n == 0) return RTP_OK;
   if (!a || !sa || !b || !sb || !out) return RTP_ERR_SHAPE;
   const long need = ((long)k + 15) & ~15L;
-  if ((m > 1 && lda < need) || (n > 1 && ldb < need)) return RTP_ERR_SHAPE;
+  if ((m > 1 && lda < need) || (n > 1 && ldb < need) || lda > (1L << 22) || ldb > (1L << 22)) return RTP_ERR_SHAPE;   // tiles index 32 bits
   if (((size_t)a & 15) || ((size_t)b & 15) || (lda & 15) || (ldb & 15)) return RTP_ERR_ALIGN;
   if ((long)rtp_div_up(m, 16) * rtp_div_up(n, 16) >= (1L << 31)) return RTP_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;

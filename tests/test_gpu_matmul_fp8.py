@@ -54,7 +54,8 @@ def check(out, a, sa, b, sb, square):
 
 
 SIZES = [(1, 1, 1), (1, 16, 128), (4, 130, 1000), (16, 256, 129), (17, 33, 16), (31, 500, 2048), (33, 128, 384), (64, 100, 777), (65, 129, 640),
-         (127, 1000, 130), (300, 200, 1030), (1500, 1400, 256), (2000, 1111, 400), (1411, 1600, 127), (4100, 3500, 300), (3584, 4096, 1000)]
+         (127, 1000, 130), (300, 200, 1030), (1500, 1400, 256), (2000, 1111, 400), (1411, 1600, 127), (4100, 3500, 300), (3584, 4096, 1000),
+         (5, 16400, 300), (20, 16400, 1100), (60, 16390, 260), (9, 8200, 520), (30, 8200, 300), (50, 8200, 700), (4000, 4090, 2050)]   # every cut of n, the large tile
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)
