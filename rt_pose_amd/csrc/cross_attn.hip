@@ -15,6 +15,7 @@
 // (ds_read_b64_tr_b16) in that same order.  p never leaves the registers.  dq works the same way; dk / dv with rows and keys exchanged.
 // Operands of 16 bits, everything else fp32: p and ds are rounded once to 16 bits for their second product (2^-9 of each, averaged over the
 // keys), the sums they enter are fp32.
+#include <stdlib.h>
 #include <type_traits>
 
 #include "rtp_prof.h"
@@ -22,10 +23,12 @@
 
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4_xa;
-typedef __attribute__((address_space(3))) void lds_void_xa;
-typedef __attribute__((address_space(1))) void glb_void_xa;
+typedef __attribute__((address_space(3))) uint8_t lds_u8_xa;
+typedef __attribute__((address_space(4))) unsigned cst_u32_xa;   // read-only for the whole launch: uniform addresses become scalar loads
 
 __device__ __attribute__((aligned(16))) bf16_t g_zero_line_xa[8];   // what masked rows and columns behind the head's width are staged from
+
+__device__ float g_inf_xa = INFINITY;
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
@@ -33,6 +36,16 @@ __device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __
 template <typename T> struct Vec8;
 template <> struct Vec8<bf16_t> { typedef bf16x8 type; };
 template <> struct Vec8<_Float16> { typedef f16x8 type; };
+
+// sixteen fp32 values of a lane as the second operands of two products; with LO what their rounding left over follows in two more.  Where few rows
+// leave the matrix unit idle (KW = 4) p and ds go in as both halves: nothing of them is lost then.
+template <typename T, bool LO> struct XaSecond {
+  typename Vec8<T>::type v[LO ? 4 : 2];
+  __device__ __forceinline__ void set(int i, float x) {
+    v[i >> 3][i & 7] = (T)x;
+    if constexpr (LO) v[2 + (i >> 3)][i & 7] = (T)(x - (float)(T)x);
+  }
+};
 
 struct XaParams {
   const void *q, *k, *v, *d_o;
@@ -50,23 +63,35 @@ struct XaParams {
 };
 
 // Workgroup -> (tile, unit): all tiles of a unit run on one XCD (workgroups go round the 8 XCDs), so that a unit's k and v stay in one L2.
-__device__ __forceinline__ bool xa_place(const XaParams& p, int& tile, int& bh, int& split) {
+// Batch entries with more keys come first (up to 64 entries: each lane ranks one): the last workgroups to start are then the short ones.
+__device__ __forceinline__ bool xa_place(const XaParams& p, int& tile, int& b, int& hk, int& split) {
   const unsigned j = blockIdx.x >> 3, unit = (j / (unsigned)p.tiles) * 8 + (blockIdx.x & 7);
   tile = j % (unsigned)p.tiles;
   if (unit >= (unsigned)p.units) return false;
-  bh = unit / (unsigned)p.nsplit;
+  const int bh = unit / (unsigned)p.nsplit;
   split = unit % (unsigned)p.nsplit;
+  b = bh / p.hkv;
+  hk = bh % p.hkv;
+  if (p.lens && p.b > 1 && p.b <= 64) {
+    const int lane = threadIdx.x & 63, mine = lane < p.b ? p.lens[lane] : 0;
+    int rank = 0;
+    for (int i = 0; i < p.b; ++i) {
+      const int other = __builtin_amdgcn_readlane(mine, i);
+      rank += other > mine || (other == mine && i < lane);
+    }
+    b = __builtin_ctzll(__ballot(lane < p.b && rank == b));
+  }
   return true;
 }
 
 __device__ __forceinline__ int xa_len(const XaParams& p, int b) {
   if (!p.lens) return p.sk;
-  const int n = p.lens[b];
+  const int n = (int)((const cst_u32_xa*)p.lens)[b];
   return n < 0 ? 0 : n > p.sk ? p.sk : n;
 }
 // bits of the 32 keys from key0 on
 __device__ __forceinline__ unsigned xa_word(const XaParams& p, int b, int len, int key0) {
-  if (p.bits) return p.bits[(long)b * p.words + (key0 >> 5)];
+  if (p.bits) return ((const cst_u32_xa*)p.bits)[(long)b * p.words + (key0 >> 5)];
   const int n = len - key0;
   return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
 }
@@ -108,18 +133,66 @@ __device__ __forceinline__ V xa_frag_tr(const uint8_t* img, int lo, int hi) {
   return __builtin_bit_cast(V, r);
 }
 
-// Stage ROWS rows of `src` (row r at src + off(r), valid where ok(r)) by LDS-DMA: 256 threads, 16 B each and step, no registers for the data.
-template <int DT, int ROWS, typename T, typename Off, typename Ok>
-__device__ __forceinline__ void xa_stage(uint8_t* img, const T* src, int d, Off off, Ok ok) {
-  constexpr int CH = XaImg<DT>::CH, STEPS = ROWS * CH / 256;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int item = i * 256 + threadIdx.x, r = item / CH, c = (item % CH) ^ XaImg<DT>::swz(r);
-    const void* a = ok(r) && c * 8 < d ? (const void*)(src + off(r) + c * 8) : (const void*)g_zero_line_xa;
-    __builtin_amdgcn_global_load_lds((const glb_void_xa*)a, (lds_void_xa*)(img + i * 4096 + wave * 1024), 16, 0, 0);
-  }
+// Staging by LDS-DMA: 256 threads, 16 B each and step, no registers for the data.  Step i brings rows i * 256 / CH + thread / CH.
+template <int DT>
+__device__ __forceinline__ int xa_chunk() {      // this thread's column chunk: the same in every step (swz has period 16, steps are 16 rows or more)
+  constexpr int CH = XaImg<DT>::CH;
+  return (int)(threadIdx.x % CH) ^ XaImg<DT>::swz(threadIdx.x / CH);
 }
+// The transfers are written out: from the builtin the compiler knows that LDS is written, and waits for ALL of them in front of every
+// transposing read.  Nothing is returned to registers; xa_landed() is what orders them.
+__device__ __forceinline__ unsigned xa_m0(const uint8_t* img, int bytes) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return __builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_u8_xa*)img + bytes + wave * 1024);
+}
+__device__ __forceinline__ void xa_dma(uint8_t* img, int step, const void* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(xa_m0(img, step * 4096)), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void xa_dma(uint8_t* img, int step, const void* base, unsigned off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(xa_m0(img, step * 4096)), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void xa_dma4(uint8_t* lds, const void* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane((unsigned)(size_t)(lds_u8_xa*)lds)), "v"(src)
+               : "memory", "m0");
+}
+// Which rows of an image a thread brings, and their byte offsets from the first one.  Where every row and column of a tile counts (most tiles)
+// an access is a uniform address and one 32-bit offset a lane; otherwise each lane picks its row or the line of zeros.
+template <int DT, typename T>
+struct XaLoader {
+  static constexpr int CH = XaImg<DT>::CH, ROWS = 256 / CH;
+  int r, c;
+  bool col;
+  __device__ __forceinline__ XaLoader(int d) : r(threadIdx.x / CH), c(xa_chunk<DT>() * 8), col(c < d) {}
+  // keys: bit of w for each
+  template <int BK>
+  __device__ __forceinline__ void keys(uint8_t* img, const T* src, long ss, unsigned off, bool whole, const unsigned (&w)[BK / 32]) const {
+#pragma unroll
+    for (int i = 0; i < BK / ROWS; ++i) {
+      const char* at = (const char*)(src + (long)(i * ROWS) * ss);
+      if (whole) {
+        xa_dma(img, i, at, off);
+      } else {
+        const unsigned word = CH == 4 ? (threadIdx.x < 128 ? w[2 * i] : w[2 * i + 1]) : w[i * ROWS / 32];
+        xa_dma(img, i, col && ((word >> ((i * ROWS + r) & 31)) & 1u) ? at + off : (const char*)g_zero_line_xa);
+      }
+    }
+  }
+  // query rows r0 .. r0 + BR - 1; `even`: the group divides a step's rows, so that a step is a whole number of tokens
+  template <int BR>
+  __device__ __forceinline__ void rows(uint8_t* img, const XaParams& p, const T* src, long ss, long hs, unsigned off, bool even, bool whole, int r0) const {
+#pragma unroll
+    for (int i = 0; i < BR / ROWS; ++i) {
+      const int first = r0 + i * ROWS;
+      const char* at = (const char*)(src + (even ? (long)(first / p.grp) * ss : 0L));
+      if (whole) {
+        xa_dma(img, i, at, off);
+      } else {
+        const char* mine = even ? at + off : (const char*)(src + xa_row_off(p, first + r, ss, hs) + c);
+        xa_dma(img, i, col && first + r < p.rows ? mine : (const char*)g_zero_line_xa);
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ float xa_halves_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -144,25 +217,103 @@ __device__ __forceinline__ void xa_load_row(typename Vec8<T>::type (&f)[2 * DT],
 #define XA_M0 (-3.402823466e38f)
 #define XA_SLACK 8.0f   // the running maximum moves only when it is exceeded by 2^8: p stays below 2^8, and most tiles rescale nothing
 
-// ------------------------------------------------------------------------------------------------ forward
+// ------------------------------------------------------------------------------------------------ the loop over keys
 // Four waves: 4 / KW groups of 32 rows, and KW waves that share rows and split each tile of keys (few rows: the keys are the work).
-// Tiles of BK keys go through two LDS buffers, the next one on its way while this one is used: one barrier a tile.
-template <int KW> struct XaKeys { static constexpr int BK = KW == 4 ? 128 : 64, SUB = BK / 32 / KW; };
+// Tiles of BK keys go round NBUF LDS buffers: while one is used, the next NBUF - 1 are on their way, and the barrier in front of a tile waits
+// for that tile's transfers alone (they complete in order, PER of them a wave and tile).  Three buffers where they leave room for the waves
+// that the registers allow.  The mask's words are scalar loads, one tile further ahead, so that nothing else counts as a vector access.
+template <int DT, int KW> struct XaKeys {
+  static constexpr int BK = KW == 4 ? 128 : 64, SUB = BK / 32 / KW, NW = BK / 32, IMG = BK * XaImg<DT>::PITCH;
+  static constexpr int NBUF = DT == 1 ? 3 : 2, BYTES = NBUF * 2 * IMG;
+};
+// The compiler does not know of the transfers: whatever it loaded before the loop has to have arrived before the loop, or it would wait for it
+// inside, and with it for all transfers.
+__device__ __forceinline__ void xa_settle() { __builtin_amdgcn_s_waitcnt(0x0F70); }   // vmcnt(0)
+// everything but the newest N vector accesses of this wave is done, and its LDS reads; then all waves
+template <int N>
+__device__ __forceinline__ void xa_landed() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-template <typename T, int DT, int KW>
-__global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaParams p) {
-  typedef typename Vec8<T>::type V;
-  constexpr int BK = XaKeys<KW>::BK, SUB = XaKeys<KW>::SUB, IMG = BK * XaImg<DT>::PITCH;
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int tile, bh, split;
-  if (!xa_place(p, tile, bh, split)) return;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = bh / p.hkv, hk = bh % p.hkv, h = lane >> 5;
-  const int kw = wave % KW, r0 = tile * (128 / KW) + (wave / KW) * 32, r = r0 + (lane & 31);
+template <typename T, int DT, int KW, typename F>
+__device__ __forceinline__ void xa_over_keys(const XaParams& p, uint8_t* lds, int b, int hk, int split, bool busy, F compute) {
+  typedef XaKeys<DT, KW> K;
+  constexpr int BK = K::BK, NW = K::NW, NBUF = K::NBUF, IMG = K::IMG, PER = 2 * BK / XaLoader<DT, T>::ROWS;
   const int len = xa_len(p, b), nt = (len + BK - 1) / BK;
   const int t0 = (int)((long)nt * split / p.nsplit), t1 = (int)((long)nt * (split + 1) / p.nsplit);
+  if (t0 >= t1) return;
   const T* kp = (const T*)p.k + (long)b * p.k_bs + (long)hk * p.k_hs;
   const T* vp = (const T*)p.v + (long)b * p.v_bs + (long)hk * p.v_hs;
+  const XaLoader<DT, T> ld(p.d);
+  const unsigned k_off = (unsigned)(ld.r * (int)p.k_ss + ld.c) * 2u, v_off = (unsigned)(ld.r * (int)p.v_ss + ld.c) * 2u;
+  const bool full = p.d == XaImg<DT>::CH * 8;
+  unsigned w[NBUF + 1][NW];           // of the tiles t, t + 1, ...
+  auto words = [&](int t, unsigned (&x)[NW]) {
+#pragma unroll
+    for (int i = 0; i < NW; ++i) x[i] = t < t1 ? xa_word(p, b, len, t * BK + i * 32) : 0u;
+  };
+  auto stage = [&](int t, uint8_t* at, const unsigned (&x)[NW]) {
+    unsigned all = full ? ~0u : 0u;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) all &= x[i];
+    if (all == ~0u) {
+      ld.template keys<BK>(at, kp + (long)t * BK * p.k_ss, p.k_ss, k_off, true, x);
+      ld.template keys<BK>(at + IMG, vp + (long)t * BK * p.v_ss, p.v_ss, v_off, true, x);
+    } else {
+      ld.template keys<BK>(at, kp + (long)t * BK * p.k_ss, p.k_ss, k_off, false, x);
+      ld.template keys<BK>(at + IMG, vp + (long)t * BK * p.v_ss, p.v_ss, v_off, false, x);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i <= NBUF; ++i) words(t0 + i, w[i]);
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i)
+    if (t0 + i < t1) stage(t0 + i, lds + i * 2 * IMG, w[i]);
+  xa_settle();
+  int use = 0, fill = (NBUF - 1) * 2 * IMG;
+  for (int t = t0; t < t1; ++t) {
+    if (NBUF == 3 && t + 1 < t1) xa_landed<PER>();
+    else xa_landed<0>();
+    if (t + NBUF - 1 < t1) stage(t + NBUF - 1, lds + fill, w[NBUF - 1]);
+    if (busy) compute(lds + use, lds + use + IMG, w[0]);
+    use = use + 2 * IMG == K::BYTES ? 0 : use + 2 * IMG;
+    fill = fill + 2 * IMG == K::BYTES ? 0 : fill + 2 * IMG;
+#pragma unroll
+    for (int j = 0; j < NBUF; ++j)
+#pragma unroll
+      for (int i = 0; i < NW; ++i) w[j][i] = w[j + 1][i];
+    words(t + NBUF + 1, w[NBUF]);
+  }
+}
+// scores of keys that do not count: minus infinity
+__device__ __forceinline__ void xa_mask(f32x16& s, unsigned w, int h) {
+  const unsigned wl = w >> (4 * h);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = (wl >> (8 * (i / 4) + i % 4)) & 1u ? s[i] : -INFINITY;
+}
+// this wave's words of a tile
+template <int KW, int NW>
+__device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigned (&m)[NW / KW]) {
+#pragma unroll
+  for (int u = 0; u < NW / KW; ++u) {
+    m[u] = w[u];
+#pragma unroll
+    for (int k = 1; k < KW; ++k) m[u] = kw == k ? w[k * (NW / KW) + u] : m[u];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// waves for each SIMD that the registers and LDS allow
+template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3; };
+
+template <typename T, int DT, int KW>
+__global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaParams p) {
+  typedef typename Vec8<T>::type V;
+  constexpr int SUB = XaKeys<DT, KW>::SUB, NW = XaKeys<DT, KW>::NW, PITCH = XaImg<DT>::PITCH;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int tile, b, hk, split;
+  if (!xa_place(p, tile, b, hk, split)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bh = b * p.hkv + hk, h = lane >> 5;
+  const int kw = wave % KW, r0 = tile * (128 / KW) + (wave / KW) * 32, r = r0 + (lane & 31);
   const XaAddr<DT> ad(lane);
 
   V qf[2 * DT];
@@ -174,71 +325,66 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaParams p) {
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = XA_M0, l = 0.f;
 
-  auto stage = [&](int t, int buf) {
-    unsigned w[BK / 32];
+  xa_over_keys<T, DT, KW>(p, lds, b, hk, split, r0 < p.rows, [&](const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+    unsigned w[SUB], any = 0, all = ~0u;
+    xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
-    for (int i = 0; i < BK / 32; ++i) w[i] = xa_word(p, b, len, t * BK + i * 32);
-    auto ok = [&](int row) {
-      unsigned x = w[0];
+    for (int u = 0; u < SUB; ++u) any |= w[u], all &= w[u];
+    if (any == 0) return;
+    ki += kw * SUB * 32 * PITCH;
+    vi += kw * SUB * 32 * PITCH;
+    f32x16 s[SUB];
 #pragma unroll
-      for (int i = 1; i < BK / 32; ++i) x = (row >> 5) == i ? w[i] : x;
-      return ((x >> (row & 31)) & 1u) != 0;
-    };
-    xa_stage<DT, BK>(lds + buf * 2 * IMG, kp + (long)t * BK * p.k_ss, p.d, [&](int row) { return (long)row * p.k_ss; }, ok);
-    xa_stage<DT, BK>(lds + buf * 2 * IMG + IMG, vp + (long)t * BK * p.v_ss, p.d, [&](int row) { return (long)row * p.v_ss; }, ok);
-  };
-  auto compute = [&](int t, int buf) {
-    const uint8_t *ki = lds + buf * 2 * IMG, *vi = ki + IMG;
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+    for (int st = 0; st < 2 * DT; ++st)
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) s[u] = mfma32(xa_frag<V>(ki + u * 32 * PITCH, ad.row[st]), qf[st], s[u]);
+    if (all != ~0u) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) xa_mask(s[u], w[u], h);
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+    mx = xa_halves_max(mx) * p.scale_log2;
+    if (__any(mx > m + XA_SLACK)) {
+      const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= a;
+#pragma unroll
+      for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t2][i] *= a;
+    }
+    XaSecond<T, KW == 4> pb[SUB];
+    float part[SUB];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
-      const int sub = kw * SUB + u;
-      const unsigned w = xa_word(p, b, len, t * BK + sub * 32);
-      if (w == 0) continue;
-      f32x16 s;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.f;
-#pragma unroll
-      for (int st = 0; st < 2 * DT; ++st) s = mfma32(xa_frag<V>(ki + sub * 32 * XaImg<DT>::PITCH, ad.row[st]), qf[st], s);
-      if (w != ~0u) {
-        const unsigned wl = w >> (4 * h);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (wl >> (8 * (i / 4) + i % 4)) & 1u ? s[i] : -INFINITY;
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-      mx = xa_halves_max(mx) * p.scale_log2;
-      if (__any(mx > m + XA_SLACK)) {
-        const float mn = fmaxf(m, mx), a = exp2f(m - mn);
-        m = mn;
-        l *= a;
-#pragma unroll
-        for (int t2 = 0; t2 < DT; ++t2)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[t2][i] *= a;
-      }
-      V pb[2];
+      part[u] = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(s[i] * p.scale_log2 - m);
-        l += e;
-        pb[i >> 3][i & 7] = (T)e;
+        const float e = __builtin_amdgcn_exp2f(s[u][i] * p.scale_log2 - m);
+        part[u] += e;
+        pb[u].set(i, e);
       }
+      l += part[u];
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int t2 = 0; t2 < DT; ++t2)
-          o[t2] = mfma32(xa_frag_tr<V>(vi + (sub * 32 + c * 16) * XaImg<DT>::PITCH, ad.tr[t2][0], ad.tr[t2][1]), pb[c], o[t2]);
-    }
-  };
-  if (t0 < t1) {
-    stage(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-      __syncthreads();
-      if (t + 1 < t1) stage(t + 1, (t + 1 - t0) & 1);
-      if (r0 < p.rows) compute(t, (t - t0) & 1);
-    }
-  }
+        for (int t2 = 0; t2 < DT; ++t2) {
+          const V f = xa_frag_tr<V>(vi + (u * 32 + c * 16) * PITCH, ad.tr[t2][0], ad.tr[t2][1]);
+          if constexpr (KW == 4) o[t2] = mfma32(f, pb[u].v[2 + c], o[t2]);
+          o[t2] = mfma32(f, pb[u].v[c], o[t2]);
+        }
+  });
   l = xa_halves_sum(l);
   if constexpr (KW > 1) {       // waves of one row group meet in LDS, added in wave order
     __syncthreads();
@@ -307,32 +453,47 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XaParams p) {
   }
 }
 
-// o of a row = sum over splits of 2^(L_split - L) o_split.  16 lanes a row, 8 columns each.
+// Partial results of the splits, joined by one wave per row: four groups of 16 lanes (8 columns each) take every fourth split, so that the
+// loads of a row are under way together, and the groups are added in a fixed order.
+__device__ __forceinline__ float xa_groups_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// o of a row = sum over splits of 2^(L_split - L) o_split
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XaParams p) {
-  const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int c = (threadIdx.x & 15) * 8;
+  const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = (lane & 15) * 8;
   if (row >= rows) return;
   float mx = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) {
+  for (int s = lane; s < p.nsplit; s += 64) {
     const float x = p.part_lse[s * rows + row];
     mx = x > mx || x != x ? x : mx;      // a NaN stays
   }
-  float sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (mx > -INFINITY || mx != mx)
-    for (int s = 0; s < p.nsplit; ++s) {
-      const float w = exp2f(p.part_lse[s * rows + row] - mx);
-      sum += w;
-      if (c < p.d) {
-        float v[8];
-        load8(v, p.part + (s * rows + row) * p.d + c, 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] += v[j] * w;
-      }
+  for (int o = 32; o > 0; o >>= 1) {
+    const float x = __shfl_xor(mx, o, 64);
+    mx = x > mx || x != x ? x : mx;
+  }
+  float sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (mx != -INFINITY) {
+#pragma unroll 4
+    for (int s = lane >> 4; s < p.nsplit; s += 4) {
+      const float w = exp2f(p.part_lse[s * rows + row] - mx);
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (c < p.d) load8(v, p.part + (s * rows + row) * p.d + c, 8);
+      sum += w;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += v[j] * w;
     }
+    sum = xa_groups_sum(sum);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = xa_groups_sum(acc[j]);
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (p.lse && (threadIdx.x & 15) == 0) p.lse[row] = sum == 0.f ? INFINITY : mx + log2f(sum);
-  if (c >= p.d) return;
+  if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? INFINITY : mx + log2f(sum);
+  if (c >= p.d || lane > 15) return;
   const int bh = (int)(row / p.rows), r = (int)(row % p.rows), s = r / p.grp, g = r % p.grp;
   const long oo = (((long)(bh / p.hkv) * p.sq + s) * p.hq + (bh % p.hkv) * p.grp + g) * p.d + c;
   float lo[8];
@@ -383,20 +544,16 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XaParams p) {
 // ------------------------------------------------------------------------------------------------ backward: dq
 // the forward kernel's shape: s^T and dp^T with a lane per row, dq^T = k^T ds^T, k read from LDS both ways
 template <typename T, int DT, int KW>
-__global__ __launch_bounds__(256, (DT > 2 ? 1 : 2)) void xattn_dq_kernel(XaParams p) {
+__global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
-  constexpr int BK = XaKeys<KW>::BK, SUB = XaKeys<KW>::SUB, IMG = BK * XaImg<DT>::PITCH;
+  constexpr int SUB = XaKeys<DT, KW>::SUB, NW = XaKeys<DT, KW>::NW, PITCH = XaImg<DT>::PITCH;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int tile, bh, split;
-  if (!xa_place(p, tile, bh, split)) return;
+  int tile, b, hk, split;
+  if (!xa_place(p, tile, b, hk, split)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = bh / p.hkv, hk = bh % p.hkv, h = lane >> 5;
+  const int bh = b * p.hkv + hk, h = lane >> 5;
   const int kw = wave % KW, r0 = tile * (128 / KW) + (wave / KW) * 32, r = r0 + (lane & 31);
   const bool rok = r < p.rows;
-  const int len = xa_len(p, b), nt = (len + BK - 1) / BK;
-  const int t0 = (int)((long)nt * split / p.nsplit), t1 = (int)((long)nt * (split + 1) / p.nsplit);
-  const T* kp = (const T*)p.k + (long)b * p.k_bs + (long)hk * p.k_hs;
-  const T* vp = (const T*)p.v + (long)b * p.v_bs + (long)hk * p.v_hs;
   const XaAddr<DT> ad(lane);
   const long row = (long)bh * p.rows + r;
   V qf[2 * DT], df[2 * DT];
@@ -409,57 +566,44 @@ __global__ __launch_bounds__(256, (DT > 2 ? 1 : 2)) void xattn_dq_kernel(XaParam
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  auto stage = [&](int t, int buf) {
-    unsigned w[BK / 32];
+  xa_over_keys<T, DT, KW>(p, lds, b, hk, split, r0 < p.rows, [&](const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+    unsigned w[SUB], any = 0;
+    xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
-    for (int i = 0; i < BK / 32; ++i) w[i] = xa_word(p, b, len, t * BK + i * 32);
-    auto ok = [&](int row) {
-      unsigned x = w[0];
+    for (int u = 0; u < SUB; ++u) any |= w[u];
+    if (any == 0) return;
+    ki += kw * SUB * 32 * PITCH;
+    vi += kw * SUB * 32 * PITCH;
+    f32x16 s[SUB], dp[SUB];
 #pragma unroll
-      for (int i = 1; i < BK / 32; ++i) x = (row >> 5) == i ? w[i] : x;
-      return ((x >> (row & 31)) & 1u) != 0;
-    };
-    xa_stage<DT, BK>(lds + buf * 2 * IMG, kp + (long)t * BK * p.k_ss, p.d, [&](int row) { return (long)row * p.k_ss; }, ok);
-    xa_stage<DT, BK>(lds + buf * 2 * IMG + IMG, vp + (long)t * BK * p.v_ss, p.d, [&](int row) { return (long)row * p.v_ss; }, ok);
-  };
-  auto compute = [&](int t, int buf) {
-    const uint8_t *ki = lds + buf * 2 * IMG, *vi = ki + IMG;
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      const int sub = kw * SUB + u;
-      const unsigned w = xa_word(p, b, len, t * BK + sub * 32);
-      if (w == 0) continue;
-      f32x16 s, dp;
+      for (int i = 0; i < 16; ++i) s[u][i] = dp[u][i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
       for (int st = 0; st < 2 * DT; ++st) {
-        s = mfma32(xa_frag<V>(ki + sub * 32 * XaImg<DT>::PITCH, ad.row[st]), qf[st], s);
-        dp = mfma32(xa_frag<V>(vi + sub * 32 * XaImg<DT>::PITCH, ad.row[st]), df[st], dp);
+        s[u] = mfma32(xa_frag<V>(ki + u * 32 * PITCH, ad.row[st]), qf[st], s[u]);
+        dp[u] = mfma32(xa_frag<V>(vi + u * 32 * PITCH, ad.row[st]), df[st], dp[u]);
       }
-      if (w != ~0u) {
-        const unsigned wl = w >> (4 * h);
+    XaSecond<T, KW == 4> ds[SUB];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = (wl >> (8 * (i / 4) + i % 4)) & 1u ? s[i] : -INFINITY;
-      }
-      V ds[2];
+    for (int u = 0; u < SUB; ++u) {
+      if (w[u] != ~0u) xa_mask(s[u], w[u], h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ds[i >> 3][i & 7] = (T)(__builtin_amdgcn_exp2f(s[i] * p.scale_log2 - L) * (dp[i] - delta));
+      for (int i = 0; i < 16; ++i) ds[u].set(i, __builtin_amdgcn_exp2f(s[u][i] * p.scale_log2 - L) * (dp[u][i] - delta));
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int t2 = 0; t2 < DT; ++t2)
-          acc[t2] = mfma32(xa_frag_tr<V>(ki + (sub * 32 + c * 16) * XaImg<DT>::PITCH, ad.tr[t2][0], ad.tr[t2][1]), ds[c], acc[t2]);
-    }
-  };
-  if (t0 < t1) {
-    stage(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-      __syncthreads();
-      if (t + 1 < t1) stage(t + 1, (t + 1 - t0) & 1);
-      if (r0 < p.rows) compute(t, (t - t0) & 1);
-    }
-  }
+        for (int t2 = 0; t2 < DT; ++t2) {
+          const V f = xa_frag_tr<V>(ki + (u * 32 + c * 16) * PITCH, ad.tr[t2][0], ad.tr[t2][1]);
+          if constexpr (KW == 4) acc[t2] = mfma32(f, ds[u].v[2 + c], acc[t2]);
+          acc[t2] = mfma32(f, ds[u].v[c], acc[t2]);
+        }
+  });
   if constexpr (KW > 1) {
     __syncthreads();
     float* x = (float*)lds;
@@ -504,18 +648,23 @@ __global__ __launch_bounds__(256, (DT > 2 ? 1 : 2)) void xattn_dq_kernel(XaParam
     }
 }
 
-// dq of a row = sum over splits, in their order
+// dq of a row = sum over splits
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
-  const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int c = (threadIdx.x & 15) * 8;
-  if (row >= rows || c >= p.d) return;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8];
-  for (int s = 0; s < p.nsplit; ++s) {
-    load8(v, p.part + (s * rows + row) * p.d + c, 8);
+  const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = (lane & 15) * 8;
+  if (row >= rows) return;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = lane >> 4; s < p.nsplit; s += 4) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < p.d) load8(v, p.part + (s * rows + row) * p.d + c, 8);
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] += v[j];
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = xa_groups_sum(acc[j]);
+  if (c >= p.d || lane > 15) return;
   const int bh = (int)(row / p.rows), r = (int)(row % p.rows), s = r / p.grp, g = r % p.grp;
   store8((T*)p.dq + (((long)(bh / p.hkv) * p.sq + s) * p.hq + (bh % p.hkv) * p.grp + g) * p.d + c, acc, 8);
 }
@@ -524,15 +673,19 @@ __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
 // Each wave keeps 32 keys (k, v as second operands in registers, dk^T and dv^T as accumulators) and walks the rows: s = q k^T and
 // dp = do v^T with a lane per key, then dv^T += do^T p and dk^T += q^T ds with q and do read from LDS both ways.  A lane's key touches its own
 // column of the products alone, so a masked key needs nothing inside the loop: zeros are written for it at the end.
+template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane of the wave that brings their L or delta
+  static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, NBUF = 2, BYTES = NBUF * BUF;
+};
 template <typename T, int DT>
-__global__ __launch_bounds__(256, (DT > 2 ? 1 : 2)) void xattn_dkv_kernel(XaParams p) {
+__global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
-  constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4;
+  typedef XaRows<DT> R;
+  constexpr int BR = R::BR, IMG = R::IMG, BUF = R::BUF, NBUF = R::NBUF;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int tile, bh, split;
-  if (!xa_place(p, tile, bh, split)) return;
+  int tile, b, hk, split;
+  if (!xa_place(p, tile, b, hk, split)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int b = bh / p.hkv, hk = bh % p.hkv, h = lane >> 5;
+  const int bh = b * p.hkv + hk, h = lane >> 5;
   const int key0 = tile * 128 + wave * 32, key = key0 + (lane & 31);
   const int len = xa_len(p, b), nt = (p.rows + BR - 1) / BR;
   unsigned any = 0;
@@ -553,21 +706,27 @@ __global__ __launch_bounds__(256, (DT > 2 ? 1 : 2)) void xattn_dkv_kernel(XaPara
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
 
-  auto stage = [&](int t, int buf) {
-    uint8_t* at = lds + buf * BUF;
-    auto ok = [&](int row) { return t * BR + row < p.rows; };
-    xa_stage<DT, BR>(at, qp, p.d, [&](int row) { return xa_row_off(p, t * BR + row, p.q_ss, p.q_hs); }, ok);
-    xa_stage<DT, BR>(at + IMG, dp_, p.d, [&](int row) { return xa_row_off(p, t * BR + row, p.o_ss, p.o_hs); }, ok);
-    if (threadIdx.x < 2 * BR) {      // L and delta of the rows; rows that are none get p = 0
-      const int row = t * BR + (threadIdx.x & (BR - 1));
-      const bool first = threadIdx.x < BR;
-      float x = first ? INFINITY : 0.f;
-      if (row < p.rows) x = (first ? p.lse_in : p.delta)[(long)bh * p.rows + row];
-      ((float*)(at + 2 * IMG))[threadIdx.x] = x;
+  const XaLoader<DT, T> ld(p.d);
+  const bool even = XaLoader<DT, T>::ROWS % p.grp == 0, full = p.d == XaImg<DT>::CH * 8;
+  const int lr = ld.r / p.grp, lg = ld.r % p.grp;
+  const unsigned q_off = (unsigned)(lr * (int)p.q_ss + lg * (int)p.q_hs + ld.c) * 2u, o_off = (unsigned)(lr * (int)p.o_ss + lg * (int)p.o_hs + ld.c) * 2u;
+  auto stage = [&](int t, uint8_t* at) {
+    if (full && even && (t + 1) * BR <= p.rows) {
+      ld.template rows<BR>(at, p, qp, p.q_ss, p.q_hs, q_off, true, true, t * BR);
+      ld.template rows<BR>(at + IMG, p, dp_, p.o_ss, p.o_hs, o_off, true, true, t * BR);
+    } else {
+      ld.template rows<BR>(at, p, qp, p.q_ss, p.q_hs, q_off, even, false, t * BR);
+      ld.template rows<BR>(at + IMG, p, dp_, p.o_ss, p.o_hs, o_off, even, false, t * BR);
+    }
+    if (wave < 2) {      // L and delta of the rows, by DMA too; rows that are none get L = infinity and so p = 0
+      const int row = t * BR + lane;
+      const float* src = wave ? (const float*)g_zero_line_xa : &g_inf_xa;
+      if (row < p.rows) src = (wave ? p.delta : p.lse_in) + (long)bh * p.rows + row;
+      xa_dma4(at + 2 * IMG + wave * (BR * 4), src);
     }
   };
-  auto compute = [&](int t, int buf) {
-    const uint8_t *qi = lds + buf * BUF, *di = qi + IMG;
+  auto compute = [&](int t, const uint8_t* qi) {
+    const uint8_t* di = qi + IMG;
     const float* st = (const float*)(qi + 2 * IMG);
 #pragma unroll
     for (int u = 0; u < BR / 32; ++u) {
@@ -601,13 +760,17 @@ __global__ __launch_bounds__(256, (DT > 2 ? 1 : 2)) void xattn_dkv_kernel(XaPara
         }
     }
   };
-  if (t0 < t1) {
-    stage(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-      __syncthreads();
-      if (t + 1 < t1) stage(t + 1, (t + 1 - t0) & 1);
-      if (w) compute(t, (t - t0) & 1);
-    }
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i)
+    if (t0 + i < t1) stage(t0 + i, lds + i * BUF);
+  xa_settle();
+  int use = 0, fill = (NBUF - 1) * BUF;
+  for (int t = t0; t < t1; ++t) {
+    xa_landed<0>();
+    if (t + NBUF - 1 < t1) stage(t + NBUF - 1, lds + fill);
+    if (w) compute(t, lds + use);
+    use = use + BUF == R::BYTES ? 0 : use + BUF;
+    fill = fill + BUF == R::BYTES ? 0 : fill + BUF;
   }
   if (key >= p.sk) return;
   typedef T tv4 __attribute__((ext_vector_type(4)));
@@ -661,12 +824,18 @@ static int xa_clamp(long v, long lo, long hi) { return (int)(v < lo ? lo : v > h
 static XaPlan xa_plan(const RtpXattn* a) {
   XaPlan pl;
   const long rows = (long)a->sq * (a->hq / a->hkv), bh = (long)a->b * a->hkv;
-  // up to 32 rows the four waves of a workgroup split the keys, up to 64 two and two: with few rows the keys are the work
-  pl.kw = rows <= 32 ? 4 : rows <= 64 ? 2 : 1;
+  // Up to 32 rows the four waves of a workgroup split the keys: with few rows the keys are the work.  Two and two up to 64 rows, and where four
+  // groups of rows would leave fewer than four workgroups to a CU (4 x 2560 rows x 8 heads, 640 workgroups: forward 99 us, two and two 84).
+  const long wide = rtp_div_up(rows, 128) * bh;
+  pl.kw = rows <= 32 ? 4 : rows <= 64 || wide < 1024 ? 2 : 1;
+  if (getenv("XA_KW")) pl.kw = atoi(getenv("XA_KW"));
   pl.tiles = rtp_div_up(rows, 128 / pl.kw);
   const long wgs = pl.tiles * bh, bk = pl.kw == 4 ? 128 : 64, nt = rtp_div_up(a->sk, bk);
-  // two workgroups for each CU; a split has at least four tiles, or its partial results cost as much as they save
-  pl.nsplit = xa_clamp(512 / (wgs > 0 ? wgs : 1), 1, nt / 4 > 1 ? nt / 4 : 1);
+  // as many workgroups as run at once (LDS: two for each CU, one with four waves on keys of over 64 columns, three below 32); a split has at
+  // least four tiles, or its partial results cost as much as they save
+  const long slots = pl.kw < 4 ? 512 : a->d > 64 ? 256 : a->d > 32 ? 512 : 768;
+  pl.nsplit = xa_clamp(slots / (wgs > 0 ? wgs : 1), 1, nt / 4 > 1 ? nt / 4 : 1);
+  if (getenv("XA_NS")) pl.nsplit = atoi(getenv("XA_NS"));
   pl.ktiles = rtp_div_up(a->sk, 128);
   const long kwgs = pl.ktiles * bh, rt = rtp_div_up(rows, 64);
   pl.ksplit = xa_clamp(512 / (kwgs > 0 ? kwgs : 1), 1, rt / 4 > 1 ? rt / 4 : 1);
@@ -689,6 +858,11 @@ static int xa_check(const RtpXattn* a) {
   return RTP_OK;
 }
 static bool xa_aligned(const void* p, long bs, long ss, long hs) { return !((size_t)p & 15) && !(bs & 7) && !(ss & 7) && !(hs & 7); }
+// offsets inside a staged step are 32 bits: up to 64 tokens and the heads of a group
+static bool xa_near(const RtpXattn* a, long ss, long hs) {
+  const long grp = a->hq / a->hkv;
+  return ss >= 0 && hs >= 0 && ss <= (1L << 23) && hs * grp <= (1L << 28);
+}
 
 static XaParams xa_params(const RtpXattn* a) {
   XaParams p = {};
@@ -754,22 +928,21 @@ static int xa_launch(K kernel, int grid, int bytes, bool* once, hipStream_t st, 
   RTP_CHECK_LAUNCH();
   return RTP_OK;
 }
-template <int DT, int KW> constexpr int xa_bytes() { return 4 * XaKeys<KW>::BK * XaImg<DT>::PITCH; }
 
 template <typename T, int DT, int KW>
 static int xa_fwd(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
-  return xa_launch(xattn_fwd_kernel<T, DT, KW>, grid, xa_bytes<DT, KW>(), once, st, p);
+  return xa_launch(xattn_fwd_kernel<T, DT, KW>, grid, XaKeys<DT, KW>::BYTES, once, st, p);
 }
 template <typename T, int DT, int KW>
 static int xa_dq(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
-  return xa_launch(xattn_dq_kernel<T, DT, KW>, grid, xa_bytes<DT, KW>(), once, st, p);
+  return xa_launch(xattn_dq_kernel<T, DT, KW>, grid, XaKeys<DT, KW>::BYTES, once, st, p);
 }
 template <typename T, int DT>
 static int xa_dkv(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
-  return xa_launch(xattn_dkv_kernel<T, DT>, grid, 2 * (2 * 64 * XaImg<DT>::PITCH + 2 * 64 * 4), once, st, p);
+  return xa_launch(xattn_dkv_kernel<T, DT>, grid, XaRows<DT>::BYTES, once, st, p);
 }
 
 extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* lse, void* ws, long ws_bytes, void* stream) {
@@ -780,6 +953,7 @@ extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* 
   if (!xa_aligned(a->q, a->q_bs, a->q_ss, a->q_hs) || !xa_aligned(a->k, a->k_bs, a->k_ss, a->k_hs) || !xa_aligned(a->v, a->v_bs, a->v_ss, a->v_hs) ||
       ((size_t)o & 15) || ((size_t)o_lo & 15) || ((size_t)ws & 255))
     return RTP_ERR_ALIGN;
+  if (!xa_near(a, a->q_ss, a->q_hs) || !xa_near(a, a->k_ss, 0) || !xa_near(a, a->v_ss, 0)) return RTP_ERR_SHAPE;
   const long need = rtp_xattn_workspace_bytes(a, 0);
   if (ws_bytes < need || (need > 0 && !ws)) return RTP_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
@@ -801,7 +975,7 @@ extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* 
     constexpr int DT = decltype(dt)::value;
     const int r = pl.kw == 4 ? xa_fwd<T, DT, 4>(grid, st, p) : pl.kw == 2 ? xa_fwd<T, DT, 2>(grid, st, p) : xa_fwd<T, DT, 1>(grid, st, p);
     if (r != RTP_OK || pl.nsplit == 1) return r;
-    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(rtp_div_up(rows, 16)), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
     RTP_CHECK_LAUNCH();
     return RTP_OK;
   });
@@ -816,6 +990,7 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
   if (!xa_aligned(a->q, a->q_bs, a->q_ss, a->q_hs) || !xa_aligned(a->k, a->k_bs, a->k_ss, a->k_hs) || !xa_aligned(a->v, a->v_bs, a->v_ss, a->v_hs) ||
       !xa_aligned(d_o, o_bs, o_ss, o_hs) || (((size_t)o | (size_t)o_lo | (size_t)dq | (size_t)dk | (size_t)dv) & 15) || ((size_t)ws & 255))
     return RTP_ERR_ALIGN;
+  if (!xa_near(a, a->q_ss, a->q_hs) || !xa_near(a, a->k_ss, 0) || !xa_near(a, a->v_ss, 0) || !xa_near(a, o_ss, o_hs)) return RTP_ERR_SHAPE;
   if (ws_bytes < rtp_xattn_workspace_bytes(a, 1)) return RTP_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
   RtpProfScope prof(RTP_FAM_POINTWISE, st);
@@ -840,7 +1015,7 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
       const int r = pl.kw == 4 ? xa_dq<T, DT, 4>(grid, st, p) : pl.kw == 2 ? xa_dq<T, DT, 2>(grid, st, p) : xa_dq<T, DT, 1>(grid, st, p);
       if (r != RTP_OK) return r;
       if (pl.nsplit > 1) {
-        hipLaunchKernelGGL((xattn_dq_join_kernel<T>), dim3(rtp_div_up(rows, 16)), dim3(256), 0, st, p);
+        hipLaunchKernelGGL((xattn_dq_join_kernel<T>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
         RTP_CHECK_LAUNCH();
       }
     }
