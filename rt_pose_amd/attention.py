@@ -68,21 +68,21 @@ def _workspace(a, backward, like):
     return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None, n
 
 
-def _forward(q, k, v, key_lens, key_mask, scale, train):
-    a = _operands(q, k, v, key_lens, key_mask, scale)
+def _forward(a, q, o_lo=None, lse=None):
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    o_lo, lse = (torch.empty_like(o), q.new_empty(o.shape[:3].numel(), dtype=torch.float32)) if train else (None, None)
     if o.numel():
         ws, n = _workspace(a, 0, q)
         call("rtp_xattn_forward", q, C.byref(a), p(o), p(o_lo), p(lse), p(ws), n)
-    return o, o_lo, lse
+    return o
 
 
 class CrossAttentionFunction(Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lens, key_mask, scale):
-        o, o_lo, lse = _forward(q, k, v, key_lens, key_mask, scale, True)
-        ctx.scale = scale
+        a = _operands(q, k, v, key_lens, key_mask, scale)
+        o_lo, lse = torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty(q.shape[:3].numel(), dtype=torch.float32)
+        o = _forward(a, q, o_lo, lse)
+        ctx.operands, ctx.scale = a, scale
         ctx.save_for_backward(q, k, v, key_lens, key_mask, o, o_lo, lse)
         return o
 
@@ -90,13 +90,15 @@ class CrossAttentionFunction(Function):
     @once_differentiable
     def backward(ctx, do):
         q, k, v, key_lens, key_mask, o, o_lo, lse = ctx.saved_tensors
-        need_q, need_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
-        dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if need_kv else None for t in (k, v))
+        dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if need_k or need_v else None for t in (k, v))
         if q.numel() == 0 or k.numel() == 0:
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv)) + (None, None, None)
-        do = _aligned(do)
-        a = _operands(q, k, v, key_lens, key_mask, ctx.scale)
+        a, do = ctx.operands, _aligned(do)
+        if (a.q, a.k, a.v) != (p(q), p(k), p(v)) or a.key_lens != p(key_lens) or a.key_mask != p(key_mask):   # saved tensors kept elsewhere meanwhile
+            q, k, v = _aligned(q), _aligned(k), _aligned(v)
+            a = _operands(q, k, v, key_lens, key_mask, ctx.scale)
         ws, n = _workspace(a, 1, q)
         call("rtp_xattn_backward", q, C.byref(a), p(o), p(o_lo), p(lse), p(do), *_strides(do), p(dq), p(dk), p(dv), p(ws), n)
         return dq, dk, dv, None, None, None
@@ -111,4 +113,4 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
         key_lens = (key_lens if key_lens.dtype == torch.int32 else key_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return CrossAttentionFunction.apply(q, k, v, key_lens, key_mask, scale)
-    return _forward(q, k, v, key_lens, key_mask, scale, False)[0]
+    return _forward(_operands(q, k, v, key_lens, key_mask, scale), q)

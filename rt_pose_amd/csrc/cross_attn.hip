@@ -15,7 +15,6 @@
 // (ds_read_b64_tr_b16) in that same order.  p never leaves the registers.  dq works the same way; dk / dv with rows and keys exchanged.
 // Operands of 16 bits, everything else fp32: p and ds are rounded once to 16 bits for their second product (2^-9 of each, averaged over the
 // keys), the sums they enter are fp32.
-#include <stdlib.h>
 #include <type_traits>
 
 #include "rtp_prof.h"
@@ -217,11 +216,37 @@ __device__ __forceinline__ void xa_load_row(typename Vec8<T>::type (&f)[2 * DT],
 #define XA_M0 (-3.402823466e38f)
 #define XA_SLACK 8.0f   // the running maximum moves only when it is exceeded by 2^8: p stays below 2^8, and most tiles rescale nothing
 
+// fp16 has 2^-14 .. 65504 at full precision, and p (1 / keys on the average) and ds lie at its lower end.  So p is taken times 2^7 forward (with the
+// slack at most 2^15) and times 2^14 backward (p <= 1); ds starts at 2^14 too, and a row or key whose |ds| would pass 2^15 lowers its own
+// factor and what it has summed so far.  bf16 has fp32's range: no factors.
+template <typename T> struct XaRange { static constexpr bool NARROW = false; static constexpr float FWD = 0.f, BWD = 0.f; };
+template <> struct XaRange<_Float16> { static constexpr bool NARROW = true; static constexpr float FWD = 7.f, BWD = 14.f; };
+// this lane's sixteen ds (times 2^ex) and the other half wave's of the same row or key; acc: the DT accumulators of that row or key
+template <int DT>
+__device__ __forceinline__ bool xa_narrow(f32x16& x, f32x16 (&acc)[DT], float& ex) {
+  float mx = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fabsf(x[i]));
+  mx = xa_halves_max(mx);
+  if (!__any(mx > 32768.f)) return false;
+  const float drop = mx > 32768.f ? fminf(ceilf(log2f(mx)) - 8.f, 100.f) : 0.f, f = exp2f(-drop);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] *= f;
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] *= f;
+  ex -= drop;
+  return true;
+}
+
 // ------------------------------------------------------------------------------------------------ the loop over keys
 // Four waves: 4 / KW groups of 32 rows, and KW waves that share rows and split each tile of keys (few rows: the keys are the work).
 // Tiles of BK keys go round NBUF LDS buffers: while one is used, the next NBUF - 1 are on their way, and the barrier in front of a tile waits
-// for that tile's transfers alone (they complete in order, PER of them a wave and tile).  Three buffers where they leave room for the waves
-// that the registers allow.  The mask's words are scalar loads, one tile further ahead, so that nothing else counts as a vector access.
+// for that tile's transfers alone (they complete in order, PER of them a wave and tile).  Two buffers leave room for more workgroups on a CU,
+// which hide more than a third one (heads of 64: forward 89 us with three, 81 with two); heads up to 32 columns have small tiles and three.
+// The mask's words are scalar loads, one tile further ahead, so that nothing else counts as a vector access.
+// (Forming the next tile's scores beside this one's exponentials in one wave takes half as many registers again: 81 -> 103 us.)
 template <int DT, int KW> struct XaKeys {
   static constexpr int BK = KW == 4 ? 128 : 64, SUB = BK / 32 / KW, NW = BK / 32, IMG = BK * XaImg<DT>::PITCH;
   static constexpr int NBUF = DT == 1 ? 3 : 2, BYTES = NBUF * 2 * IMG;
@@ -351,7 +376,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
     for (int u = 0; u < SUB; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-    mx = xa_halves_max(mx) * p.scale_log2;
+    mx = xa_halves_max(mx) * p.scale_log2 - XaRange<T>::FWD;
     if (__any(mx > m + XA_SLACK)) {
       const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -519,8 +544,7 @@ __global__ __launch_bounds__(256) void xattn_bits_kernel(const uint8_t* mask, lo
 }
 
 // ------------------------------------------------------------------------------------------------ backward: delta
-// delta of a row = sum_d do * o, from o as it was before its rounding (o + what the rounding left over): with few keys the difference
-// dp - delta cancels, and o's rounding alone would be most of it.  16 lanes a row.
+// delta of a row by itself, for a pass without the gradient of q (whose kernel forms it otherwise).  16 lanes a row.
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_delta_kernel(XaParams p) {
   const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -559,7 +583,23 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
   V qf[2 * DT], df[2 * DT];
   xa_load_row<DT, T>(qf, (const T*)p.q + (long)b * p.q_bs + (long)(hk * p.grp) * p.q_hs + (rok ? xa_row_off(p, r, p.q_ss, p.q_hs) : 0), rok, p.d, h);
   xa_load_row<DT, T>(df, (const T*)p.d_o + (long)b * p.o_bs + (long)(hk * p.grp) * p.o_hs + (rok ? xa_row_off(p, r, p.o_ss, p.o_hs) : 0), rok, p.d, h);
-  const float L = rok ? p.lse_in[row] : INFINITY, delta = rok ? p.delta[row] : 0.f;
+  float ex = XaRange<T>::BWD, L = (rok ? p.lse_in[row] : INFINITY) - ex;     // p times 2^ex
+  // delta = sum_d do o of this lane's row, from o as it was before its rounding (o + what the rounding left over): with few keys the difference
+  // dp - delta cancels, and o's rounding alone would be most of it.  It is left for the gradients of k and v too (every split the same value).
+  float delta = 0.f;
+  {
+    const int tok = rok ? r / p.grp : 0, g = rok ? r % p.grp : 0;
+    const long oo = (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
+    V oh[2 * DT], ol[2 * DT];
+    xa_load_row<DT, T>(oh, (const T*)p.o + oo, rok, p.d, h);
+    xa_load_row<DT, T>(ol, (const T*)p.o_lo + oo, rok, p.d, h);
+#pragma unroll
+    for (int st = 0; st < 2 * DT; ++st)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += ((float)oh[st][j] + (float)ol[st][j]) * (float)df[st][j];
+    delta = xa_halves_sum(delta);
+    if (rok && h == 0 && kw == 0) p.delta[row] = delta;
+  }
   f32x16 acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
@@ -591,7 +631,25 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
     for (int u = 0; u < SUB; ++u) {
       if (w[u] != ~0u) xa_mask(s[u], w[u], h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) ds[u].set(i, __builtin_amdgcn_exp2f(s[u][i] * p.scale_log2 - L) * (dp[u][i] - delta));
+      for (int i = 0; i < 16; ++i) dp[u][i] = __builtin_amdgcn_exp2f(s[u][i] * p.scale_log2 - L) * (dp[u][i] - delta);
+    }
+    if constexpr (XaRange<T>::NARROW) {
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const float before = ex;
+        if (xa_narrow<DT>(dp[u], acc, ex)) {
+          L += before - ex;
+          const float f = exp2f(ex - before);
+#pragma unroll
+          for (int k = 0; k < SUB; ++k)
+            if (k != u) dp[k] *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds[u].set(i, dp[u][i]);
     }
 #pragma unroll
     for (int u = 0; u < SUB; ++u)
@@ -604,6 +662,11 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
           acc[t2] = mfma32(f, ds[u].v[c], acc[t2]);
         }
   });
+  const float out = p.scale * exp2f(-ex);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] *= out;
   if constexpr (KW > 1) {
     __syncthreads();
     float* x = (float*)lds;
@@ -637,7 +700,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
     for (int i = 0; i < 16; i += 4) {
       const int c = 32 * t + 2 * i + 4 * h;
       if (c < p.d) {
-        const f32x4 v = {acc[t][i] * p.scale, acc[t][i + 1] * p.scale, acc[t][i + 2] * p.scale, acc[t][i + 3] * p.scale};
+        const f32x4 v = {acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
         if (p.nsplit > 1) {
           *(f32x4*)(po + c) = v;
         } else {
@@ -673,14 +736,14 @@ __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
 // Each wave keeps 32 keys (k, v as second operands in registers, dk^T and dv^T as accumulators) and walks the rows: s = q k^T and
 // dp = do v^T with a lane per key, then dv^T += do^T p and dk^T += q^T ds with q and do read from LDS both ways.  A lane's key touches its own
 // column of the products alone, so a masked key needs nothing inside the loop: zeros are written for it at the end.
-template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane of the wave that brings their L or delta
-  static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, NBUF = 2, BYTES = NBUF * BUF;
+template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane of the wave that brings their L or delta; two buffers
+  static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, BYTES = 2 * BUF;
 };
-template <typename T, int DT>
+template <typename T, int DT, bool LO>
 __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
   typedef XaRows<DT> R;
-  constexpr int BR = R::BR, IMG = R::IMG, BUF = R::BUF, NBUF = R::NBUF;
+  constexpr int BR = R::BR, IMG = R::IMG, BUF = R::BUF;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
   int tile, b, hk, split;
   if (!xa_place(p, tile, b, hk, split)) return;
@@ -705,6 +768,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[t][i] = dv[t][i] = 0.f;
+  float ex = XaRange<T>::BWD, less = 1.f;      // ds times 2^ex, in p's factor times `less`
 
   const XaLoader<DT, T> ld(p.d);
   const bool even = XaLoader<DT, T>::ROWS % p.grp == 0, full = p.d == XaImg<DT>::CH * 8;
@@ -739,40 +803,47 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
         s = mfma32(xa_frag<V>(qi + u * 32 * XaImg<DT>::PITCH, ad.row[e]), kf[e], s);
         dp = mfma32(xa_frag<V>(di + u * 32 * XaImg<DT>::PITCH, ad.row[e]), vf[e], dp);
       }
-      V pb[2], sb[2];
+      XaSecond<T, LO> pb, sb;
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const f32x4 L = *(const f32x4*)(st + u * 32 + 2 * i + 4 * h), dl = *(const f32x4*)(st + BR + u * 32 + 2 * i + 4 * h);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float e = __builtin_amdgcn_exp2f(s[i + j] * p.scale_log2 - L[j]);
-          pb[(i + j) >> 3][(i + j) & 7] = (T)e;
-          sb[(i + j) >> 3][(i + j) & 7] = (T)(e * (dp[i + j] - dl[j]));
+          const float e = __builtin_amdgcn_exp2f(s[i + j] * p.scale_log2 - (XaRange<T>::NARROW ? L[j] - XaRange<T>::BWD : L[j]));
+          pb.set(i + j, e);
+          dp[i + j] = e * (dp[i + j] - dl[j]);
+          if constexpr (XaRange<T>::NARROW) dp[i + j] *= less;
         }
       }
+      if constexpr (XaRange<T>::NARROW) {
+        if (xa_narrow<DT>(dp, dk, ex)) less = exp2f(ex - XaRange<T>::BWD);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sb.set(i, dp[i]);
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int t2 = 0; t2 < DT; ++t2) {
           const int off = (u * 32 + c * 16) * XaImg<DT>::PITCH;
-          dv[t2] = mfma32(xa_frag_tr<V>(di + off, ad.tr[t2][0], ad.tr[t2][1]), pb[c], dv[t2]);
-          dk[t2] = mfma32(xa_frag_tr<V>(qi + off, ad.tr[t2][0], ad.tr[t2][1]), sb[c], dk[t2]);
+          const V df = xa_frag_tr<V>(di + off, ad.tr[t2][0], ad.tr[t2][1]), qf = xa_frag_tr<V>(qi + off, ad.tr[t2][0], ad.tr[t2][1]);
+          if constexpr (LO) {
+            dv[t2] = mfma32(df, pb.v[2 + c], dv[t2]);
+            dk[t2] = mfma32(qf, sb.v[2 + c], dk[t2]);
+          }
+          dv[t2] = mfma32(df, pb.v[c], dv[t2]);
+          dk[t2] = mfma32(qf, sb.v[c], dk[t2]);
         }
     }
   };
-#pragma unroll
-  for (int i = 0; i < NBUF - 1; ++i)
-    if (t0 + i < t1) stage(t0 + i, lds + i * BUF);
+  if (t0 < t1) stage(t0, lds);
   xa_settle();
-  int use = 0, fill = (NBUF - 1) * BUF;
   for (int t = t0; t < t1; ++t) {
     xa_landed<0>();
-    if (t + NBUF - 1 < t1) stage(t + NBUF - 1, lds + fill);
-    if (w) compute(t, lds + use);
-    use = use + BUF == R::BYTES ? 0 : use + BUF;
-    fill = fill + BUF == R::BYTES ? 0 : fill + BUF;
+    if (t + 1 < t1) stage(t + 1, lds + ((t + 1 - t0) & 1) * BUF);
+    if (w) compute(t, lds + ((t - t0) & 1) * BUF);
   }
   if (key >= p.sk) return;
+  const float k_out = p.scale * exp2f(-ex), v_out = exp2f(-XaRange<T>::BWD);
   typedef T tv4 __attribute__((ext_vector_type(4)));
   const long oo = (((long)b * p.sk + key) * p.hkv + hk) * p.d;
   const long all = (long)p.b * p.sk * p.hkv * p.d;
@@ -785,8 +856,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
         f32x4 x, y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          x[j] = kok ? dk[t][i + j] * p.scale : 0.f;
-          y[j] = kok ? dv[t][i + j] : 0.f;
+          x[j] = kok ? dk[t][i + j] * k_out : 0.f;
+          y[j] = kok ? dv[t][i + j] * v_out : 0.f;
         }
         if (p.nsplit > 1) {
           *(f32x4*)(p.part + (2L * split) * all + oo + c) = x;
@@ -828,14 +899,12 @@ static XaPlan xa_plan(const RtpXattn* a) {
   // groups of rows would leave fewer than four workgroups to a CU (4 x 2560 rows x 8 heads, 640 workgroups: forward 99 us, two and two 84).
   const long wide = rtp_div_up(rows, 128) * bh;
   pl.kw = rows <= 32 ? 4 : rows <= 64 || wide < 1024 ? 2 : 1;
-  if (getenv("XA_KW")) pl.kw = atoi(getenv("XA_KW"));
   pl.tiles = rtp_div_up(rows, 128 / pl.kw);
   const long wgs = pl.tiles * bh, bk = pl.kw == 4 ? 128 : 64, nt = rtp_div_up(a->sk, bk);
   // as many workgroups as run at once (LDS: two for each CU, one with four waves on keys of over 64 columns, three below 32); a split has at
   // least four tiles, or its partial results cost as much as they save
   const long slots = pl.kw < 4 ? 512 : a->d > 64 ? 256 : a->d > 32 ? 512 : 768;
   pl.nsplit = xa_clamp(slots / (wgs > 0 ? wgs : 1), 1, nt / 4 > 1 ? nt / 4 : 1);
-  if (getenv("XA_NS")) pl.nsplit = atoi(getenv("XA_NS"));
   pl.ktiles = rtp_div_up(a->sk, 128);
   const long kwgs = pl.ktiles * bh, rt = rtp_div_up(rows, 64);
   pl.ksplit = xa_clamp(512 / (kwgs > 0 ? kwgs : 1), 1, rt / 4 > 1 ? rt / 4 : 1);
@@ -939,10 +1008,10 @@ static int xa_dq(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
   return xa_launch(xattn_dq_kernel<T, DT, KW>, grid, XaKeys<DT, KW>::BYTES, once, st, p);
 }
-template <typename T, int DT>
+template <typename T, int DT, bool LO>
 static int xa_dkv(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
-  return xa_launch(xattn_dkv_kernel<T, DT>, grid, XaRows<DT>::BYTES, once, st, p);
+  return xa_launch(xattn_dkv_kernel<T, DT, LO>, grid, XaRows<DT>::BYTES, once, st, p);
 }
 
 extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* lse, void* ws, long ws_bytes, void* stream) {
@@ -1008,9 +1077,10 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
   return xa_types(a, [&](auto t, auto dt) {
     typedef decltype(t) T;
     constexpr int DT = decltype(dt)::value;
-    hipLaunchKernelGGL((xattn_delta_kernel<T>), dim3(rtp_div_up(rows, 16)), dim3(256), 0, st, p);
-    RTP_CHECK_LAUNCH();
-    if (dq) {
+    if (!dq) {
+      hipLaunchKernelGGL((xattn_delta_kernel<T>), dim3(rtp_div_up(rows, 16)), dim3(256), 0, st, p);
+      RTP_CHECK_LAUNCH();
+    } else {
       const int grid = xa_grid(p, pl.tiles, pl.nsplit);
       const int r = pl.kw == 4 ? xa_dq<T, DT, 4>(grid, st, p) : pl.kw == 2 ? xa_dq<T, DT, 2>(grid, st, p) : xa_dq<T, DT, 1>(grid, st, p);
       if (r != RTP_OK) return r;
@@ -1020,7 +1090,7 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
       }
     }
     if (!dk) return RTP_OK;
-    const int grid = xa_grid(p, pl.ktiles, pl.ksplit), r = xa_dkv<T, DT>(grid, st, p);
+    const int grid = xa_grid(p, pl.ktiles, pl.ksplit), r = pl.kw == 4 ? xa_dkv<T, DT, true>(grid, st, p) : xa_dkv<T, DT, false>(grid, st, p);
     if (r != RTP_OK) return r;
     if (pl.ksplit > 1) {
       const long all = (long)a->b * a->sk * a->hkv * a->d;
