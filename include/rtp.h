@@ -572,7 +572,7 @@ int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int w_dtype, c
                          void* dw, float* part, long rows, int h, int dtype, float eps, void* stream);
 /* x -> q, scale with blocks of 1 x 128 (square = 0) or 128 x 128 (square = 1): a = max(largest magnitude, 2^-100), q = e4m3(x * (448 / a)),
  * scale = a / 448.  turned = 1: x is given by columns, x[r][c] at c * x_rs + r (a transpose that is never written out).  The bytes between
- * cols and cols rounded up to 8 are written too. */
+ * cols and cols rounded up to 16 are written too. */
 int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, float* scale, long rows, int cols, int square, int dtype,
                      void* stream);
 

@@ -1,6 +1,7 @@
 """Marshalling shared by the token operators (rmsnorm.py, fp8.py, attention.py).  Small calls are bound by the host: one native call, no
 context manager and no stream object where the tensor's device is already the current one."""
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -18,7 +19,7 @@ _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cud
 
 def call(name, t, *args):
     """The native entry `name` on the current stream of t's device, with that device current; RtpError if it fails."""
-    index = t.device.index
+    index = t.get_device()
     if index == _current_device():
         rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
     else:
@@ -28,12 +29,28 @@ def call(name, t, *args):
         _lib.check(rc, name)
 
 
+def once(backward):
+    """A Function's backward that cannot be differentiated again (autograd says so if one tries).  The guard is put on only where a graph of the
+    backward pass is asked for: a backward pass runs in a thread of its own, where every line of Python costs twice."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def same_device(x, *others):
     if not x.is_cuda:
         raise NotImplementedError("rt_pose_amd has no CPU path")
+    index = x.get_device()
     for t in others:
-        if t is not None and t.device != x.device:
+        if t is not None and t.get_device() != index:
             raise ValueError("operands on different devices (%s and %s)" % (x.device, t.device))
+
+
+def like(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def rows_of(t):

@@ -13,63 +13,69 @@ import ctypes as C
 
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tokens import DTYPES, call, p, same_device
+from ._tokens import DTYPES, call, like, once, p, same_device
 
 
 def _check(q, k, v, key_lens, key_mask, scale):
     same_device(q, k, v, key_lens, key_mask)
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise NotImplementedError("cross_attention: bf16 or fp16 only (got %s)" % q.dtype)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError("cross_attention: q, k and v of one type expected (got %s, %s, %s)" % (q.dtype, k.dtype, v.dtype))
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
-        raise ValueError("cross_attention: [b, sq, hq, d] and twice [b, sk, hkv, d] expected (got %s, %s, %s)"
-                         % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
-    if k.shape[2] < 1 or q.shape[2] < 1 or q.shape[2] % k.shape[2]:
-        raise ValueError("cross_attention: %d query heads are no multiple of %d key heads" % (q.shape[2], k.shape[2]))
-    if q.shape[3] < 8 or q.shape[3] % 8 or q.shape[3] > 128:
-        raise NotImplementedError("cross_attention: head widths of a multiple of 8 up to 128 (got %d)" % q.shape[3])
-    if key_lens is not None and (key_lens.shape != q.shape[:1] or key_lens.dtype not in (torch.int32, torch.int64)):
-        raise ValueError("cross_attention: key_lens of shape (%d,) and whole numbers expected (got %s %s)"
-                         % (q.shape[0], tuple(key_lens.shape), key_lens.dtype))
+    dtype, qs, ks = q.dtype, q.shape, k.shape
+    if dtype != torch.bfloat16 and dtype != torch.float16:
+        raise NotImplementedError("cross_attention: bf16 or fp16 only (got %s)" % dtype)
+    if k.dtype != dtype or v.dtype != dtype:
+        raise ValueError("cross_attention: q, k and v of one type expected (got %s, %s, %s)" % (dtype, k.dtype, v.dtype))
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[3] != ks[3]:
+        raise ValueError("cross_attention: [b, sq, hq, d] and twice [b, sk, hkv, d] expected (got %s, %s, %s)" % (tuple(qs), tuple(ks), tuple(v.shape)))
+    if ks[2] < 1 or qs[2] < 1 or qs[2] % ks[2]:
+        raise ValueError("cross_attention: %d query heads are no multiple of %d key heads" % (qs[2], ks[2]))
+    if qs[3] < 8 or qs[3] % 8 or qs[3] > 128:
+        raise NotImplementedError("cross_attention: head widths of a multiple of 8 up to 128 (got %d)" % qs[3])
+    if key_lens is not None and (key_lens.shape != qs[:1] or key_lens.dtype not in (torch.int32, torch.int64)):
+        raise ValueError("cross_attention: key_lens of shape (%d,) and whole numbers expected (got %s %s)" % (qs[0], tuple(key_lens.shape), key_lens.dtype))
     if key_mask is not None and key_mask.dtype != torch.bool:
         raise NotImplementedError("cross_attention: key_mask of truth values only, True where a key counts (got %s)" % key_mask.dtype)
-    if key_mask is not None and key_mask.shape != k.shape[:2]:
-        raise ValueError("cross_attention: key_mask of shape %s expected (got %s)" % (tuple(k.shape[:2]), tuple(key_mask.shape)))
+    if key_mask is not None and key_mask.shape != ks[:2]:
+        raise ValueError("cross_attention: key_mask of shape %s expected (got %s)" % (tuple(ks[:2]), tuple(key_mask.shape)))
     if not 0.0 < scale <= 3e38:
         raise ValueError("cross_attention: a positive, finite scale expected (got %r)" % (scale,))
 
 
 def _aligned(t):
     """t with contiguous heads in rows on 16-byte boundaries: itself, or a copy."""
-    st = t.stride()
-    if st[3] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 or n == 1 for s, n in zip(st[:3], t.shape)):
-        return t
-    return t.contiguous()
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        st = t.stride()
+        if st[3] == 1 and all(s % 8 == 0 or n == 1 for s, n in zip(st, t.shape[:3])):
+            return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
 def _strides(t):
+    """of batch, token and head; of a dimension of one any would do, and a tensor may have any there"""
+    if t.is_contiguous():
+        _, n, h, d = t.shape
+        return n * h * d, h * d, d
     return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
 
 
 def _operands(q, k, v, key_lens, key_mask, scale):
     b, sq, hq, d = q.shape
-    return _lib.RtpXattn(p(q), p(k), p(v), *_strides(q), *_strides(k), *_strides(v), p(key_mask),
-                         *((0, 0) if key_mask is None else key_mask.stride()), p(key_lens), b, sq, k.shape[1], hq, k.shape[2], d, DTYPES[q.dtype], scale)
+    _, sk, hkv, _ = k.shape
+    return _lib.RtpXattn(q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q), *_strides(k), *_strides(v), p(key_mask),
+                         *((0, 0) if key_mask is None else key_mask.stride()), p(key_lens), b, sq, sk, hq, hkv, d, DTYPES[q.dtype], scale)
 
 
-def _workspace(a, backward, like):
+def _workspace(a, backward, ref):
     n = _lib.load().rtp_xattn_workspace_bytes(C.byref(a), backward)
     if n < 0:
-        raise _lib.RtpError("cross_attention: sizes beyond what the kernels index (%s)" % (tuple(like.shape),))
-    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None, n
+        raise _lib.RtpError("cross_attention: sizes beyond what the kernels index (%s)" % (tuple(ref.shape),))
+    return ref.new_empty(n, dtype=torch.uint8) if n else None, n
 
 
 def _forward(a, q, o_lo=None, lse=None):
-    o = torch.empty_like(q, memory_format=torch.contiguous_format)
+    o = like(q)
     if o.numel():
         ws, n = _workspace(a, 0, q)
         call("rtp_xattn_forward", q, C.byref(a), p(o), p(o_lo), p(lse), p(ws), n)
@@ -80,24 +86,24 @@ class CrossAttentionFunction(Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lens, key_mask, scale):
         a = _operands(q, k, v, key_lens, key_mask, scale)
-        o_lo, lse = torch.empty_like(q, memory_format=torch.contiguous_format), q.new_empty(q.shape[:3].numel(), dtype=torch.float32)
+        o_lo, lse = like(q), q.new_empty(q.shape[:3].numel(), dtype=torch.float32)
         o = _forward(a, q, o_lo, lse)
         ctx.operands, ctx.scale = a, scale
         ctx.save_for_backward(q, k, v, key_lens, key_mask, o, o_lo, lse)
         return o
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, do):
         q, k, v, key_lens, key_mask, o, o_lo, lse = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        dq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
-        dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) if need_k or need_v else None for t in (k, v))
+        dq = like(q) if need_q else None
+        dk, dv = (like(k), like(v)) if need_k or need_v else (None, None)
         if q.numel() == 0 or k.numel() == 0:
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv)) + (None, None, None)
         a, do = ctx.operands, _aligned(do)
-        if (a.q, a.k, a.v) != (p(q), p(k), p(v)) or a.key_lens != p(key_lens) or a.key_mask != p(key_mask):   # saved tensors kept elsewhere meanwhile
-            q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        if a.q != q.data_ptr() or a.k != k.data_ptr() or a.v != v.data_ptr() or a.key_lens != p(key_lens) or a.key_mask != p(key_mask):
+            q, k, v = _aligned(q), _aligned(k), _aligned(v)          # saved tensors were kept elsewhere meanwhile
             a = _operands(q, k, v, key_lens, key_mask, ctx.scale)
         ws, n = _workspace(a, 1, q)
         call("rtp_xattn_backward", q, C.byref(a), p(o), p(o_lo), p(lse), p(do), *_strides(do), p(dq), p(dk), p(dv), p(ws), n)

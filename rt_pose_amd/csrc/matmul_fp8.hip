@@ -194,7 +194,8 @@ __global__ __launch_bounds__(64 * MM8_FEW_WAVES) void mm8_few_kernel(Mm8Params p
 
 // ------------------------------------------------------------------------------------------------ tiles
 // BM x BN per workgroup, WM x WN per wave.  Blocks of 128 k are staged by LDS-DMA (16 B a lane, no registers) into two buffers, the next
-// one while this one is multiplied: one barrier per block.  A row is 128 B in LDS, its 16-byte chunk c at slot c ^ ((row / 2) % 8), and lanes
+// one while this one is multiplied: one barrier per block.  A row is 128 B in LDS, its 16-byte chunk c at slot c ^ ((row / 2) % 8) (rows of b, read
+// in another order: c ^ (row / 8 % 4 * 2 + row / 2 % 2)), and lanes
 // of group g = lane / 16 read chunks g and g + 4.  A 16-byte LDS read goes by the lanes {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same of
 // the upper half: each of these sets then touches 16 different slots of the 256-byte bank row (chunks 2 g and 2 g + 1 instead: every read
 // two-way, half of the LDS cycles, 637 -> 621 us at 8192^3).
@@ -222,7 +223,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
 #pragma unroll
   for (int i = 0; i < AI + BI; ++i) {
     const int item = (i < AI ? i : i - AI) * THREADS + threadIdx.x, row = item >> 3;
-    const int chunk = (item & 7) ^ ((row >> 1) & 7);
+    const int chunk = (item & 7) ^ (i < AI ? (row >> 1) & 7 : (row >> 2 & 6) | (row >> 1 & 1));
     if (i < AI)
       src[i] = (m0 + row < p.m ? row : p.m - 1 - m0) * (int)p.lda + chunk * 16;
     else
@@ -245,7 +246,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
   auto stage = [&](int kb, int buf, int i) {
     if (i < AI + BI) {
       const bool tail = (kb + 1) * 128 > p.k;
-      const int chunk = ((threadIdx.x & 7) ^ ((threadIdx.x >> 4) & 7)) * 16;   // THREADS is a multiple of 128: the same in every step
+      const int row = threadIdx.x >> 3;                                        // and multiples of 16 (32): the same chunk in every step
+      const int chunk = ((threadIdx.x & 7) ^ (i < AI ? (row >> 1) & 7 : (row >> 2 & 6) | (row >> 1 & 1))) * 16;
       // a chunk behind k: any readable one in its place, the fragment's mask makes it zero
       const int off = tail && kb * 128 + chunk >= p.k ? src[i] - chunk - kb * 128 : src[i];
       __builtin_amdgcn_global_load_lds((const glb_void*)((i < AI ? ab : bb) + (long)kb * 128 + off),
@@ -265,31 +267,36 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
     for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int sw = (col >> 1) & 7;
   const int off0 = col * 128 + (g ^ sw) * 16, off1 = col * 128 + ((g + 4) ^ sw) * 16;
+  // rows of b in pairs of tiles: instruction row r of tile 2 i is n = 32 i + 8 (r / 4) + r % 4, of tile 2 i + 1 four more; a lane then holds eight
+  // neighbouring n of one m and stores them at once
+  const int brow = 8 * (col >> 2) + (col & 3), bsw = (brow >> 2 & 6) | (brow >> 1 & 1);
+  const int boff0 = brow * 128 + (g ^ bsw) * 16, boff1 = brow * 128 + ((g + 4) ^ bsw) * 16;
   auto compute = [&](int kb, int buf, bool tail, bool more) {
     const uint8_t* la = lds + buf * BUF + wm * 128;
     const uint8_t* lb = lds + buf * BUF + BM * 128 + wn * 128;
     const float* ls = (const float*)(lds + buf * BUF + (BM + BN) * 128);
     i32x8 mask;
     if (tail) mask = tail_mask(kb * 128 + g * 16, kb * 128 + g * 16 + 64, p.k);
-    auto frag = [&](const uint8_t* t) {
-      const i32x4 lo = *(const i32x4*)(t + off0), hi = *(const i32x4*)(t + off1);
+    auto frag = [&](const uint8_t* t, int o0, int o1) {
+      const i32x4 lo = *(const i32x4*)(t + o0), hi = *(const i32x4*)(t + o1);
       i32x8 r = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       if (tail) r &= mask;
       Frag f;
       make_frag(f, r);
       return f;
     };
+    auto b_frag = [&](int i) { return frag(lb + (i >> 1) * 4096 + (i & 1) * 512, boff0, boff1); };
     Frag af[MT];
     float f[MT];
     const float sbu = SQUARE ? ls[BM + (wn >> 7)] : 1.f;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      af[j] = frag(la + j * 2048);
+      af[j] = frag(la + j * 2048, off0, off1);
       f[j] = ls[wm + j * 16 + col] * sbu;
     }
     // step i multiplies, while the results of step i - 1 are scaled and added and the fragment of step i + 2 is read
     constexpr int PER = 4;
-    Frag bf = frag(lb), b1 = frag(lb + 2048);
+    Frag bf = b_frag(0), b1 = b_frag(1);
     f32x4 r[MT], sb4 = {1.f, 1.f, 1.f, 1.f};
 #pragma unroll
     for (int i = 0; i <= NT; ++i) {
@@ -299,9 +306,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
         __builtin_amdgcn_sched_barrier(0);
       }
       Frag next = b1;
-      if (i + 2 < NT) next = frag(lb + (i + 2) * 2048);
+      if (i + 2 < NT) next = b_frag(i + 2);
       f32x4 sn = sb4;
-      if (!SQUARE && i < NT) sn = *(const f32x4*)(ls + BM + wn + i * 16 + g * 4);
+      if (!SQUARE && i < NT) sn = *(const f32x4*)(ls + BM + wn + (i >> 1) * 32 + g * 8 + (i & 1) * 4);
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
         f32x4 t = r[j];
@@ -342,9 +349,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
     if (mr < p.m) {
       O* o = (O*)p.out + mr * p.ldo;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int nc = n0 + wn + i * 16 + g * 4;
-        store4(o + nc, acc[i][j], p.n - nc);
+      for (int i = 0; i < NT; i += 2) {
+        const int nc = n0 + wn + i * 16 + g * 8;
+        const float v[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
+        store8(o + nc, v, p.n - nc);
       }
     }
   }

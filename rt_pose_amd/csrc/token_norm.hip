@@ -122,13 +122,22 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
   }
   for (long row = (long)blockIdx.x * GROUPS + grp; row < p.rows; row += (long)gridDim.x * GROUPS) {
-    float s[NV][8], g[NV][8];
+    float s[NV][8], g[NV][8], d[NV][8];      // all of a row's loads at once: one trip to memory for it
     float sq = 0.f, gs = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (lane + i * LPR) * 8;
       load8(s[i], (const T*)p.s + row * p.s_rs + c, p.h - c);
       load8(g[i], (const T*)p.dy + row * p.dy_rs + c, p.h - c);
+    }
+    if (p.ds) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load8(d[i], (const T*)p.ds + row * p.ds_rs + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[i][j] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -142,15 +151,12 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (lane + i * LPR) * 8, n = p.h - c;
-      float d[8];
-      if (p.ds) load8(d, (const T*)p.ds + row * p.ds_rs + c, n);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         dw[i][j] += g[i][j] * s[i][j] * rho;
-        const float own = rho * (g[i][j] * wv[i][j] - s[i][j] * back);
-        d[j] = p.ds ? own + d[j] : own;
+        d[i][j] += rho * (g[i][j] * wv[i][j] - s[i][j] * back);
       }
-      store8((T*)p.dx + row * p.h + c, d, n);
+      store8((T*)p.dx + row * p.h + c, d[i], n);
     }
   }
   if constexpr (GROUPS > 1) {
@@ -251,12 +257,14 @@ extern "C" int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res
   return norm_forward<true>(p, dtype, w_dtype, (hipStream_t)stream);
 }
 
-// partial rows of dw: two workgroups per CU walk the rows, fewer where there are fewer
+// partial rows of dw: four workgroups per CU walk the rows where a wave takes one (20480 x 1024: 34.5 us, with two 39.4), two where a workgroup does
+// (their partial rows are longer: 2048 x 8192 37.4 us, with four 46.2), fewer where there are fewer rows
 extern "C" int rtp_rmsnorm_backward_slots(long rows, int h) {
   if (rows < 1 || h < 1 || h > NORM_MAX_H) return 0;
   const int groups = h <= 128 ? 16 : h <= 2048 ? 4 : 1;
   const long need = (rows + groups - 1) / groups;
-  return (int)(need < 512 ? need : 512);
+  const long most = h <= 2048 ? 1024 : 512;
+  return (int)(need < most ? need : most);
 }
 
 extern "C" int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int w_dtype, const void* dy, long dy_rs, const void* ds, long ds_rs,
@@ -340,64 +348,88 @@ __global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
   if (threadIdx.x == 0) p.scale[blockIdx.x] = a / RTP_FP8_MAX;
 }
 
-// Either block, x given by columns (a transpose's view: x[r][c] at c * x_rs + r).  A tile of 128 rows x 128 columns goes through LDS:
-// read along the columns' memory order, then each thread takes 64 columns of one row -- neighbouring lanes take neighbouring rows, so the
-// reads of a wave are consecutive halves -- and writes them as 64 bytes.  The pitch keeps the 16-byte stores aligned.
+// Either block, x given by columns (a transpose's view: x[r][c] at c * x_rs + r).  A tile of 128 rows x 128 columns goes through LDS twice: read
+// along the columns' memory order, taken by each thread as 32 columns of two neighbouring rows (one LDS word a column for 16-bit types, held in
+// registers from the maximum to the output), and the bytes once more so that they leave as whole rows.
 template <typename T, bool SQUARE>
 __global__ __launch_bounds__(256) void quant_turned_kernel(QuantParams p) {
-  constexpr int PITCH = 128 + 16 / sizeof(T);
+  constexpr int PITCH = 128 + 16 / sizeof(T), QPITCH = 144;     // keep 16-byte accesses aligned and rows apart
+  typedef T tv2 __attribute__((ext_vector_type(2)));
   __shared__ __attribute__((aligned(16))) T tile[128 * PITCH];
-  __shared__ float red[256];
-  const int b = blockIdx.x % (unsigned)p.kb;
-  const long row0 = (long)(blockIdx.x / (unsigned)p.kb) * 128;
+  __shared__ float red[4][128];
+  // workgroups go round the 8 XCDs: tiles of neighbouring rows, which share the lines at their border, follow each other on one of them
+  const unsigned rt = (unsigned)((p.rows + 127) >> 7), at = blockIdx.x >> 3;
+  const int b = (int)(at / rt) * 8 + (blockIdx.x & 7), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long row0 = (long)(at % rt) * 128;
+  if (b >= p.kb) return;
   {
     const int ch = (threadIdx.x & 15) * 8;
     const long left = p.rows - row0 - ch;
     const int n = left < 0 ? 0 : left > 8 ? 8 : (int)left;
+    float v[8][8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const int c = (threadIdx.x >> 4) + u * 16;
-      float v[8];
-      load8(v, (const T*)p.x + (long)(b * 128 + c) * p.x_rs + row0 + ch, b * 128 + c < p.cols ? n : 0);
-      store8(tile + c * PITCH + ch, v, 8);
+      load8(v[u], (const T*)p.x + (long)(b * 128 + c) * p.x_rs + row0 + ch, b * 128 + c < p.cols ? n : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) store8(tile + ((threadIdx.x >> 4) + u * 16) * PITCH + ch, v[u], 8);
+  }
+  __syncthreads();
+  float v[2][32], a[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const tv2 x = *(const tv2*)(tile + (wave * 32 + c) * PITCH + 2 * lane);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      v[e][c] = (float)x[e];
+      a[e] = fmaxf(a[e], fabsf(v[e][c]));
+    }
+  }
+  float up[2], top[2];
+  if constexpr (SQUARE) {
+    float m = fmaxf(a[0], a[1]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    top[0] = top[1] = fmaxf(fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])), RTP_FP8_AMAX_FLOOR);
+    if (threadIdx.x == 0) p.scale[(row0 >> 7) * p.kb + b] = top[0] / RTP_FP8_MAX;
+  } else {
+    red[wave][2 * lane] = a[0];
+    red[wave][2 * lane + 1] = a[1];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 2 * lane + e;
+      top[e] = fmaxf(fmaxf(fmaxf(red[0][r], red[1][r]), fmaxf(red[2][r], red[3][r])), RTP_FP8_AMAX_FLOOR);
+      if (wave == 0 && row0 + r < p.rows) p.scale[(row0 + r) * p.kb + b] = top[e] / RTP_FP8_MAX;
+    }
+  }
+  // every thread has read the tile (the barrier above): the bytes take its place
+  uint8_t* bytes = (uint8_t*)tile;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    up[e] = RTP_FP8_MAX / top[e];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float lo[8], hi[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lo[j] = v[e][16 * k + j];
+        hi[j] = v[e][16 * k + 8 + j];
+      }
+      const i32x2 l = to_fp8x8(lo, up[e]), h = to_fp8x8(hi, up[e]);
+      *(i32x4*)(bytes + (2 * lane + e) * QPITCH + wave * 32 + k * 16) = i32x4{l[0], l[1], h[0], h[1]};
     }
   }
   __syncthreads();
-  const int r = threadIdx.x & 127, half = threadIdx.x >> 7;
-  float a = 0.f;
-#pragma unroll 16
-  for (int c = 0; c < 64; ++c) a = fmaxf(a, fabsf((float)tile[(half * 64 + c) * PITCH + r]));
-  if constexpr (SQUARE) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  } else {
-    red[threadIdx.x] = a;
-    __syncthreads();
-    a = fmaxf(red[r], red[r + 128]);
+  for (int u = 0; u < 4; ++u) {
+    const int r = (threadIdx.x >> 3) + u * 32, c = (threadIdx.x & 7) * 16;
+    if (row0 + r < p.rows && b * 128 + c < p.cols)
+      *(i32x4*)(p.q + (row0 + r) * p.q_rs + b * 128 + c) = *(const i32x4*)(bytes + r * QPITCH + c);
   }
-  a = fmaxf(a, RTP_FP8_AMAX_FLOOR);
-  const float up = RTP_FP8_MAX / a;
-  if (row0 + r < p.rows) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = half * 64 + k * 16;
-      if (b * 128 + c < p.cols) {
-        float lo[8], hi[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          lo[j] = (float)tile[(c + j) * PITCH + r];
-          hi[j] = (float)tile[(c + 8 + j) * PITCH + r];
-        }
-        const i32x2 l = to_fp8x8(lo, up), h = to_fp8x8(hi, up);
-        *(i32x4*)(p.q + (row0 + r) * p.q_rs + b * 128 + c) = i32x4{l[0], l[1], h[0], h[1]};
-      }
-    }
-    if (!SQUARE && half == 0) p.scale[(row0 + r) * p.kb + b] = a / RTP_FP8_MAX;
-  }
-  if (SQUARE && threadIdx.x == 0) p.scale[blockIdx.x] = a / RTP_FP8_MAX;
 }
 
 extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, float* scale, long rows, int cols, int square, int dtype,
@@ -410,14 +442,14 @@ extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, l
   RtpProfScope prof(RTP_FAM_NORM, st);
   const int kb = (cols + 127) >> 7;
   QuantParams p{x, (uint8_t*)q, scale, x_rs, q_rs, rows, cols, kb};
-  const long tiles = ((rows + 127) >> 7) * kb, groups = ((rows + QUANT_ROWS - 1) / QUANT_ROWS) * kb;
-  if (tiles >= (1L << 31) || groups >= (1L << 31)) return RTP_ERR_SHAPE;
+  const long tiles = ((rows + 127) >> 7) * kb, turned_tiles = ((rows + 127) >> 7) * ((kb + 7) & ~7), groups = ((rows + QUANT_ROWS - 1) / QUANT_ROWS) * kb;
+  if (turned_tiles >= (1L << 31) || groups >= (1L << 31)) return RTP_ERR_SHAPE;
   auto go = [&](auto t) {
     typedef decltype(t) T;
     if (turned && square)
-      hipLaunchKernelGGL((quant_turned_kernel<T, true>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((quant_turned_kernel<T, true>), dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
     else if (turned)
-      hipLaunchKernelGGL((quant_turned_kernel<T, false>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((quant_turned_kernel<T, false>), dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
     else if (square)
       hipLaunchKernelGGL((quant_square_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, st, p);
     else

@@ -14,7 +14,6 @@ import torch
 from ._tokens import DTYPES, FP8, call, fp8_rows, p, rows_of, same_device
 
 
-@torch.no_grad()
 def quantize_fp8(x, block=(1, 128)):
     """x: [..., cols] of fp32, fp16 or bf16 (block (1, 128)), or [rows, cols] (block (128, 128)) -> q, scale.  Per block a = max(largest
     magnitude, 2^-100): q = e4m3(x * (448 / a)) rounded to nearest even, scale = a / 448.  NaN stay NaN and do not move the scale; a block
@@ -41,19 +40,18 @@ def _operand(q, what):
     add_rms_norm_fp8 return), a copy otherwise."""
     if q.dtype != FP8:
         raise NotImplementedError("matmul_fp8: %s must be float8_e4m3fn (got %s)" % (what, q.dtype))
-    rows, cols = q.shape
+    (rows, cols), (ld, step) = q.shape, q.stride()
     wide = -(-cols // 16) * 16
-    u = q.view(torch.uint8) if q.stride(-1) == 1 or cols == 1 else q.contiguous().view(torch.uint8)
-    ld = u.stride(0) if rows > 1 else max(u.stride(0), wide)
-    end = u.storage_offset() + (rows - 1) * ld + wide
-    if u.data_ptr() % 16 == 0 and ld % 16 == 0 and ld >= wide and end <= u.untyped_storage().nbytes():
-        return u, ld
+    if rows == 1:
+        ld = max(ld - ld % 16, wide)
+    if (step == 1 or cols == 1) and ld % 16 == 0 and ld >= wide and q.data_ptr() % 16 == 0 and (
+            wide == cols or q.storage_offset() + (rows - 1) * ld + wide <= q.untyped_storage().nbytes()):
+        return q, ld
     own = torch.empty(rows, wide, dtype=torch.uint8, device=q.device)
-    own[:, :cols].copy_(u)
+    own[:, :cols].copy_((q if step == 1 or cols == 1 else q.contiguous()).view(torch.uint8))
     return own, wide
 
 
-@torch.no_grad()
 def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16):
     """a: [..., m, k] and b: [n, k] in float8_e4m3fn -> [..., m, n]: the sum over k of (a * a_scale) * (b * b_scale) in fp32, rounded once to
     out_dtype (bf16, fp16 or fp32).  a_scale: [..., m, ceil(k / 128)]; b_scale: [ceil(n / 128), ceil(k / 128)] or [n, ceil(k / 128)]; both fp32.
@@ -63,19 +61,20 @@ def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16):
         raise NotImplementedError("matmul_fp8: out_dtype bf16, fp16 or fp32 (got %s)" % out_dtype)
     if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
         raise NotImplementedError("matmul_fp8: fp32 scales (got %s and %s)" % (a_scale.dtype, b_scale.dtype))
-    if a.dim() < 2 or b.dim() != 2 or a.shape[-1] != b.shape[-1] or b.shape[-1] < 1:
+    lead = a.shape[:-1]
+    if len(lead) < 1 or b.dim() != 2 or a.shape[-1] != b.shape[-1] or b.shape[-1] < 1:
         raise ValueError("matmul_fp8: [..., m, k] and [n, k] expected (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
     k, n = b.shape[1], b.shape[0]
     kb, nb = -(-k // 128), -(-n // 128)
-    if a_scale.shape != (*a.shape[:-1], kb):
-        raise ValueError("matmul_fp8: a_scale of shape %s expected (got %s)" % ((*a.shape[:-1], kb), tuple(a_scale.shape)))
+    if a_scale.shape != (*lead, kb):
+        raise ValueError("matmul_fp8: a_scale of shape %s expected (got %s)" % ((*lead, kb), tuple(a_scale.shape)))
     if b_scale.shape not in ((nb, kb), (n, kb)):
         raise ValueError("matmul_fp8: b_scale of shape %s or %s expected (got %s)" % ((nb, kb), (n, kb), tuple(b_scale.shape)))
-    out = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=a.device)
+    out = torch.empty((*lead, n), dtype=out_dtype, device=a.device)
     if out.numel() == 0:
         return out
-    a2, lda = _operand(a.reshape(-1, k), "a")
+    a2, lda = _operand(a if len(lead) == 1 else a.reshape(-1, k), "a")
     b2, ldb = _operand(b, "b")
-    sa, sb = a_scale.reshape(-1, kb).contiguous(), b_scale.contiguous()
+    sa, sb = a_scale.contiguous(), b_scale.contiguous()
     call("rtp_matmul_fp8", a, p(a2), lda, p(sa), p(b2), ldb, p(sb), int(b_scale.shape[0] == nb), p(out), a2.shape[0], n, k, DTYPES[out_dtype])
     return out

@@ -13,22 +13,22 @@ a failing native call -> RtpError.
 import torch
 import torch.nn as nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._tokens import DTYPES, call, fp8_rows, p, rows_of, same_device
+from ._tokens import DTYPES, call, fp8_rows, like, once, p, rows_of, same_device
 
 
 def _check(x, residual, weight):
     same_device(x, residual, weight)
     if x.dtype not in DTYPES:
         raise NotImplementedError("rms norm: fp32, fp16 or bf16 rows only (got %s)" % x.dtype)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("rms norm: rows of at least one column expected (got shape %s)" % (tuple(x.shape),))
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError("rms norm: rows of at least one column expected (got shape %s)" % (tuple(shape),))
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("rms norm: the residual must have x's shape and type (got %s %s beside %s %s)"
                          % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))
-    if weight.shape != x.shape[-1:]:
+    if weight.shape != shape[-1:]:
         raise ValueError("rms norm: weight of shape (%d,) expected (got %s)" % (x.shape[-1], tuple(weight.shape)))
     if weight.dtype != x.dtype and weight.dtype != torch.float32:
         raise NotImplementedError("rms norm: weight in x's type or fp32 (got %s beside %s)" % (weight.dtype, x.dtype))
@@ -37,7 +37,7 @@ def _check(x, residual, weight):
 def _forward(x, residual, weight, eps):
     x2, w = rows_of(x), weight.contiguous()
     r2 = rows_of(residual) if residual is not None else None
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = like(x)
     s = torch.empty_like(y) if residual is not None else None
     call("rtp_rmsnorm_forward", x, p(x2), x2.stride(0), p(r2), 0 if r2 is None else r2.stride(0), p(w), DTYPES[w.dtype], p(y), p(s), *x2.shape,
          DTYPES[x.dtype], eps)
@@ -48,11 +48,11 @@ def _backward(s, weight, eps, dy, ds, need_w):
     """dx (also the residual's gradient) and dw of the rows `s` that were normed."""
     s2, w = rows_of(s), weight.contiguous()
     rows, h = s2.shape
-    dx, dw = torch.empty_like(s, memory_format=torch.contiguous_format), torch.empty_like(w)
+    dx, dw = like(s), torch.empty_like(w)
     if rows == 0:
         return dx, dw.zero_() if need_w else None
     dy2, ds2 = rows_of(dy), rows_of(ds) if ds is not None else None
-    part = torch.empty(_lib.load().rtp_rmsnorm_backward_slots(rows, h) * h, dtype=torch.float32, device=s.device)
+    part = s.new_empty(_lib.load().rtp_rmsnorm_backward_slots(rows, h) * h, dtype=torch.float32)
     call("rtp_rmsnorm_backward", s, p(s2), s2.stride(0), p(w), DTYPES[w.dtype], p(dy2), dy2.stride(0), p(ds2), 0 if ds2 is None else ds2.stride(0),
          p(dx), p(dw), p(part), rows, h, DTYPES[s.dtype], eps)
     return dx, dw if need_w else None
@@ -66,7 +66,7 @@ class RMSNormFunction(Function):
         return _forward(x, None, weight, eps)[0]
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         x, weight = ctx.saved_tensors
         dx, dw = _backward(x, weight, ctx.eps, dy, None, ctx.needs_input_grad[1])
@@ -83,7 +83,7 @@ class AddRMSNormFunction(Function):
         return y, s
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy, ds):
         s, weight = ctx.saved_tensors
         if dy is None:                  # only the stream was used
@@ -104,7 +104,6 @@ def add_rms_norm(x, residual, weight, eps=1e-6):
     return AddRMSNormFunction.apply(x, residual, weight, float(eps))
 
 
-@torch.no_grad()
 def add_rms_norm_fp8(x, residual, weight, eps=1e-6):
     """For serving: the normed rows in 8 bits and their scales, as rt_pose_amd.fp8.matmul_fp8 reads them, and the stream.  residual may be
     None (the stream is x itself).  The value that is quantised is the fp32 one.  Not differentiable: the outputs carry no gradient."""

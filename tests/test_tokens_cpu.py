@@ -40,7 +40,7 @@ def test_norm_entries_check_before_they_launch():
     assert lib.rtp_rmsnorm_backward_slots(0, 8) == 0 and lib.rtp_rmsnorm_backward_slots(1, 8) == 1
     for rows in (1, 17, 20000, 10 ** 6):
         for h in (1, 128, 129, 2048, 2049, 16384):
-            assert 1 <= lib.rtp_rmsnorm_backward_slots(rows, h) <= min(rows, 512)
+            assert 1 <= lib.rtp_rmsnorm_backward_slots(rows, h) <= min(rows, 1024)
 
 
 def test_8_bit_entries_check_before_they_launch():
