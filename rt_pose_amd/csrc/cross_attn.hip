@@ -213,6 +213,26 @@ __device__ __forceinline__ void xa_load_row(typename Vec8<T>::type (&f)[2 * DT],
   }
 }
 
+// Sixteen accumulators of a lane -- columns 32 t + 8 (i / 4) + 4 h + i % 4 of one row -- rounded and stored: the half waves swap four columns each, and
+// a lane then holds eight neighbouring ones.
+template <typename T>
+__device__ __forceinline__ void xa_store(T* row, const f32x16& x, float mul, int t, int h, int d, bool ok) {
+  typedef T tv2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    unsigned a[2], b[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const tv2 lo = {(T)(x[8 * j + 2 * e] * mul), (T)(x[8 * j + 2 * e + 1] * mul)}, hi = {(T)(x[8 * j + 4 + 2 * e] * mul), (T)(x[8 * j + 5 + 2 * e] * mul)};
+      const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+      a[e] = r[0];
+      b[e] = r[1];
+    }
+    const int c = 32 * t + 16 * j + 8 * h;
+    if (ok && c < d) *(i32x4*)(row + c) = i32x4{(int)a[0], (int)a[1], (int)b[0], (int)b[1]};
+  }
+}
+
 #define XA_M0 (-3.402823466e38f)
 #define XA_SLACK 8.0f   // the running maximum moves only when it is exceeded by 2^8: p stays below 2^8, and most tiles rescale nothing
 
@@ -258,11 +278,12 @@ __device__ __forceinline__ void xa_settle() { __builtin_amdgcn_s_waitcnt(0x0F70)
 template <int N>
 __device__ __forceinline__ void xa_landed() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-template <typename T, int DT, int KW, typename F>
+// ALL: tiles without a key that counts too (gradients are written for every key).
+template <typename T, int DT, int KW, bool ALL, typename F>
 __device__ __forceinline__ void xa_over_keys(const XaParams& p, uint8_t* lds, int b, int hk, int split, bool busy, F compute) {
   typedef XaKeys<DT, KW> K;
   constexpr int BK = K::BK, NW = K::NW, NBUF = K::NBUF, IMG = K::IMG, PER = 2 * BK / XaLoader<DT, T>::ROWS;
-  const int len = xa_len(p, b), nt = (len + BK - 1) / BK;
+  const int len = xa_len(p, b), nt = ((ALL ? p.sk : len) + BK - 1) / BK;
   const int t0 = (int)((long)nt * split / p.nsplit), t1 = (int)((long)nt * (split + 1) / p.nsplit);
   if (t0 >= t1) return;
   const T* kp = (const T*)p.k + (long)b * p.k_bs + (long)hk * p.k_hs;
@@ -298,7 +319,7 @@ __device__ __forceinline__ void xa_over_keys(const XaParams& p, uint8_t* lds, in
     if (NBUF == 3 && t + 1 < t1) xa_landed<PER>();
     else xa_landed<0>();
     if (t + NBUF - 1 < t1) stage(t + NBUF - 1, lds + fill, w[NBUF - 1]);
-    if (busy) compute(lds + use, lds + use + IMG, w[0]);
+    if (busy) compute(t, lds + use, lds + use + IMG, w[0]);
     use = use + 2 * IMG == K::BYTES ? 0 : use + 2 * IMG;
     fill = fill + 2 * IMG == K::BYTES ? 0 : fill + 2 * IMG;
 #pragma unroll
@@ -350,7 +371,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = XA_M0, l = 0.f;
 
-  xa_over_keys<T, DT, KW>(p, lds, b, hk, split, r0 < p.rows, [&](const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  xa_over_keys<T, DT, KW, false>(p, lds, b, hk, split, r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[SUB], any = 0, all = ~0u;
     xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
@@ -457,24 +478,15 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
     if (p.lse && h == 0) p.lse[row] = l == 0.f ? INFINITY : L;
     const int s = r / p.grp, g = r % p.grp;
     const long oo = (((long)b * p.sq + s) * p.hq + hk * p.grp + g) * p.d;
-    typedef T tv4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
+    for (int t = 0; t < DT; ++t) {
+      xa_store<T>((T*)p.o + oo, o[t], inv, t, h, p.d, true);
+      if (p.o_lo) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int c = 32 * t + 2 * i + 4 * h;
-        if (c < p.d) {
-          tv4 hi, lo;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = o[t][i + j] * inv;
-            hi[j] = (T)x;
-            lo[j] = (T)(x - (float)hi[j]);
-          }
-          *(tv4*)((T*)p.o + oo + c) = hi;
-          if (p.o_lo) *(tv4*)((T*)p.o_lo + oo + c) = lo;
-        }
+        for (int i = 0; i < 16; ++i) o[t][i] = o[t][i] * inv - (float)(T)(o[t][i] * inv);
+        xa_store<T>((T*)p.o_lo + oo, o[t], 1.f, t, h, p.d, true);
       }
+    }
   }
 }
 
@@ -565,6 +577,68 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XaParams p) {
   if (row < rows && (threadIdx.x & 15) == 0) p.delta[row] = t;
 }
 
+// delta = sum_d do o of this lane's row (do in df), from o as it was before its rounding (o + what the rounding left over): with few keys the
+// difference dp - delta cancels, and o's rounding alone would be most of it
+template <typename T, int DT>
+__device__ __forceinline__ float xa_delta(const XaParams& p, const typename Vec8<T>::type (&df)[2 * DT], int b, int hk, int r, bool rok, int h) {
+  const int tok = rok ? r / p.grp : 0, g = rok ? r % p.grp : 0;
+  const long oo = (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
+  typename Vec8<T>::type oh[2 * DT], ol[2 * DT];
+  xa_load_row<DT, T>(oh, (const T*)p.o + oo, rok, p.d, h);
+  xa_load_row<DT, T>(ol, (const T*)p.o_lo + oo, rok, p.d, h);
+  float delta = 0.f;
+#pragma unroll
+  for (int st = 0; st < 2 * DT; ++st)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) delta += ((float)oh[st][j] + (float)ol[st][j]) * (float)df[st][j];
+  return xa_halves_sum(delta);
+}
+
+// the sums of the KW waves that share rows, in wave order; the first of them has the whole
+template <int DT, int KW>
+__device__ __forceinline__ void xa_join_waves(f32x16 (&acc)[DT], uint8_t* lds, int wave) {
+  if constexpr (KW > 1) {
+    const int kw = wave % KW, lane = threadIdx.x & 63;
+    constexpr int SLOT = DT * 16 * 64;
+    float* y = (float*)lds + (wave / KW) * (KW - 1) * SLOT + lane;
+    __syncthreads();
+    if (kw > 0) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) y[(kw - 1) * SLOT + (t * 16 + i) * 64] = acc[t][i];
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int k = 1; k < KW; ++k)
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] += y[(k - 1) * SLOT + (t * 16 + i) * 64];
+  }
+}
+
+// the gradient of row r of q, or this split's part of it
+template <typename T, int DT>
+__device__ __forceinline__ void xa_store_dq(const XaParams& p, const f32x16 (&acc)[DT], int b, int hk, int split, int r, int h) {
+  if (p.nsplit > 1) {
+    float* po = p.part + (((long)split * p.b * p.hkv + (long)b * p.hkv + hk) * p.rows + r) * p.d;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int c = 32 * t + 2 * i + 4 * h;
+        if (c < p.d) *(f32x4*)(po + c) = f32x4{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
+      }
+  } else {
+    const int tok = r / p.grp, g = r % p.grp;
+    T* to = (T*)p.dq + (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) xa_store<T>(to, acc[t], 1.f, t, h, p.d, true);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------ backward: dq
 // the forward kernel's shape: s^T and dp^T with a lane per row, dq^T = k^T ds^T, k read from LDS both ways
 template <typename T, int DT, int KW>
@@ -584,29 +658,15 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
   xa_load_row<DT, T>(qf, (const T*)p.q + (long)b * p.q_bs + (long)(hk * p.grp) * p.q_hs + (rok ? xa_row_off(p, r, p.q_ss, p.q_hs) : 0), rok, p.d, h);
   xa_load_row<DT, T>(df, (const T*)p.d_o + (long)b * p.o_bs + (long)(hk * p.grp) * p.o_hs + (rok ? xa_row_off(p, r, p.o_ss, p.o_hs) : 0), rok, p.d, h);
   float ex = XaRange<T>::BWD, L = (rok ? p.lse_in[row] : INFINITY) - ex;     // p times 2^ex
-  // delta = sum_d do o of this lane's row, from o as it was before its rounding (o + what the rounding left over): with few keys the difference
-  // dp - delta cancels, and o's rounding alone would be most of it.  It is left for the gradients of k and v too (every split the same value).
-  float delta = 0.f;
-  {
-    const int tok = rok ? r / p.grp : 0, g = rok ? r % p.grp : 0;
-    const long oo = (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
-    V oh[2 * DT], ol[2 * DT];
-    xa_load_row<DT, T>(oh, (const T*)p.o + oo, rok, p.d, h);
-    xa_load_row<DT, T>(ol, (const T*)p.o_lo + oo, rok, p.d, h);
-#pragma unroll
-    for (int st = 0; st < 2 * DT; ++st)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) delta += ((float)oh[st][j] + (float)ol[st][j]) * (float)df[st][j];
-    delta = xa_halves_sum(delta);
-    if (rok && h == 0 && kw == 0) p.delta[row] = delta;
-  }
+  const float delta = xa_delta<T, DT>(p, df, b, hk, r, rok, h);      // left for the gradients of k and v too (every split the same value)
+  if (rok && h == 0 && kw == 0) p.delta[row] = delta;
   f32x16 acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  xa_over_keys<T, DT, KW>(p, lds, b, hk, split, r0 < p.rows, [&](const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  xa_over_keys<T, DT, KW, false>(p, lds, b, hk, split, r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[SUB], any = 0;
     xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
@@ -626,7 +686,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
         s[u] = mfma32(xa_frag<V>(ki + u * 32 * PITCH, ad.row[st]), qf[st], s[u]);
         dp[u] = mfma32(xa_frag<V>(vi + u * 32 * PITCH, ad.row[st]), df[st], dp[u]);
       }
-    XaSecond<T, KW == 4> ds[SUB];
+    XaSecond<T, false> ds[SUB];
 #pragma unroll
     for (int u = 0; u < SUB; ++u) {
       if (w[u] != ~0u) xa_mask(s[u], w[u], h);
@@ -658,7 +718,6 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
 #pragma unroll
         for (int t2 = 0; t2 < DT; ++t2) {
           const V f = xa_frag_tr<V>(ki + (u * 32 + c * 16) * PITCH, ad.tr[t2][0], ad.tr[t2][1]);
-          if constexpr (KW == 4) acc[t2] = mfma32(f, ds[u].v[2 + c], acc[t2]);
           acc[t2] = mfma32(f, ds[u].v[c], acc[t2]);
         }
   });
@@ -667,48 +726,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
   for (int t = 0; t < DT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] *= out;
-  if constexpr (KW > 1) {
-    __syncthreads();
-    float* x = (float*)lds;
-    constexpr int SLOT = DT * 16 * 64;
-    if (kw > 0) {
-      float* y = x + ((wave / KW) * (KW - 1) + kw - 1) * SLOT + lane;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[(t * 16 + i) * 64] = acc[t][i];
-    }
-    __syncthreads();
-    if (kw > 0) return;
-#pragma unroll
-    for (int k = 1; k < KW; ++k) {
-      const float* y = x + ((wave / KW) * (KW - 1) + k - 1) * SLOT + lane;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[t][i] += y[(t * 16 + i) * 64];
-    }
-  }
-  if (!rok) return;
-  typedef T tv4 __attribute__((ext_vector_type(4)));
-  const int s = r / p.grp, g = r % p.grp;
-  const long oo = (((long)b * p.sq + s) * p.hq + hk * p.grp + g) * p.d;
-  float* po = p.part + ((long)split * p.b * p.hkv * p.rows + row) * p.d;
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int c = 32 * t + 2 * i + 4 * h;
-      if (c < p.d) {
-        const f32x4 v = {acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
-        if (p.nsplit > 1) {
-          *(f32x4*)(po + c) = v;
-        } else {
-          const tv4 z = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-          *(tv4*)((T*)p.dq + oo + c) = z;
-        }
-      }
-    }
+  xa_join_waves<DT, KW>(acc, lds, wave);
+  if (kw == 0 && rok) xa_store_dq<T, DT>(p, acc, b, hk, split, r, h);
 }
 
 // dq of a row = sum over splits
@@ -739,7 +758,7 @@ __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
 template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane of the wave that brings their L or delta; two buffers
   static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, BYTES = 2 * BUF;
 };
-template <typename T, int DT, bool LO>
+template <typename T, int DT>
 __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
   typedef XaRows<DT> R;
@@ -803,7 +822,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
         s = mfma32(xa_frag<V>(qi + u * 32 * XaImg<DT>::PITCH, ad.row[e]), kf[e], s);
         dp = mfma32(xa_frag<V>(di + u * 32 * XaImg<DT>::PITCH, ad.row[e]), vf[e], dp);
       }
-      XaSecond<T, LO> pb, sb;
+      XaSecond<T, false> pb, sb;
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
         const f32x4 L = *(const f32x4*)(st + u * 32 + 2 * i + 4 * h), dl = *(const f32x4*)(st + BR + u * 32 + 2 * i + 4 * h);
@@ -826,10 +845,6 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
         for (int t2 = 0; t2 < DT; ++t2) {
           const int off = (u * 32 + c * 16) * XaImg<DT>::PITCH;
           const V df = xa_frag_tr<V>(di + off, ad.tr[t2][0], ad.tr[t2][1]), qf = xa_frag_tr<V>(qi + off, ad.tr[t2][0], ad.tr[t2][1]);
-          if constexpr (LO) {
-            dv[t2] = mfma32(df, pb.v[2 + c], dv[t2]);
-            dk[t2] = mfma32(qf, sb.v[2 + c], dk[t2]);
-          }
           dv[t2] = mfma32(df, pb.v[c], dv[t2]);
           dk[t2] = mfma32(qf, sb.v[c], dk[t2]);
         }
@@ -844,31 +859,173 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
   }
   if (key >= p.sk) return;
   const float k_out = p.scale * exp2f(-ex), v_out = exp2f(-XaRange<T>::BWD);
-  typedef T tv4 __attribute__((ext_vector_type(4)));
   const long oo = (((long)b * p.sk + key) * p.hkv + hk) * p.d;
   const long all = (long)p.b * p.sk * p.hkv * p.d;
 #pragma unroll
-  for (int t = 0; t < DT; ++t)
+  for (int t = 0; t < DT; ++t) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int c = 32 * t + 2 * i + 4 * h;
-      if (c < p.d) {
-        f32x4 x, y;
+    for (int i = 0; i < 16; ++i) {     // a key that does not count: zeros, whatever the products made of its column
+      dk[t][i] = kok ? dk[t][i] * k_out : 0.f;
+      dv[t][i] = kok ? dv[t][i] * v_out : 0.f;
+    }
+    if (p.nsplit > 1) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = kok ? dk[t][i + j] * k_out : 0.f;
-          y[j] = kok ? dv[t][i + j] * v_out : 0.f;
-        }
-        if (p.nsplit > 1) {
-          *(f32x4*)(p.part + (2L * split) * all + oo + c) = x;
-          *(f32x4*)(p.part + (2L * split + 1) * all + oo + c) = y;
-        } else {
-          const tv4 zx = {(T)x[0], (T)x[1], (T)x[2], (T)x[3]}, zy = {(T)y[0], (T)y[1], (T)y[2], (T)y[3]};
-          *(tv4*)((T*)p.dk + oo + c) = zx;
-          *(tv4*)((T*)p.dv + oo + c) = zy;
+      for (int i = 0; i < 16; i += 4) {
+        const int c = 32 * t + 2 * i + 4 * h;
+        if (c < p.d) {
+          *(f32x4*)(p.part + (2L * split) * all + oo + c) = f32x4{dk[t][i], dk[t][i + 1], dk[t][i + 2], dk[t][i + 3]};
+          *(f32x4*)(p.part + (2L * split + 1) * all + oo + c) = f32x4{dv[t][i], dv[t][i + 1], dv[t][i + 2], dv[t][i + 3]};
         }
       }
+    } else {
+      xa_store<T>((T*)p.dk + oo, dk[t], 1.f, t, h, p.d, true);
+      xa_store<T>((T*)p.dv + oo, dv[t], 1.f, t, h, p.d, true);
     }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward, up to 32 rows
+// All rows are one tile, so a tile of keys is done with once read: its dk and dv are complete, and dq is summed on.  One pass over k and v, which
+// are the work (heads of 32, 15 rows x 20480 keys: dq and dk / dv by the kernels above 105 us, here XXX).  Each wave takes 32 keys of a tile both
+// ways round from the same fragments, operands exchanged: a lane per row for ds^T and dq, a lane per key for p, ds and dk / dv.
+template <int DT> struct XaFew {       // key tiles, then the images of do and q, then L and delta of the rows
+  static constexpr int ROWS_IMG = 32 * XaImg<DT>::PITCH, AT = XaKeys<DT, 4>::BYTES, BYTES = AT + 2 * ROWS_IMG + 2 * 32 * 4;
+};
+template <typename T, int DT>
+__global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_bwd_few_kernel(XaParams p) {
+  typedef typename Vec8<T>::type V;
+  constexpr int NW = XaKeys<DT, 4>::NW, PITCH = XaImg<DT>::PITCH;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  int tile, b, hk, split;
+  if (!xa_place(p, tile, b, hk, split)) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bh = b * p.hkv + hk, h = lane >> 5, r = lane & 31;
+  const bool rok = r < p.rows;
+  const XaAddr<DT> ad(lane);
+  const long row = (long)bh * p.rows + r;
+  V qf[2 * DT], df[2 * DT];
+  xa_load_row<DT, T>(qf, (const T*)p.q + (long)b * p.q_bs + (long)(hk * p.grp) * p.q_hs + (rok ? xa_row_off(p, r, p.q_ss, p.q_hs) : 0), rok, p.d, h);
+  xa_load_row<DT, T>(df, (const T*)p.d_o + (long)b * p.o_bs + (long)(hk * p.grp) * p.o_hs + (rok ? xa_row_off(p, r, p.o_ss, p.o_hs) : 0), rok, p.d, h);
+  const float delta = xa_delta<T, DT>(p, df, b, hk, r, rok, h), L0 = rok ? p.lse_in[row] : INFINITY;
+  float ex = XaRange<T>::BWD, L = L0 - ex;
+  uint8_t *di = lds + XaFew<DT>::AT, *qi = di + XaFew<DT>::ROWS_IMG;
+  float* st = (float*)(qi + XaFew<DT>::ROWS_IMG);
+  if (wave == 0) {       // the rows once more as images, and their statistics, for the other way round
+#pragma unroll
+    for (int e = 0; e < 2 * DT; ++e) {
+      *(V*)(di + ad.row[e]) = df[e];
+      *(V*)(qi + ad.row[e]) = qf[e];
+    }
+    if (h == 0) {
+      st[r] = L0 - XaRange<T>::BWD;
+      st[32 + r] = delta;
+    }
+  }
+  __syncthreads();
+  f32x16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
+
+  xa_over_keys<T, DT, 4, true>(p, lds, b, hk, split, true, [&](int t, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+    unsigned w[1];
+    xa_mine<4, NW>(words, wave, w);
+    const int key = t * 128 + wave * 32 + r;
+    const long oo = (((long)b * p.sk + key) * p.hkv + hk) * p.d;
+    const bool in = key < p.sk, kok = (w[0] >> r) & 1u;
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dk[t2][i] = dv[t2][i] = 0.f;
+    if (w[0] != 0) {
+      ki += wave * 32 * PITCH;
+      vi += wave * 32 * PITCH;
+      f32x16 s, dp, s2, d2;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = dp[i] = s2[i] = d2[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 2 * DT; ++e) {
+        const V kf = xa_frag<V>(ki, ad.row[e]), vf = xa_frag<V>(vi, ad.row[e]);
+        s = mfma32(kf, qf[e], s);
+        dp = mfma32(vf, df[e], dp);
+        s2 = mfma32(qf[e], kf, s2);
+        d2 = mfma32(df[e], vf, d2);
+      }
+      // a lane per row: dq
+      if (w[0] != ~0u) xa_mask(s, w[0], h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dp[i] = __builtin_amdgcn_exp2f(s[i] * p.scale_log2 - L) * (dp[i] - delta);
+      if constexpr (XaRange<T>::NARROW) {
+        const float before = ex;
+        if (xa_narrow<DT>(dp, acc, ex)) L += before - ex;
+      }
+      XaSecond<T, true> ds, pb, sb;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ds.set(i, dp[i]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t2 = 0; t2 < DT; ++t2) {
+          const V f = xa_frag_tr<V>(ki + c * 16 * PITCH, ad.tr[t2][0], ad.tr[t2][1]);
+          acc[t2] = mfma32(f, ds.v[2 + c], acc[t2]);
+          acc[t2] = mfma32(f, ds.v[c], acc[t2]);
+        }
+      // a lane per key: dk, dv
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const f32x4 Lr = *(const f32x4*)(st + 2 * i + 4 * h), dl = *(const f32x4*)(st + 32 + 2 * i + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = __builtin_amdgcn_exp2f(s2[i + j] * p.scale_log2 - Lr[j]);
+          pb.set(i + j, e);
+          d2[i + j] = e * (d2[i + j] - dl[j]);
+        }
+      }
+      float k_out = p.scale;
+      if constexpr (XaRange<T>::NARROW) {
+        float kx = XaRange<T>::BWD;
+        xa_narrow<DT>(d2, dk, kx);
+        k_out *= exp2f(-kx);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sb.set(i, d2[i]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int t2 = 0; t2 < DT; ++t2) {
+          const V f = xa_frag_tr<V>(di + c * 16 * PITCH, ad.tr[t2][0], ad.tr[t2][1]), g = xa_frag_tr<V>(qi + c * 16 * PITCH, ad.tr[t2][0], ad.tr[t2][1]);
+          dv[t2] = mfma32(f, pb.v[2 + c], dv[t2]);
+          dv[t2] = mfma32(f, pb.v[c], dv[t2]);
+          dk[t2] = mfma32(g, sb.v[2 + c], dk[t2]);
+          dk[t2] = mfma32(g, sb.v[c], dk[t2]);
+        }
+      const float v_out = exp2f(-XaRange<T>::BWD);
+#pragma unroll
+      for (int t2 = 0; t2 < DT; ++t2)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {     // a key that does not count: zeros, whatever the products made of its column
+          dk[t2][i] = kok ? dk[t2][i] * k_out : 0.f;
+          dv[t2][i] = kok ? dv[t2][i] * v_out : 0.f;
+        }
+    }
+    if (p.dk) {
+#pragma unroll
+      for (int t2 = 0; t2 < DT; ++t2) {
+        xa_store<T>((T*)p.dk + oo, dk[t2], 1.f, t2, h, p.d, in);
+        xa_store<T>((T*)p.dv + oo, dv[t2], 1.f, t2, h, p.d, in);
+      }
+    }
+  });
+  if (!p.dq) return;
+  const float out = p.scale * exp2f(-ex);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] *= out;
+  xa_join_waves<DT, 4>(acc, lds, wave);
+  if (wave == 0 && rok) xa_store_dq<T, DT>(p, acc, b, hk, split, r, h);
 }
 
 // dk and dv = sums over the splits of the rows, in their order; the splits lie 2 * all floats apart, dk and dv in turn
@@ -1008,10 +1165,15 @@ static int xa_dq(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
   return xa_launch(xattn_dq_kernel<T, DT, KW>, grid, XaKeys<DT, KW>::BYTES, once, st, p);
 }
-template <typename T, int DT, bool LO>
+template <typename T, int DT>
 static int xa_dkv(int grid, hipStream_t st, const XaParams& p) {
   static bool once[RTP_MAX_DEVICES];
-  return xa_launch(xattn_dkv_kernel<T, DT, LO>, grid, XaRows<DT>::BYTES, once, st, p);
+  return xa_launch(xattn_dkv_kernel<T, DT>, grid, XaRows<DT>::BYTES, once, st, p);
+}
+template <typename T, int DT>
+static int xa_bwd_few(int grid, hipStream_t st, const XaParams& p) {
+  static bool once[RTP_MAX_DEVICES];
+  return xa_launch(xattn_bwd_few_kernel<T, DT>, grid, XaFew<DT>::BYTES, once, st, p);
 }
 
 extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* lse, void* ws, long ws_bytes, void* stream) {
@@ -1077,20 +1239,26 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
   return xa_types(a, [&](auto t, auto dt) {
     typedef decltype(t) T;
     constexpr int DT = decltype(dt)::value;
+    auto join_dq = [&]() {
+      if (pl.nsplit > 1) hipLaunchKernelGGL((xattn_dq_join_kernel<T>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
+      RTP_CHECK_LAUNCH();
+      return RTP_OK;
+    };
+    if (pl.kw == 4) {
+      const int grid = xa_grid(p, pl.tiles, pl.nsplit), r = xa_bwd_few<T, DT>(grid, st, p);
+      return r != RTP_OK || !dq ? r : join_dq();
+    }
     if (!dq) {
       hipLaunchKernelGGL((xattn_delta_kernel<T>), dim3(rtp_div_up(rows, 16)), dim3(256), 0, st, p);
       RTP_CHECK_LAUNCH();
     } else {
       const int grid = xa_grid(p, pl.tiles, pl.nsplit);
-      const int r = pl.kw == 4 ? xa_dq<T, DT, 4>(grid, st, p) : pl.kw == 2 ? xa_dq<T, DT, 2>(grid, st, p) : xa_dq<T, DT, 1>(grid, st, p);
+      int r = pl.kw == 2 ? xa_dq<T, DT, 2>(grid, st, p) : xa_dq<T, DT, 1>(grid, st, p);
+      if (r == RTP_OK) r = join_dq();
       if (r != RTP_OK) return r;
-      if (pl.nsplit > 1) {
-        hipLaunchKernelGGL((xattn_dq_join_kernel<T>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
-        RTP_CHECK_LAUNCH();
-      }
     }
     if (!dk) return RTP_OK;
-    const int grid = xa_grid(p, pl.ktiles, pl.ksplit), r = pl.kw == 4 ? xa_dkv<T, DT, true>(grid, st, p) : xa_dkv<T, DT, false>(grid, st, p);
+    const int grid = xa_grid(p, pl.ktiles, pl.ksplit), r = xa_dkv<T, DT>(grid, st, p);
     if (r != RTP_OK) return r;
     if (pl.ksplit > 1) {
       const long all = (long)a->b * a->sk * a->hkv * a->d;
