@@ -213,23 +213,74 @@ __device__ __forceinline__ void xa_load_row(typename Vec8<T>::type (&f)[2 * DT],
   }
 }
 
-// Sixteen accumulators of a lane -- columns 32 t + 8 (i / 4) + 4 h + i % 4 of one row -- rounded and stored: the half waves swap four columns each, and
-// a lane then holds eight neighbouring ones.
+// Eight accumulators of a lane -- columns 16 q + 8 (i / 4) + 4 h + i % 4 of one row, i < 8 -- rounded and stored: the half waves swap four columns
+// each, and a lane then holds eight neighbouring ones.
 template <typename T>
-__device__ __forceinline__ void xa_store(T* row, const f32x16& x, float mul, int t, int h, int d, bool ok) {
+__device__ __forceinline__ void xa_store8(T* row, const float (&x)[8], int q, int h, int d, bool ok) {
   typedef T tv2 __attribute__((ext_vector_type(2)));
+  unsigned a[2], b[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const tv2 lo = {(T)x[2 * e], (T)x[2 * e + 1]}, hi = {(T)x[4 + 2 * e], (T)x[5 + 2 * e]};
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
+    a[e] = r[0];
+    b[e] = r[1];
+  }
+  const int c = 16 * q + 8 * h;
+  if (ok && c < d) *(i32x4*)(row + c) = i32x4{(int)a[0], (int)a[1], (int)b[0], (int)b[1]};
+}
+// the same for partial results, which stay fp32
+__device__ __forceinline__ void xa_store8(float* row, const float (&x)[8], int q, int h, int d) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int c = 16 * q + 8 * e + 4 * h;
+    if (c < d) *(f32x4*)(row + c) = f32x4{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]};
+  }
+}
+// a whole accumulator: columns 32 t .. 32 t + 31
+template <typename T>
+__device__ __forceinline__ void xa_store(T* row, const f32x16& x, int t, int h, int d, bool ok) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    unsigned a[2], b[2];
+    const float y[8] = {x[8 * j], x[8 * j + 1], x[8 * j + 2], x[8 * j + 3], x[8 * j + 4], x[8 * j + 5], x[8 * j + 6], x[8 * j + 7]};
+    xa_store8<T>(row, y, 2 * t + j, h, d, ok);
+  }
+}
+
+// The accumulators of the KW waves that share rows, added with the given weights in wave order.  Every wave leaves its own in LDS and gathers every
+// KW-th sixteen columns of all of them: f(q, values) for its q, columns 16 q + ...  Waves that share nothing (KW = 1) keep theirs.
+template <int DT, int KW> struct XaMeet { static constexpr int SLOT = DT * 16 * 64 * 4, BYTES = KW > 1 ? 4 * SLOT + 4 * 2 * 64 * 4 : 0; };
+template <int DT, int KW, typename F>
+__device__ __forceinline__ void xa_gather(const f32x16 (&acc)[DT], const float (&weight)[KW], uint8_t* lds, int wave, F f) {
+  const int lane = threadIdx.x & 63, kw = wave % KW;
+  if constexpr (KW == 1) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const tv2 lo = {(T)(x[8 * j + 2 * e] * mul), (T)(x[8 * j + 2 * e + 1] * mul)}, hi = {(T)(x[8 * j + 4 + 2 * e] * mul), (T)(x[8 * j + 5 + 2 * e] * mul)};
-      const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, hi), false, false);
-      a[e] = r[0];
-      b[e] = r[1];
+    for (int q = 0; q < 2 * DT; ++q) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = acc[q / 2][8 * (q & 1) + i] * weight[0];
+      f(q, v);
     }
-    const int c = 32 * t + 16 * j + 8 * h;
-    if (ok && c < d) *(i32x4*)(row + c) = i32x4{(int)a[0], (int)a[1], (int)b[0], (int)b[1]};
+  } else {
+    constexpr int SLOT = XaMeet<DT, KW>::SLOT / 4;
+    float* mine = (float*)lds + wave * SLOT + lane;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[(t * 16 + i) * 64] = acc[t][i];
+    __syncthreads();
+    const float* all = (const float*)lds + (wave / KW) * KW * SLOT + lane;
+#pragma unroll
+    for (int u = 0; u < (2 * DT + KW - 1) / KW; ++u) {
+      const int q = kw + u * KW;
+      if (q >= 2 * DT) break;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KW; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] += all[k * SLOT + (q * 8 + i) * 64] * weight[k];
+      f(q, v);
+    }
   }
 }
 
@@ -269,7 +320,8 @@ __device__ __forceinline__ bool xa_narrow(f32x16& x, f32x16 (&acc)[DT], float& e
 // (Forming the next tile's scores beside this one's exponentials in one wave takes half as many registers again: 81 -> 103 us.)
 template <int DT, int KW> struct XaKeys {
   static constexpr int BK = KW == 4 ? 128 : 64, SUB = BK / 32 / KW, NW = BK / 32, IMG = BK * XaImg<DT>::PITCH;
-  static constexpr int NBUF = DT == 1 ? 3 : 2, BYTES = NBUF * 2 * IMG;
+  static constexpr int NBUF = DT == 1 ? 3 : 2, RING = NBUF * 2 * IMG;
+  static constexpr int BYTES = RING > XaMeet<DT, KW>::BYTES ? RING : XaMeet<DT, KW>::BYTES;     // the waves meet where the tiles were
 };
 // The compiler does not know of the transfers: whatever it loaded before the loop has to have arrived before the loop, or it would wait for it
 // inside, and with it for all transfers.
@@ -320,8 +372,8 @@ __device__ __forceinline__ void xa_over_keys(const XaParams& p, uint8_t* lds, in
     else xa_landed<0>();
     if (t + NBUF - 1 < t1) stage(t + NBUF - 1, lds + fill, w[NBUF - 1]);
     if (busy) compute(t, lds + use, lds + use + IMG, w[0]);
-    use = use + 2 * IMG == K::BYTES ? 0 : use + 2 * IMG;
-    fill = fill + 2 * IMG == K::BYTES ? 0 : fill + 2 * IMG;
+    use = use + 2 * IMG == K::RING ? 0 : use + 2 * IMG;
+    fill = fill + 2 * IMG == K::RING ? 0 : fill + 2 * IMG;
 #pragma unroll
     for (int j = 0; j < NBUF; ++j)
 #pragma unroll
@@ -432,62 +484,49 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
         }
   });
   l = xa_halves_sum(l);
-  if constexpr (KW > 1) {       // waves of one row group meet in LDS, added in wave order
+  float weight[KW];              // of the waves that share these rows
+  if constexpr (KW > 1) {
+    __syncthreads();             // nobody reads the tiles any more
+    float* st = (float*)(lds + 4 * XaMeet<DT, KW>::SLOT);
+    st[wave * 128 + lane] = m;
+    st[wave * 128 + 64 + lane] = l;
     __syncthreads();
-    float* x = (float*)lds;
-    constexpr int SLOT = (DT * 16 + 2) * 64;
-    if (kw > 0) {
-      float* y = x + ((wave / KW) * (KW - 1) + kw - 1) * SLOT + lane;
+    const float* all = st + (wave / KW) * KW * 128 + lane;
+    m = XA_M0;
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
+    for (int k = 0; k < KW; ++k) m = fmaxf(m, all[k * 128]);
+    l = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[(t * 16 + i) * 64] = o[t][i];
-      y[DT * 16 * 64] = m;
-      y[(DT * 16 + 1) * 64] = l;
+    for (int k = 0; k < KW; ++k) {
+      weight[k] = __builtin_amdgcn_exp2f(all[k * 128] - m);
+      l += all[k * 128 + 64] * weight[k];
     }
-    __syncthreads();
-    if (kw > 0) return;
-#pragma unroll
-    for (int k = 1; k < KW; ++k) {
-      const float* y = x + ((wave / KW) * (KW - 1) + k - 1) * SLOT + lane;
-      const float m2 = y[DT * 16 * 64], l2 = y[(DT * 16 + 1) * 64], mn = fmaxf(m, m2), a = exp2f(m - mn), a2 = exp2f(m2 - mn);
-      m = mn;
-      l = l * a + l2 * a2;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] = o[t][i] * a + y[(t * 16 + i) * 64] * a2;
-    }
-  }
-  if (r >= p.rows) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float L = l == 0.f ? -INFINITY : m + log2f(l);
-  const long row = (long)bh * p.rows + r;
-  if (p.nsplit > 1) {
-    const long prow = (long)split * p.b * p.hkv * p.rows + row;
-    if (h == 0) p.part_lse[prow] = L;
-    float* po = p.part + prow * p.d;
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int c = 32 * t + 2 * i + 4 * h;
-        if (c < p.d) *(f32x4*)(po + c) = f32x4{o[t][i] * inv, o[t][i + 1] * inv, o[t][i + 2] * inv, o[t][i + 3] * inv};
-      }
   } else {
-    if (p.lse && h == 0) p.lse[row] = l == 0.f ? INFINITY : L;
-    const int s = r / p.grp, g = r % p.grp;
-    const long oo = (((long)b * p.sq + s) * p.hq + hk * p.grp + g) * p.d;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-      xa_store<T>((T*)p.o + oo, o[t], inv, t, h, p.d, true);
-      if (p.o_lo) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[t][i] = o[t][i] * inv - (float)(T)(o[t][i] * inv);
-        xa_store<T>((T*)p.o_lo + oo, o[t], 1.f, t, h, p.d, true);
-      }
-    }
+    weight[0] = 1.f;
   }
+  const bool rok = r < p.rows, none = l == 0.f;
+  const float inv = none ? 0.f : 1.f / l, L = m + log2f(l);
+#pragma unroll
+  for (int k = 0; k < KW; ++k) weight[k] *= inv;
+  const long row = (long)bh * p.rows + r, prow = (long)split * p.b * p.hkv * p.rows + row;
+  if (rok && h == 0 && kw == 0) {
+    if (p.nsplit > 1) p.part_lse[prow] = none ? -INFINITY : L;
+    else if (p.lse) p.lse[row] = none ? INFINITY : L;
+  }
+  const int tok = rok ? r / p.grp : 0, g = rok ? r % p.grp : 0;
+  const long oo = (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
+  xa_gather<DT, KW>(o, weight, lds, wave, [&](int q, float (&v)[8]) {
+    if (p.nsplit > 1) {
+      if (rok && !none) xa_store8(p.part + prow * p.d, v, q, h, p.d);      // a split without keys leaves nothing: nobody reads it
+      return;
+    }
+    xa_store8<T>((T*)p.o + oo, v, q, h, p.d, rok);
+    if (p.o_lo) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] -= (float)(T)v[i];
+      xa_store8<T>((T*)p.o_lo + oo, v, q, h, p.d, rok);
+    }
+  });
 }
 
 // Partial results of the splits, joined by one wave per row: four groups of 16 lanes (8 columns each) take every fourth split, so that the
@@ -517,9 +556,9 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaParams p) {
   if (mx != -INFINITY) {
 #pragma unroll 4
     for (int s = lane >> 4; s < p.nsplit; s += 4) {
-      const float w = exp2f(p.part_lse[s * rows + row] - mx);
+      const float lse = p.part_lse[s * rows + row], w = exp2f(lse - mx);
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (c < p.d) load8(v, p.part + (s * rows + row) * p.d + c, 8);
+      if (c < p.d && lse != -INFINITY) load8(v, p.part + (s * rows + row) * p.d + c, 8);
       sum += w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] += v[j] * w;
@@ -594,49 +633,28 @@ __device__ __forceinline__ float xa_delta(const XaParams& p, const typename Vec8
   return xa_halves_sum(delta);
 }
 
-// the sums of the KW waves that share rows, in wave order; the first of them has the whole
-template <int DT, int KW>
-__device__ __forceinline__ void xa_join_waves(f32x16 (&acc)[DT], uint8_t* lds, int wave) {
-  if constexpr (KW > 1) {
-    const int kw = wave % KW, lane = threadIdx.x & 63;
-    constexpr int SLOT = DT * 16 * 64;
-    float* y = (float*)lds + (wave / KW) * (KW - 1) * SLOT + lane;
+// the gradient of row r of q (acc times `out`, summed over the KW waves that share it), or this split's part of it
+template <typename T, int DT, int KW>
+__device__ __forceinline__ void xa_store_dq(const XaParams& p, const f32x16 (&acc)[DT], float out, uint8_t* lds, int wave, int b, int hk, int split, int r, int h) {
+  const bool rok = r < p.rows;
+  const long prow = ((long)split * p.b * p.hkv + (long)b * p.hkv + hk) * p.rows + r;
+  const int tok = rok ? r / p.grp : 0, g = rok ? r % p.grp : 0;
+  const long oo = (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
+  float weight[KW];
+  if constexpr (KW > 1) {        // fp16: each wave has a factor of its own
     __syncthreads();
-    if (kw > 0) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[(kw - 1) * SLOT + (t * 16 + i) * 64] = acc[t][i];
-    }
+    float* st = (float*)(lds + 4 * XaMeet<DT, KW>::SLOT);
+    st[wave * 64 + (threadIdx.x & 63)] = out;
     __syncthreads();
-    if (kw > 0) return;
 #pragma unroll
-    for (int k = 1; k < KW; ++k)
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[t][i] += y[(k - 1) * SLOT + (t * 16 + i) * 64];
-  }
-}
-
-// the gradient of row r of q, or this split's part of it
-template <typename T, int DT>
-__device__ __forceinline__ void xa_store_dq(const XaParams& p, const f32x16 (&acc)[DT], int b, int hk, int split, int r, int h) {
-  if (p.nsplit > 1) {
-    float* po = p.part + (((long)split * p.b * p.hkv + (long)b * p.hkv + hk) * p.rows + r) * p.d;
-#pragma unroll
-    for (int t = 0; t < DT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int c = 32 * t + 2 * i + 4 * h;
-        if (c < p.d) *(f32x4*)(po + c) = f32x4{acc[t][i], acc[t][i + 1], acc[t][i + 2], acc[t][i + 3]};
-      }
+    for (int k = 0; k < KW; ++k) weight[k] = st[((wave / KW) * KW + k) * 64 + (threadIdx.x & 63)];
   } else {
-    const int tok = r / p.grp, g = r % p.grp;
-    T* to = (T*)p.dq + (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) xa_store<T>(to, acc[t], 1.f, t, h, p.d, true);
+    weight[0] = out;
   }
+  xa_gather<DT, KW>(acc, weight, lds, wave, [&](int q, float (&v)[8]) {
+    if (p.nsplit == 1) xa_store8<T>((T*)p.dq + oo, v, q, h, p.d, rok);
+    else if (rok) xa_store8(p.part + prow * p.d, v, q, h, p.d);
+  });
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq
@@ -721,13 +739,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
           acc[t2] = mfma32(f, ds[u].v[c], acc[t2]);
         }
   });
-  const float out = p.scale * exp2f(-ex);
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[t][i] *= out;
-  xa_join_waves<DT, KW>(acc, lds, wave);
-  if (kw == 0 && rok) xa_store_dq<T, DT>(p, acc, b, hk, split, r, h);
+  xa_store_dq<T, DT, KW>(p, acc, p.scale * exp2f(-ex), lds, wave, b, hk, split, r, h);
 }
 
 // dq of a row = sum over splits
@@ -878,15 +890,15 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaPara
         }
       }
     } else {
-      xa_store<T>((T*)p.dk + oo, dk[t], 1.f, t, h, p.d, true);
-      xa_store<T>((T*)p.dv + oo, dv[t], 1.f, t, h, p.d, true);
+      xa_store<T>((T*)p.dk + oo, dk[t], t, h, p.d, true);
+      xa_store<T>((T*)p.dv + oo, dv[t], t, h, p.d, true);
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ backward, up to 32 rows
 // All rows are one tile, so a tile of keys is done with once read: its dk and dv are complete, and dq is summed on.  One pass over k and v, which
-// are the work (heads of 32, 15 rows x 20480 keys: dq and dk / dv by the kernels above 105 us, here XXX).  Each wave takes 32 keys of a tile both
+// are the work (8 x 8 heads of 32, 15 rows x 20480 keys: dq and dk / dv one after the other 105 us, here 67).  Each wave takes 32 keys of a tile both
 // ways round from the same fragments, operands exchanged: a lane per row for ds^T and dq, a lane per key for p, ds and dk / dv.
 template <int DT> struct XaFew {       // key tiles, then the images of do and q, then L and delta of the rows
   static constexpr int ROWS_IMG = 32 * XaImg<DT>::PITCH, AT = XaKeys<DT, 4>::BYTES, BYTES = AT + 2 * ROWS_IMG + 2 * 32 * 4;
@@ -1013,19 +1025,13 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_bwd_few_kernel(Xa
     if (p.dk) {
 #pragma unroll
       for (int t2 = 0; t2 < DT; ++t2) {
-        xa_store<T>((T*)p.dk + oo, dk[t2], 1.f, t2, h, p.d, in);
-        xa_store<T>((T*)p.dv + oo, dv[t2], 1.f, t2, h, p.d, in);
+        xa_store<T>((T*)p.dk + oo, dk[t2], t2, h, p.d, in);
+        xa_store<T>((T*)p.dv + oo, dv[t2], t2, h, p.d, in);
       }
     }
   });
   if (!p.dq) return;
-  const float out = p.scale * exp2f(-ex);
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) acc[t][i] *= out;
-  xa_join_waves<DT, 4>(acc, lds, wave);
-  if (wave == 0 && rok) xa_store_dq<T, DT>(p, acc, b, hk, split, r, h);
+  xa_store_dq<T, DT, 4>(p, acc, p.scale * exp2f(-ex), lds, wave, b, hk, split, r, h);
 }
 
 // dk and dv = sums over the splits of the rows, in their order; the splits lie 2 * all floats apart, dk and dv in turn
