@@ -37,17 +37,19 @@ def _check(q, k, v, key_lens, key_mask, scale):
         raise NotImplementedError("cross_attention: key_mask of truth values only, True where a key counts (got %s)" % key_mask.dtype)
     if key_mask is not None and key_mask.shape != ks[:2]:
         raise ValueError("cross_attention: key_mask of shape %s expected (got %s)" % (tuple(ks[:2]), tuple(key_mask.shape)))
-    if not 0.0 < scale <= 3e38:
+    if max(qs[0], qs[1], qs[2], ks[1]) > 1 << 30:
+        raise ValueError("cross_attention: sizes beyond 2^30 (got %s and %s)" % (tuple(qs), tuple(ks)))
+    if not 1e-45 < scale <= 2e38:
         raise ValueError("cross_attention: a positive, finite scale expected (got %r)" % (scale,))
 
 
-def _aligned(t):
-    """t with contiguous heads in rows on 16-byte boundaries: itself, or a copy."""
+def _aligned(t, group=0):
+    """t with contiguous heads in rows on 16-byte boundaries: itself, or a copy.  The kernels index 64 tokens, and `group` heads, in 32 bits."""
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
             return t
         st = t.stride()
-        if st[3] == 1 and all(s % 8 == 0 or n == 1 for s, n in zip(st, t.shape[:3])):
+        if st[3] == 1 and st[1] <= 1 << 23 and st[2] * group <= 1 << 28 and all(s % 8 == 0 or n == 1 for s, n in zip(st, t.shape[:3])):
             return t
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
@@ -88,7 +90,7 @@ class CrossAttentionFunction(Function):
         a = _operands(q, k, v, key_lens, key_mask, scale)
         o_lo, lse = like(q), q.new_empty(q.shape[:3].numel(), dtype=torch.float32)
         o = _forward(a, q, o_lo, lse)
-        ctx.operands, ctx.scale = a, scale
+        ctx.operands, ctx.scale, ctx.layout = a, scale, (q.stride(), k.stride(), v.stride())
         ctx.save_for_backward(q, k, v, key_lens, key_mask, o, o_lo, lse)
         return o
 
@@ -101,9 +103,10 @@ class CrossAttentionFunction(Function):
         dk, dv = (like(k), like(v)) if need_k or need_v else (None, None)
         if q.numel() == 0 or k.numel() == 0:
             return tuple(None if t is None else t.zero_() for t in (dq, dk, dv)) + (None, None, None)
-        a, do = ctx.operands, _aligned(do)
-        if a.q != q.data_ptr() or a.k != k.data_ptr() or a.v != v.data_ptr() or a.key_lens != p(key_lens) or a.key_mask != p(key_mask):
-            q, k, v = _aligned(q), _aligned(k), _aligned(v)          # saved tensors were kept elsewhere meanwhile
+        a, do = ctx.operands, _aligned(do, q.shape[2] // k.shape[2])
+        if a.q != q.data_ptr() or a.k != k.data_ptr() or a.v != v.data_ptr() or a.key_lens != p(key_lens) or a.key_mask != p(key_mask) or ctx.layout != (
+                q.stride(), k.stride(), v.stride()):
+            q, k, v = _aligned(q, q.shape[2] // k.shape[2]), _aligned(k), _aligned(v)          # saved tensors were kept elsewhere meanwhile
             a = _operands(q, k, v, key_lens, key_mask, ctx.scale)
         ws, n = _workspace(a, 1, q)
         call("rtp_xattn_backward", q, C.byref(a), p(o), p(o_lo), p(lse), p(do), *_strides(do), p(dq), p(dk), p(dv), p(ws), n)
@@ -114,7 +117,7 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     """scale: 1 / sqrt(d) by default.  key_lens: [b] int32 or int64 (taken between 0 and sk); key_mask: [b, sk], True where a key counts."""
     scale = q.shape[-1] ** -0.5 if scale is None and q.dim() == 4 and q.shape[-1] else 1.0 if scale is None else float(scale)
     _check(q, k, v, key_lens, key_mask, scale)
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    q, k, v = _aligned(q, q.shape[2] // k.shape[2]), _aligned(k), _aligned(v)
     if key_lens is not None:
         key_lens = (key_lens if key_lens.dtype == torch.int32 else key_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -1083,10 +1083,11 @@ static int xa_check(const RtpXattn* a) {
   const long grp = a->hq / a->hkv, rows = a->sq * grp;
   if (rows * grp >= (1L << 31) || a->sk > (1 << 30)) return RTP_ERR_SHAPE;
   const XaPlan pl = xa_plan(a);
-  const long units = (long)a->b * a->hkv * (pl.nsplit > pl.ksplit ? pl.nsplit : pl.ksplit);
-  const long tiles = pl.tiles > pl.ktiles ? pl.tiles : pl.ktiles;
-  if ((units + 8) * tiles >= (1L << 31) || (long)a->b * xa_words(a->sk) >= (1L << 31) || (long)a->b * a->hkv * rows >= (1L << 34)) return RTP_ERR_SHAPE;
-  if (!(a->scale > 0.f) || a->scale > 3e38f) return RTP_ERR_SHAPE;
+  const long bh = (long)a->b * a->hkv;
+  if (bh >= (1L << 28) || !rtp_launchable((bh * pl.nsplit + 8) * pl.tiles, 256) || !rtp_launchable((bh * pl.ksplit + 8) * pl.ktiles, 256) ||
+      !rtp_launchable(bh * rows, 16) || !rtp_launchable((long)a->b * xa_words(a->sk), 32))
+    return RTP_ERR_SHAPE;
+  if (!(a->scale > 0.f) || a->scale > 2e38f) return RTP_ERR_SHAPE;       // times log2(e) still finite
   return RTP_OK;
 }
 static bool xa_aligned(const void* p, long bs, long ss, long hs) { return !((size_t)p & 15) && !(bs & 7) && !(ss & 7) && !(hs & 7); }

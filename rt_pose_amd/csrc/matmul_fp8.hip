@@ -372,6 +372,7 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     p.tiles_n = rtp_div_up(p.n, 16 * nt);
     p.tiles_m = (int)rows;
     auto few = [&](auto kernel) {
+      if (!rtp_launchable(rows * p.tiles_n, 64 * MM8_FEW_WAVES)) return RTP_ERR_SHAPE;
       hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * p.tiles_n)), dim3(64 * MM8_FEW_WAVES), 0, st, p);
       RTP_CHECK_LAUNCH();
       return RTP_OK;
@@ -382,11 +383,12 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
   }
   const long tiles256 = (long)rtp_div_up(p.m, 256) * rtp_div_up(p.n, 256);
   auto go = [&](auto kernel, int bm, int bn, int threads, bool* once) {
+    p.tiles_m = rtp_div_up(p.m, bm);
+    p.tiles_n = rtp_div_up(p.n, bn);
+    if (!rtp_launchable((long)p.tiles_m * p.tiles_n, threads)) return RTP_ERR_SHAPE;
     const int bytes = 2 * ((bm + bn) * 128 + (bm + (SQUARE ? 64 : bn)) * 4);
     if (rtp_once_per_device(once) && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
       return RTP_ERR_LAUNCH;
-    p.tiles_m = rtp_div_up(p.m, bm);
-    p.tiles_n = rtp_div_up(p.n, bn);
     hipLaunchKernelGGL(kernel, dim3((unsigned)((long)p.tiles_m * p.tiles_n)), dim3(threads), bytes, st, p);
     RTP_CHECK_LAUNCH();
     return RTP_OK;
@@ -404,13 +406,12 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
 
 extern "C" int rtp_matmul_fp8(const void* a, long lda, const float* sa, const void* b, long ldb, const float* sb, int b_square, void* out, int m,
                               int n, int k, int out_dtype, void* stream) {
-  if (m < 0 || n < 0 || k < 1) return RTP_ERR_SHAPE;
+  if (m < 0 || n < 0 || k < 1 || m > (1 << 30) || n > (1 << 30)) return RTP_ERR_SHAPE;
   if (m == 0 || n == 0) return RTP_OK;
   if (!a || !sa || !b || !sb || !out) return RTP_ERR_SHAPE;
   const long need = ((long)k + 15) & ~15L;
   if ((m > 1 && lda < need) || (n > 1 && ldb < need) || lda > (1L << 22) || ldb > (1L << 22)) return RTP_ERR_SHAPE;   // tiles index 32 bits
   if (((size_t)a & 15) || ((size_t)b & 15) || (lda & 15) || (ldb & 15)) return RTP_ERR_ALIGN;
-  if ((long)rtp_div_up(m, 16) * rtp_div_up(n, 16) >= (1L << 31)) return RTP_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
   RtpProfScope prof(RTP_FAM_CONV, st);
   Mm8Params p{(const uint8_t*)a, (const uint8_t*)b, sa, sb, out, lda, ldb, n, m, n, k, (k + 127) >> 7, 0, 0};

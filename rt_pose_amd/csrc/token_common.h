@@ -8,6 +8,9 @@ typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 #define RTP_FP8_MAX 448.0f
+// a launch counts its threads in 32 bits
+static inline bool rtp_launchable(long blocks, long threads) { return blocks * threads < (1L << 32); }
+
 #define RTP_FP8_AMAX_FLOOR 0x1p-100f   // keeps 448 / amax finite; a block of zeros gets the floor's scale
 
 // Eight consecutive values at any address (rows of odd length or odd stride start anywhere): one unaligned 16- or 32-byte access,

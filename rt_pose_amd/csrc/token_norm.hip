@@ -233,6 +233,7 @@ static int norm_forward(const NormParams& p, int dtype, int w_dtype, hipStream_t
   return norm_types(dtype, w_dtype, [&](auto t, auto w) {
     return norm_shape(p.h, [&](auto lpr, auto nv) {
       constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, THREADS = LPR > 256 ? LPR : 256;
+      if (!rtp_launchable(rtp_div_up(p.rows, THREADS / LPR), THREADS)) return RTP_ERR_SHAPE;
       hipLaunchKernelGGL((rmsnorm_fwd_kernel<decltype(t), decltype(w), LPR, NV, OUT8>), dim3(rtp_div_up(p.rows, THREADS / LPR)), dim3(THREADS), 0,
                          st, p);
       RTP_CHECK_LAUNCH();
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(256) void quant_turned_kernel(QuantParams p) {
 
 extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, float* scale, long rows, int cols, int square, int dtype,
                                 void* stream) {
-  if (rows < 0 || cols < 1 || q_rs < ((cols + 15) & ~15)) return RTP_ERR_SHAPE;
+  if (rows < 0 || rows >= (1L << 31) || cols < 1 || cols > (1 << 30) || q_rs < ((cols + 15) & ~15)) return RTP_ERR_SHAPE;
   if (rows == 0) return RTP_OK;
   if (!x || !q || !scale) return RTP_ERR_SHAPE;
   if (((size_t)q & 15) || (q_rs & 15)) return RTP_ERR_ALIGN;
@@ -443,7 +444,7 @@ extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, l
   const int kb = (cols + 127) >> 7;
   QuantParams p{x, (uint8_t*)q, scale, x_rs, q_rs, rows, cols, kb};
   const long tiles = ((rows + 127) >> 7) * kb, turned_tiles = ((rows + 127) >> 7) * ((kb + 7) & ~7), groups = ((rows + QUANT_ROWS - 1) / QUANT_ROWS) * kb;
-  if (turned_tiles >= (1L << 31) || groups >= (1L << 31)) return RTP_ERR_SHAPE;
+  if (!rtp_launchable(turned ? turned_tiles : square ? tiles : (groups + 15) / 16, 256)) return RTP_ERR_SHAPE;
   auto go = [&](auto t) {
     typedef decltype(t) T;
     if (turned && square)

@@ -26,6 +26,8 @@ def quantize_fp8(x, block=(1, 128)):
     square = tuple(block) == (128, 128)
     if x.dim() < 1 or x.shape[-1] < 1 or (square and x.dim() != 2):
         raise ValueError("quantize_fp8: [..., cols] expected, [rows, cols] for blocks of 128 x 128 (got %s)" % (tuple(x.shape),))
+    if x.shape[-1] > 1 << 30:
+        raise ValueError("quantize_fp8: rows of up to 2^30 columns (got %d)" % x.shape[-1])
     turned = x.dim() == 2 and x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1
     x2 = x if turned else rows_of(x)
     rows, cols = x2.shape
@@ -36,15 +38,15 @@ def quantize_fp8(x, block=(1, 128)):
 
 
 def _operand(q, what):
-    """q as [rows, cols] whose rows are 16-byte aligned and readable up to a multiple of 16 bytes: itself where it is so (what quantize_fp8 and
-    add_rms_norm_fp8 return), a copy otherwise."""
+    """q as [rows, cols] whose rows are 16-byte aligned, readable up to a multiple of 16 bytes and at most 4 MiB apart: itself where it is so (what
+    quantize_fp8 and add_rms_norm_fp8 return), a copy otherwise."""
     if q.dtype != FP8:
         raise NotImplementedError("matmul_fp8: %s must be float8_e4m3fn (got %s)" % (what, q.dtype))
     (rows, cols), (ld, step) = q.shape, q.stride()
     wide = -(-cols // 16) * 16
     if rows == 1:
-        ld = max(ld - ld % 16, wide)
-    if (step == 1 or cols == 1) and ld % 16 == 0 and ld >= wide and q.data_ptr() % 16 == 0 and (
+        ld = wide
+    if (step == 1 or cols == 1) and ld % 16 == 0 and wide <= ld <= 1 << 22 and q.data_ptr() % 16 == 0 and (
             wide == cols or q.storage_offset() + (rows - 1) * ld + wide <= q.untyped_storage().nbytes()):
         return q, ld
     own = torch.empty(rows, wide, dtype=torch.uint8, device=q.device)
@@ -66,6 +68,8 @@ def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16):
         raise ValueError("matmul_fp8: [..., m, k] and [n, k] expected (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
     k, n = b.shape[1], b.shape[0]
     kb, nb = -(-k // 128), -(-n // 128)
+    if k > 1 << 22 or max(n, lead.numel()) > 1 << 30:
+        raise ValueError("matmul_fp8: up to 2^22 columns and 2^30 rows (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
     if a_scale.shape != (*lead, kb):
         raise ValueError("matmul_fp8: a_scale of shape %s expected (got %s)" % ((*lead, kb), tuple(a_scale.shape)))
     if b_scale.shape not in ((nb, kb), (n, kb)):

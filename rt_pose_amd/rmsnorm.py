@@ -25,6 +25,8 @@ def _check(x, residual, weight):
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("rms norm: rows of at least one column expected (got shape %s)" % (tuple(shape),))
+    if shape[-1] > 16384:
+        raise NotImplementedError("rms norm: rows of up to 16384 columns (got %d)" % shape[-1])
     if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise ValueError("rms norm: the residual must have x's shape and type (got %s %s beside %s %s)"
                          % (tuple(residual.shape), residual.dtype, tuple(x.shape), x.dtype))

@@ -317,3 +317,72 @@ def test_captured_and_replayed():
         want = [t.detach().clone() for t in step()]
         for _, out in graphs:
             assert all(torch.equal(a, c) for a, c in zip(out, want))
+
+
+def test_strides_beyond_what_the_kernels_index_and_sizes_beyond_all():
+    from rt_pose_amd.attention import cross_attention
+    q, k, v, do, _, _ = case(1, 3, 3, 2, 1, 8, torch.bfloat16, seed=40)
+    o = cross_attention(q, k, v)
+    want = (o, *torch.autograd.grad(o, (q, k, v), do))
+
+    def far(t, ss):                                                       # tokens `ss` elements apart
+        big = torch.zeros(2 * ss + t[0, 0].numel(), dtype=t.dtype, device="cuda")
+        view = big.as_strided(t.shape, (0, ss, 8, 1))
+        view.copy_(t.detach())
+        return view
+    for ss in (2 ** 23, 2 ** 23 + 8):
+        q2, k2, v2 = (far(t, ss).requires_grad_(True) for t in (q, k, v))
+        o2 = cross_attention(q2, k2, v2)
+        got = (o2, *torch.autograd.grad(o2, (q2, k2, v2), far(do, ss)))
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+    line = torch.zeros(8, dtype=torch.bfloat16, device="cuda")
+    for sq, sk, hq in ((2 ** 32 + 1, 1, 1), (1, 2 ** 32 + 1, 1), (1, 1, 2 ** 32 + 1)):
+        with pytest.raises(ValueError):
+            cross_attention(line.expand(1, sq, hq, 8), line.expand(1, sk, 1, 8), line.expand(1, sk, 1, 8))
+
+
+def test_saved_operands_that_come_back_elsewhere_or_in_another_layout():
+    from rt_pose_amd.attention import cross_attention
+    q, k, v, do, lens, mask = case(2, 20, 150, 4, 2, 32, torch.float16, [150, 70], 0.8, seed=50)
+    L = lens.cuda()
+    want = torch.autograd.grad(cross_attention(q, k, v, L, mask), (q, k, v), do)
+    with torch.autograd.graph.save_on_cpu():
+        o = cross_attention(q, k, v, L, mask)
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(o, (q, k, v), do), want))
+    # back at the same address, but packed: the place of q is the front of a wider tensor's
+    wide = torch.zeros(2, 20, 8, 32, dtype=q.dtype, device="cuda")
+    q2 = wide[:, :, ::2]
+    q2.copy_(q.detach())
+    q2 = q2.detach().requires_grad_(True)
+
+    def back(t):
+        if t[0] != wide.data_ptr():
+            return t[1]
+        packed = wide.view(-1)[:t[1].numel()].view(t[1].shape)
+        packed.copy_(t[1])
+        return packed
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (t.data_ptr(), t.detach().clone(memory_format=torch.contiguous_format)), back):
+        o = cross_attention(q2, k, v, L, mask)
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(o, (q2, k, v), do), want))
+
+
+def test_two_calls_at_once():
+    from rt_pose_amd.attention import cross_attention
+    cases = [case(2, 1, 3000, 8, 2, 64, torch.bfloat16, [3000, 1700], 0.9, seed=60), case(2, 200, 700, 4, 4, 64, torch.bfloat16, [700, 9], 0.9, seed=70)]
+
+    def step(c):
+        q, k, v, do, lens, mask = c
+        o = cross_attention(q, k, v, lens.to("cuda", non_blocking=True), mask)
+        return (o, *torch.autograd.grad(o, (q, k, v), do))
+    want = [step(c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(3):
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(step(c))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))

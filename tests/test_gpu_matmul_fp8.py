@@ -140,3 +140,23 @@ def test_the_three_products_of_a_layer():
         eb = torch.maximum(Q.abs() * 2.0 ** -4, wide * 2.0 ** -10)
         bound = (ea @ Q.abs().t() + P.abs() @ eb.t() + ea @ eb.t()) * 1.0001
         assert bool(((out.double() - P @ Q.t()).abs() <= bound).all())
+
+
+def test_far_rows_and_sizes_beyond():
+    from rt_pose_amd.fp8 import matmul_fp8
+    (a, sa), (b, sb) = operand(3, 48, False, 90), operand(5, 48, True, 91)
+    want = matmul_fp8(a, sa, b, sb)
+    for ld in (2 ** 22, 2 ** 22 + 16):                                     # rows further apart than a tile indexes: copied
+        far = torch.zeros(4 * ld + 48, dtype=torch.uint8, device="cuda")
+        a2, b2 = (far.as_strided((n, 48), (ld, 1)) for n in (3, 5))
+        a2.copy_(a.view(torch.uint8))
+        assert torch.equal(matmul_fp8(a2.view(a.dtype), sa, b, sb), want)
+        assert torch.equal(matmul_fp8(a2[1:2].view(a.dtype), sa[1:2], b, sb), want[1:2])
+        b2.copy_(b.view(torch.uint8))
+        assert torch.equal(matmul_fp8(a, sa, b2.view(b.dtype), sb), want)
+    byte = torch.zeros(1, dtype=torch.uint8, device="cuda").view(a.dtype)
+    one = torch.ones(1, device="cuda")
+    for m, n, k in ((2 ** 32 + 1, 1, 16), (1, 2 ** 32 + 1, 16), (1, 1, 2 ** 32 + 16), (1, 1, 2 ** 22 + 1)):
+        kb = -(-k // 128)
+        with pytest.raises(ValueError):
+            matmul_fp8(byte.expand(m, k), one.expand(m, kb), byte.expand(n, k), one.expand(n, kb))

@@ -246,3 +246,36 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         got = [o.detach().float().clone() for o in out]
         assert all(torch.equal(a, b.detach().float()) for a, b in zip(got, step()))
+
+
+def test_the_same_rows_twice_broadcast_rows_and_widths_beyond():
+    from rt_pose_amd.fp8 import quantize_fp8
+    from rt_pose_amd.rmsnorm import RMSNorm, add_rms_norm, add_rms_norm_fp8, rms_norm
+    x, w, dy, ds = (rnd(6, 200, seed=80 + i, dtype=torch.float32) for i in range(4))
+    x.requires_grad_(True)
+    r = x.detach().clone().requires_grad_(True)
+    y, s = add_rms_norm(x, x, w[0])                                        # the residual is x itself: both gradients add
+    (g,) = torch.autograd.grad((y, s), x, (dy, ds))
+    y2, s2 = add_rms_norm(x, r, w[0])
+    gx, gr = torch.autograd.grad((y2, s2), (x, r), (dy, ds))
+    assert torch.equal(y, y2) and torch.equal(s, s2) and torch.equal(gx, gr) and torch.equal(g, gx + gr)
+    x.grad = r.grad = None
+    torch.autograd.backward(add_rms_norm(x, r, w[0]), (dy, ds))            # one tensor is the gradient of both: each leaf keeps its own
+    x.grad.zero_()
+    assert torch.equal(r.grad, gr)
+    row = rnd(200, seed=90, dtype=torch.bfloat16)
+    many = row.expand(5, 3, 200)
+    assert torch.equal(rms_norm(many, row), rms_norm(many.contiguous(), row))
+    for a, b in zip(quantize_fp8(row.expand(300, 200), (128, 128)), quantize_fp8(row.repeat(300, 1), (128, 128))):
+        assert torch.equal(a.float(), b.float())
+    columns = row[:, None].expand(200, 300)                                # a transpose's view whose columns are all the same memory
+    for block in ((1, 128), (128, 128)):
+        for a, b in zip(quantize_fp8(columns, block), quantize_fp8(columns.contiguous(), block)):
+            assert torch.equal(a.float(), b.float())
+    wide = torch.zeros(1, 16385, device="cuda")
+    for call in (lambda: rms_norm(wide, wide[0]), lambda: add_rms_norm_fp8(wide, None, wide[0]), lambda: RMSNorm(16385).cuda()(wide, wide)):
+        with pytest.raises(NotImplementedError):
+            call()
+    for n in (2 ** 30 + 1, 2 ** 32 + 8):
+        with pytest.raises(ValueError):
+            quantize_fp8(wide[:, :1].expand(1, n))

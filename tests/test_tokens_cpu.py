@@ -107,3 +107,20 @@ def test_workspace_is_sized_for_every_cut():
                     for back in (0, 1):
                         n = lib.rtp_xattn_workspace_bytes(C.byref(attn(b=b, sq=sq, sk=sk, hq=hq, hkv=hkv)), back)
                         assert 0 <= n < 2 ** 33
+
+
+def test_sizes_that_no_launch_can_count_are_refused():
+    """A launch counts its threads in 32 bits; what would pass that is refused before anything is read."""
+    lib = _lib.load()
+    a = P(4096)
+    for rows, h in ((2 ** 28, 8), (2 ** 26, 200), (2 ** 24, 4096), (2 ** 31, 8)):
+        assert lib.rtp_rmsnorm_forward(a, h, None, 0, a, 0, a, None, rows, h, 0, 1e-6, None) == SHAPE
+        assert lib.rtp_rmsnorm_fp8_forward(a, h, None, 0, a, 0, a, 4096, a, None, rows, h, 0, 1e-6, None) == SHAPE
+    for rows, cols, square, turned in ((2 ** 30, 8, 0, 0), (2 ** 31, 8, 1, 0), (2 ** 28, 8, 0, 1), (2 ** 28, 8, 1, 1), (1, 2 ** 30 + 1, 0, 0)):
+        assert lib.rtp_quantize_fp8(a, cols, turned, a, 2 ** 31, a, rows, cols, square, 0, None) == SHAPE
+    for m, n in ((2 ** 30 + 1, 1), (1, 2 ** 30 + 1), (1, 2 ** 29), (2 ** 20, 2 ** 20)):
+        assert lib.rtp_matmul_fp8(a, 16, a, a, 16, a, 1, a, m, n, 16, 2, None) == SHAPE
+    assert lib.rtp_matmul_fp8(a, 2 ** 22 + 16, a, a, 16, a, 1, a, 2, 2, 16, 2, None) == SHAPE
+    size = lambda back=0, **k: lib.rtp_xattn_workspace_bytes(C.byref(attn(**k)), back)
+    for bad in (dict(b=2 ** 24, hkv=1, hq=1), dict(b=2 ** 20, sk=2 ** 16), dict(b=2 ** 10, sq=2 ** 18, hq=2, hkv=2), dict(scale=2.5e38), dict(b=2 ** 30, hkv=64, hq=64)):
+        assert size(**bad) == -1 and size(1, **bad) == -1
