@@ -55,22 +55,33 @@ struct XaParams {
   unsigned grp_magic;        // ceil(2^32 / grp): r / grp = mulhi(r, magic) for r * grp < 2^32
   int words;
   int tiles, units, nsplit;  // workgroups = tiles x units (batch x kv head x split)
+  int near;                  // kv heads whose rows share a 128-byte line
+  int pairs;                 // forward: pairs of a batch entry and a run of its tiles of keys, or 0: units are batch x kv head
+  bool ragged;               // pairs follow the entries' lengths
   float scale, scale_log2;
   void *o, *o_lo, *dq, *dk, *dv;
   float *lse, *delta, *part, *part_lse;
   const float* lse_in;
 };
 
+// workgroup -> tile of rows, group of `near` units, which of them.  Heads whose rows share a line follow each other on one XCD: with one of them on
+// each XCD every line goes to several L2s (15 rows x 20480 keys, 8 x 8 heads of 32: forward 55.7 us, so 40.4; backward 95.8, so 79.5).
+__device__ __forceinline__ bool xa_group(const XaParams& p, int& tile, unsigned& group, unsigned& member) {
+  const unsigned j = blockIdx.x >> 3, y = j / (unsigned)p.tiles;
+  tile = j % (unsigned)p.tiles;
+  group = y / (unsigned)p.near * 8 + (blockIdx.x & 7);
+  member = y % (unsigned)p.near;
+  return group * p.near < (unsigned)p.units;
+}
 // Workgroup -> (tile, unit): all tiles of a unit run on one XCD (workgroups go round the 8 XCDs), so that a unit's k and v stay in one L2.
 // Batch entries with more keys come first (up to 64 entries: each lane ranks one): the last workgroups to start are then the short ones.
 __device__ __forceinline__ bool xa_place(const XaParams& p, int& tile, int& b, int& hk, int& split) {
-  const unsigned j = blockIdx.x >> 3, unit = (j / (unsigned)p.tiles) * 8 + (blockIdx.x & 7);
-  tile = j % (unsigned)p.tiles;
-  if (unit >= (unsigned)p.units) return false;
-  const int bh = unit / (unsigned)p.nsplit;
-  split = unit % (unsigned)p.nsplit;
-  b = bh / p.hkv;
-  hk = bh % p.hkv;
+  unsigned group, member;
+  if (!xa_group(p, tile, group, member)) return false;
+  const unsigned some = p.hkv / p.near, bg = group / (unsigned)p.nsplit;
+  split = group % (unsigned)p.nsplit;
+  b = bg / some;
+  hk = (bg % some) * p.near + member;
   if (p.lens && p.b > 1 && p.b <= 64) {
     const int lane = threadIdx.x & 63, mine = lane < p.b ? p.lens[lane] : 0;
     int rank = 0;
@@ -83,10 +94,70 @@ __device__ __forceinline__ bool xa_place(const XaParams& p, int& tile, int& b, i
   return true;
 }
 
+// The forward pass in runs of tiles of keys, `pairs` of them at most.  Where entries have lengths (p.ragged, 2 to 64 entries, a lane each) one
+// length of run does for all: the shortest (long ones: up to a sixteenth) that leaves no more runs than pairs, so that every workgroup has the same
+// to do, whatever the lengths are (one row, 8 entries of 0 to 5120 keys x 8 heads of 128: 20.1 us; every entry in as many runs 26.6).  Entry i has runs
+// first .. first + n - 1.  A run has two tiles at least: 8 x 8 heads, 256 keys, in two runs of one tile 7.4 us and 3.7 for the join, uncut 8.9.
+struct XaShares { int tiles, run, first, n; };      // tiles, first and n: of the lane's entry
+#define XA_RUN 2
+__device__ __forceinline__ XaShares xa_shares(const XaParams& p, int bk) {
+  const int lane = threadIdx.x & 63;
+  XaShares s;
+  const int len = lane < p.b ? p.lens[lane] : 0;
+  s.tiles = ((len < 0 ? 0 : len > p.sk ? p.sk : len) + bk - 1) / bk;
+  auto sum = [&](int v) {
+    for (int o = 1; o < p.b; o <<= 1) v += __shfl_xor(v, o, 64);
+    return __builtin_amdgcn_readfirstlane(v);
+  };
+  const unsigned even = ((unsigned)sum(s.tiles) + p.pairs - 1) / (unsigned)p.pairs;
+  s.run = even > XA_RUN ? even : XA_RUN;
+  while (true) {                 // ends: one run for each entry is fewer than pairs
+    s.n = (unsigned)(s.tiles + s.run - 1) / (unsigned)s.run;
+    if (sum(s.n) <= p.pairs) break;
+    s.run += 1 + s.run / 16;
+  }
+  s.first = s.n;
+  for (int o = 1; o < p.b; o <<= 1) {
+    const int v = __shfl_up(s.first, o, 64);
+    s.first += lane >= o ? v : 0;
+  }
+  s.first -= s.n;
+  return s;
+}
+
 __device__ __forceinline__ int xa_len(const XaParams& p, int b) {
   if (!p.lens) return p.sk;
   const int n = (int)((const cst_u32_xa*)p.lens)[b];
   return n < 0 ? 0 : n > p.sk ? p.sk : n;
+}
+// this workgroup's tile of rows, batch entry, kv head, pair and run of tiles of keys
+__device__ __forceinline__ bool xa_place_run(const XaParams& p, int bk, int& tile, int& b, int& hk, int& pair, int& t0, int& t1) {
+  if (p.pairs == 0) {
+    if (!xa_place(p, tile, b, hk, pair)) return false;
+    t0 = 0;
+    t1 = (xa_len(p, b) + bk - 1) / bk;
+    return true;
+  }
+  unsigned group, member;
+  if (!xa_group(p, tile, group, member)) return false;
+  const unsigned some = p.hkv / p.near;
+  pair = group / some;
+  hk = (group % some) * p.near + member;
+  if (!p.ragged) {
+    b = pair / p.nsplit;
+    const int split = pair % p.nsplit, nt = (xa_len(p, b) + bk - 1) / bk;
+    t0 = (int)((long)nt * split / p.nsplit);
+    t1 = (int)((long)nt * (split + 1) / p.nsplit);
+    return true;
+  }
+  const XaShares s = xa_shares(p, bk);
+  const unsigned long mine = __ballot(pair >= s.first && pair < s.first + s.n);
+  if (mine == 0) return false;
+  b = __builtin_ctzll(mine);
+  t0 = (pair - __builtin_amdgcn_readlane(s.first, b)) * s.run;
+  t1 = __builtin_amdgcn_readlane(s.tiles, b);
+  if (t0 + s.run < t1) t1 = t0 + s.run;
+  return true;
 }
 // bits of the 32 keys from key0 on
 __device__ __forceinline__ unsigned xa_word(const XaParams& p, int b, int len, int key0) {
@@ -330,14 +401,13 @@ __device__ __forceinline__ void xa_settle() { __builtin_amdgcn_s_waitcnt(0x0F70)
 template <int N>
 __device__ __forceinline__ void xa_landed() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory"); }
 
-// ALL: tiles without a key that counts too (gradients are written for every key).
-template <typename T, int DT, int KW, bool ALL, typename F>
-__device__ __forceinline__ void xa_over_keys(const XaParams& p, uint8_t* lds, int b, int hk, int split, bool busy, F compute) {
+// f(tile, images of k and v, words) for the tiles t0 .. t1 - 1
+template <typename T, int DT, int KW, typename F>
+__device__ __forceinline__ void xa_over_keys(const XaParams& p, uint8_t* lds, int b, int hk, int t0, int t1, bool busy, F compute) {
   typedef XaKeys<DT, KW> K;
   constexpr int BK = K::BK, NW = K::NW, NBUF = K::NBUF, IMG = K::IMG, PER = 2 * BK / XaLoader<DT, T>::ROWS;
-  const int len = xa_len(p, b), nt = ((ALL ? p.sk : len) + BK - 1) / BK;
-  const int t0 = (int)((long)nt * split / p.nsplit), t1 = (int)((long)nt * (split + 1) / p.nsplit);
   if (t0 >= t1) return;
+  const int len = xa_len(p, b);
   const T* kp = (const T*)p.k + (long)b * p.k_bs + (long)hk * p.k_hs;
   const T* vp = (const T*)p.v + (long)b * p.v_bs + (long)hk * p.v_hs;
   const XaLoader<DT, T> ld(p.d);
@@ -407,8 +477,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
   typedef typename Vec8<T>::type V;
   constexpr int SUB = XaKeys<DT, KW>::SUB, NW = XaKeys<DT, KW>::NW, PITCH = XaImg<DT>::PITCH;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  int tile, b, hk, split;
-  if (!xa_place(p, tile, b, hk, split)) return;
+  int tile, b, hk, pair, t0, t1;
+  if (!xa_place_run(p, XaKeys<DT, KW>::BK, tile, b, hk, pair, t0, t1)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bh = b * p.hkv + hk, h = lane >> 5;
   const int kw = wave % KW, r0 = tile * (128 / KW) + (wave / KW) * 32, r = r0 + (lane & 31);
@@ -423,7 +493,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
     for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
   float m = XA_M0, l = 0.f;
 
-  xa_over_keys<T, DT, KW, false>(p, lds, b, hk, split, r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  xa_over_keys<T, DT, KW>(p, lds, b, hk, t0, t1, r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[SUB], any = 0, all = ~0u;
     xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
@@ -508,16 +578,16 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
   const float inv = none ? 0.f : 1.f / l, L = m + log2f(l);
 #pragma unroll
   for (int k = 0; k < KW; ++k) weight[k] *= inv;
-  const long row = (long)bh * p.rows + r, prow = (long)split * p.b * p.hkv * p.rows + row;
+  const long row = (long)bh * p.rows + r, prow = ((long)pair * p.hkv + hk) * p.rows + r;
   if (rok && h == 0 && kw == 0) {
-    if (p.nsplit > 1) p.part_lse[prow] = none ? -INFINITY : L;
+    if (p.pairs) p.part_lse[prow] = none ? -INFINITY : L;
     else if (p.lse) p.lse[row] = none ? INFINITY : L;
   }
   const int tok = rok ? r / p.grp : 0, g = rok ? r % p.grp : 0;
   const long oo = (((long)b * p.sq + tok) * p.hq + hk * p.grp + g) * p.d;
   xa_gather<DT, KW>(o, weight, lds, wave, [&](int q, float (&v)[8]) {
-    if (p.nsplit > 1) {
-      if (rok && !none) xa_store8(p.part + prow * p.d, v, q, h, p.d);      // a split without keys leaves nothing: nobody reads it
+    if (p.pairs) {
+      if (rok && !none) xa_store8(p.part + prow * p.d, v, q, h, p.d);      // a run without keys leaves nothing: nobody reads it
       return;
     }
     xa_store8<T>((T*)p.o + oo, v, q, h, p.d, rok);
@@ -529,22 +599,34 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
   });
 }
 
-// Partial results of the splits, joined by one wave per row: four groups of 16 lanes (8 columns each) take every fourth split, so that the
-// loads of a row are under way together, and the groups are added in a fixed order.
+// Partial results, joined by one wave per row: groups of L lanes (8 columns each) take turns, so that the loads of a row are under way together, and
+// the groups are added in a fixed order.
+template <int DT> struct XaJoin { static constexpr int L = DT == 1 ? 4 : DT == 2 ? 8 : 16; };
+template <int L>
 __device__ __forceinline__ float xa_groups_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+#pragma unroll
+  for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
 }
 
-// o of a row = sum over splits of 2^(L_split - L) o_split
-template <typename T>
-__global__ __launch_bounds__(256) void xattn_join_kernel(XaParams p) {
+// o of a row = sum over runs of 2^(L_run - L) o_run.  bk: keys of a tile
+template <typename T, int DT>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XaParams p, int bk) {
   const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, c = (lane & 15) * 8;
+  constexpr int L = XaJoin<DT>::L;
+  const int lane = threadIdx.x & 63, c = lane % L * 8;
   if (row >= rows) return;
+  const int bh = (int)(row / p.rows), b = bh / p.hkv, hk = bh % p.hkv, r = (int)(row % p.rows);
+  int first = b * p.nsplit, n = p.nsplit;
+  if (p.ragged) {
+    const XaShares s = xa_shares(p, bk);
+    first = __builtin_amdgcn_readlane(s.first, __builtin_amdgcn_readfirstlane(b));
+    n = __builtin_amdgcn_readlane(s.n, __builtin_amdgcn_readfirstlane(b));
+  }
+  const long at = ((long)first * p.hkv + hk) * p.rows + r, step = (long)p.hkv * p.rows;     // this row of the runs
   float mx = -INFINITY;
-  for (int s = lane; s < p.nsplit; s += 64) {
-    const float x = p.part_lse[s * rows + row];
+  for (int s = lane; s < n; s += 64) {
+    const float x = p.part_lse[at + s * step];
     mx = x > mx || x != x ? x : mx;      // a NaN stays
   }
 #pragma unroll
@@ -555,23 +637,23 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaParams p) {
   float sum = 0.f, acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (mx != -INFINITY) {
 #pragma unroll 4
-    for (int s = lane >> 4; s < p.nsplit; s += 4) {
-      const float lse = p.part_lse[s * rows + row], w = exp2f(lse - mx);
+    for (int s = lane / L; s < n; s += 64 / L) {
+      const float lse = p.part_lse[at + s * step], w = exp2f(lse - mx);
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (c < p.d && lse != -INFINITY) load8(v, p.part + (s * rows + row) * p.d + c, 8);
+      if (c < p.d) load8(v, p.part + (at + s * step) * p.d + c, 8);
       sum += w;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] += v[j] * w;
+      for (int j = 0; j < 8; ++j) acc[j] += lse == -INFINITY ? 0.f : v[j] * w;      // a run without keys has left nothing
     }
-    sum = xa_groups_sum(sum);
+    sum = xa_groups_sum<L>(sum);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = xa_groups_sum(acc[j]);
+    for (int j = 0; j < 8; ++j) acc[j] = xa_groups_sum<L>(acc[j]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   if (p.lse && lane == 0) p.lse[row] = sum == 0.f ? INFINITY : mx + log2f(sum);
-  if (c >= p.d || lane > 15) return;
-  const int bh = (int)(row / p.rows), r = (int)(row % p.rows), s = r / p.grp, g = r % p.grp;
-  const long oo = (((long)(bh / p.hkv) * p.sq + s) * p.hq + (bh % p.hkv) * p.grp + g) * p.d + c;
+  if (c >= p.d || lane >= L) return;
+  const int s = r / p.grp, g = r % p.grp;
+  const long oo = (((long)b * p.sq + s) * p.hq + hk * p.grp + g) * p.d + c;
   float lo[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -684,7 +766,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  xa_over_keys<T, DT, KW, false>(p, lds, b, hk, split, r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  const int nt = (xa_len(p, b) + XaKeys<DT, KW>::BK - 1) / XaKeys<DT, KW>::BK;
+  xa_over_keys<T, DT, KW>(p, lds, b, hk, (int)((long)nt * split / p.nsplit), (int)((long)nt * (split + 1) / p.nsplit), r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[SUB], any = 0;
     xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
@@ -743,22 +826,23 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
 }
 
 // dq of a row = sum over splits
-template <typename T>
+template <typename T, int DT>
 __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
   const long rows = (long)p.b * p.hkv * p.rows, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, c = (lane & 15) * 8;
+  constexpr int L = XaJoin<DT>::L;
+  const int lane = threadIdx.x & 63, c = lane % L * 8;
   if (row >= rows) return;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = lane >> 4; s < p.nsplit; s += 4) {
+  for (int s = lane / L; s < p.nsplit; s += 64 / L) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < p.d) load8(v, p.part + (s * rows + row) * p.d + c, 8);
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] += v[j];
   }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = xa_groups_sum(acc[j]);
-  if (c >= p.d || lane > 15) return;
+  for (int j = 0; j < 8; ++j) acc[j] = xa_groups_sum<L>(acc[j]);
+  if (c >= p.d || lane >= L) return;
   const int bh = (int)(row / p.rows), r = (int)(row % p.rows), s = r / p.grp, g = r % p.grp;
   store8((T*)p.dq + (((long)(bh / p.hkv) * p.sq + s) * p.hq + (bh % p.hkv) * p.grp + g) * p.d + c, acc, 8);
 }
@@ -940,7 +1024,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_bwd_few_kernel(Xa
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
-  xa_over_keys<T, DT, 4, true>(p, lds, b, hk, split, true, [&](int t, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  const int nt = (p.sk + XaKeys<DT, 4>::BK - 1) / XaKeys<DT, 4>::BK;       // tiles without a key that counts too: every key gets its gradient
+  xa_over_keys<T, DT, 4>(p, lds, b, hk, (int)((long)nt * split / p.nsplit), (int)((long)nt * (split + 1) / p.nsplit), true, [&](int t, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[1];
     xa_mine<4, NW>(words, wave, w);
     const int key = t * 128 + wave * 32 + r;
@@ -1051,7 +1136,10 @@ __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(XaParams p, long al
 // ------------------------------------------------------------------------------------------------ launches
 // How the work is cut, from sizes alone, so that the workspace query and the launch agree.
 struct XaPlan {
-  int kw, tiles, nsplit;       // forward and dq
+  int kw, tiles, bk;           // forward and dq
+  int fsplit, pairs;           // forward: runs of an entry (without lengths), of all entries (0: not cut)
+  bool ragged;
+  int nsplit;                  // dq
   int ktiles, ksplit;          // dk, dv
 };
 static int xa_clamp(long v, long lo, long hi) { return (int)(v < lo ? lo : v > hi ? hi : v); }
@@ -1063,11 +1151,16 @@ static XaPlan xa_plan(const RtpXattn* a) {
   const long wide = rtp_div_up(rows, 128) * bh;
   pl.kw = rows <= 32 ? 4 : rows <= 64 || wide < 1024 ? 2 : 1;
   pl.tiles = rtp_div_up(rows, 128 / pl.kw);
-  const long wgs = pl.tiles * bh, bk = pl.kw == 4 ? 128 : 64, nt = rtp_div_up(a->sk, bk);
-  // as many workgroups as run at once (LDS: two for each CU, one with four waves on keys of over 64 columns, three below 32); a split has at
+  const long wgs = pl.tiles * bh, nt = rtp_div_up(a->sk, pl.kw == 4 ? 128 : 64);
+  pl.bk = pl.kw == 4 ? 128 : 64;
+  // as many workgroups as run at once (LDS: two for each CU, one with four waves on keys of over 64 columns, three below 32); a split of dq has at
   // least four tiles, or its partial results cost as much as they save
   const long slots = pl.kw < 4 ? 512 : a->d > 64 ? 256 : a->d > 32 ? 512 : 768;
   pl.nsplit = xa_clamp(slots / (wgs > 0 ? wgs : 1), 1, nt / 4 > 1 ? nt / 4 : 1);
+  pl.fsplit = xa_clamp(slots / (wgs > 0 ? wgs : 1), 1, nt / XA_RUN > 1 ? nt / XA_RUN : 1);
+  pl.ragged = pl.fsplit > 1 && a->key_lens && a->b > 1 && a->b <= 64;
+  const long most = pl.fsplit > 1 ? slots / ((long)pl.tiles * a->hkv) : 0;       // at least two for each entry
+  pl.pairs = pl.fsplit == 1 ? 0 : !pl.ragged ? a->b * pl.fsplit : xa_clamp(most, 1, a->b * ((nt + XA_RUN - 1) / XA_RUN));
   pl.ktiles = rtp_div_up(a->sk, 128);
   const long kwgs = pl.ktiles * bh, rt = rtp_div_up(rows, 64);
   pl.ksplit = xa_clamp(512 / (kwgs > 0 ? kwgs : 1), 1, rt / 4 > 1 ? rt / 4 : 1);
@@ -1084,7 +1177,7 @@ static int xa_check(const RtpXattn* a) {
   if (rows * grp >= (1L << 31) || a->sk > (1 << 30)) return RTP_ERR_SHAPE;
   const XaPlan pl = xa_plan(a);
   const long bh = (long)a->b * a->hkv;
-  if (bh >= (1L << 28) || !rtp_launchable((bh * pl.nsplit + 8) * pl.tiles, 256) || !rtp_launchable((bh * pl.ksplit + 8) * pl.ktiles, 256) ||
+  if (bh >= (1L << 28) || !rtp_launchable((bh * pl.nsplit + 64) * pl.tiles, 256) || !rtp_launchable((bh * pl.ksplit + 64) * pl.ktiles, 256) ||
       !rtp_launchable(bh * rows, 16) || !rtp_launchable((long)a->b * xa_words(a->sk), 32))
     return RTP_ERR_SHAPE;
   if (!(a->scale > 0.f) || a->scale > 2e38f) return RTP_ERR_SHAPE;       // times log2(e) still finite
@@ -1113,11 +1206,17 @@ static XaParams xa_params(const RtpXattn* a) {
   p.scale_log2 = a->scale * 1.44269504088896340736f;
   return p;
 }
+static int xa_blocks(XaParams& p) {
+  // `near` heads together, where one tile has all rows and eight groups or more are left for each XCD
+  p.near = 1;
+  while (p.tiles == 1 && p.near * 2 * p.d <= 64 && p.hkv % (p.near * 2) == 0 && p.units / (p.near * 2) >= 64) p.near *= 2;
+  return (p.units / p.near + 7) / 8 * 8 * p.near * p.tiles;
+}
 static int xa_grid(XaParams& p, int tiles, int nsplit) {
   p.tiles = tiles;
   p.nsplit = nsplit;
   p.units = p.b * p.hkv * nsplit;
-  return (p.units + 7) / 8 * 8 * tiles;
+  return xa_blocks(p);
 }
 
 extern "C" long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward) {
@@ -1125,7 +1224,8 @@ extern "C" long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward) {
   const XaPlan pl = xa_plan(a);
   const long rows = (long)a->b * a->sq * a->hq;
   long n = a->key_mask ? xa_round((long)a->b * xa_words(a->sk) * 4) : 0;
-  if (!backward) return n + (pl.nsplit > 1 ? xa_round(rows * pl.nsplit * a->d * 4) + xa_round(rows * pl.nsplit * 4) : 0);
+  const long parts = (long)pl.pairs * a->sq * a->hq;
+  if (!backward) return n + xa_round(parts * a->d * 4) + xa_round(parts * 4);
   const long q = pl.nsplit > 1 ? rows * pl.nsplit * a->d * 4 : 0;
   const long kv = pl.ksplit > 1 ? 2L * pl.ksplit * a->b * a->sk * a->hkv * a->d * 4 : 0;
   return n + xa_round(rows * 4) + xa_round(q > kv ? q : kv);   // dq and dk / dv run one after the other
@@ -1202,18 +1302,21 @@ extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* 
   if (rb != RTP_OK) return rb;
   p.o = o; p.o_lo = o_lo; p.lse = lse;
   const XaPlan pl = xa_plan(a);
-  const int grid = xa_grid(p, pl.tiles, pl.nsplit);
-  const long rows = (long)a->b * a->sq * a->hq;
-  if (pl.nsplit > 1) {
+  int grid = xa_grid(p, pl.tiles, pl.fsplit);
+  if (pl.pairs) {
+    p.pairs = pl.pairs;
+    p.ragged = pl.ragged;
+    p.units = pl.pairs * a->hkv;
+    grid = xa_blocks(p);
     p.part = (float*)at;
-    p.part_lse = (float*)(at + xa_round(rows * pl.nsplit * a->d * 4));
+    p.part_lse = (float*)(at + xa_round((long)pl.pairs * a->sq * a->hq * a->d * 4));
   }
   return xa_types(a, [&](auto t, auto dt) {
     typedef decltype(t) T;
     constexpr int DT = decltype(dt)::value;
     const int r = pl.kw == 4 ? xa_fwd<T, DT, 4>(grid, st, p) : pl.kw == 2 ? xa_fwd<T, DT, 2>(grid, st, p) : xa_fwd<T, DT, 1>(grid, st, p);
-    if (r != RTP_OK || pl.nsplit == 1) return r;
-    hipLaunchKernelGGL((xattn_join_kernel<T>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
+    if (r != RTP_OK || !pl.pairs) return r;
+    hipLaunchKernelGGL((xattn_join_kernel<T, DT>), dim3(rtp_div_up((long)a->b * a->sq * a->hq, 4)), dim3(256), 0, st, p, pl.bk);
     RTP_CHECK_LAUNCH();
     return RTP_OK;
   });
@@ -1247,7 +1350,7 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
     typedef decltype(t) T;
     constexpr int DT = decltype(dt)::value;
     auto join_dq = [&]() {
-      if (pl.nsplit > 1) hipLaunchKernelGGL((xattn_dq_join_kernel<T>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
+      if (pl.nsplit > 1) hipLaunchKernelGGL((xattn_dq_join_kernel<T, DT>), dim3(rtp_div_up(rows, 4)), dim3(256), 0, st, p);
       RTP_CHECK_LAUNCH();
       return RTP_OK;
     };

@@ -386,3 +386,19 @@ def test_two_calls_at_once():
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(g, want[i % 2]))
+
+
+@pytest.mark.parametrize("b,sk,hkv,d", [(2, 4000, 1, 128), (7, 1500, 8, 16), (8, 2560, 2, 64), (33, 900, 1, 32), (64, 700, 2, 8), (64, 600, 8, 32), (65, 600, 1, 96)])
+def test_lengths_of_every_kind(b, sk, hkv, d):
+    """Few rows: runs of keys follow the entries' lengths, from none at all to every entry full."""
+    from rt_pose_amd.attention import cross_attention
+    g = torch.Generator().manual_seed(b)
+    kinds = [torch.zeros(b), torch.full((b,), sk), torch.rand(b, generator=g) * (sk + 1), (torch.rand(b, generator=g) < 0.3) * sk, torch.arange(b), torch.ones(b)]
+    kinds[3][b // 2] = sk
+    q, k, v, do, _, mask = case(b, 2, sk, 2 * hkv, hkv, d, torch.bfloat16, None, 0.8, seed=b)
+    for i, kind in enumerate(kinds):
+        lens = kind.int()
+        m = mask if i % 2 else None
+        o = cross_attention(q, k, v, lens.cuda(), m)
+        got = (o, *torch.autograd.grad(o, (q, k, v), do))
+        check(got, reference(q, k, v, seen_of(b, sk, lens, m), d ** -0.5, do))
