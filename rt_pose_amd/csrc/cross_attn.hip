@@ -469,8 +469,9 @@ __device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigne
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// waves for each SIMD that the registers and LDS allow
-template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3; };
+// waves for each SIMD that LDS allows and the registers are shared by (backward of few rows, 8 x 8 heads x 20480 keys x 64 with three: 81 us, with two,
+// which LDS allows, and no spills: 69.5; heads of 128: two 129, one 72.5)
+template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3, FEW = DT == 1 ? 3 : DT == 2 ? 2 : 1; };
 
 template <typename T, int DT, int KW>
 __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaParams p) {
@@ -988,7 +989,7 @@ template <int DT> struct XaFew {       // key tiles, then the images of do and q
   static constexpr int ROWS_IMG = 32 * XaImg<DT>::PITCH, AT = XaKeys<DT, 4>::BYTES, BYTES = AT + 2 * ROWS_IMG + 2 * 32 * 4;
 };
 template <typename T, int DT>
-__global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_bwd_few_kernel(XaParams p) {
+__global__ __launch_bounds__(256, XaWaves<DT>::FEW) void xattn_bwd_few_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
   constexpr int NW = XaKeys<DT, 4>::NW, PITCH = XaImg<DT>::PITCH;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
