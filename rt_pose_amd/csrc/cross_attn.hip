@@ -320,7 +320,7 @@ __device__ __forceinline__ void xa_store(T* row, const f32x16& x, int t, int h, 
 
 // The accumulators of the KW waves that share rows, added with the given weights in wave order.  Every wave leaves its own in LDS and gathers every
 // KW-th sixteen columns of all of them: f(q, values) for its q, columns 16 q + ...  Waves that share nothing (KW = 1) keep theirs.
-template <int DT, int KW> struct XaMeet { static constexpr int SLOT = DT * 16 * 64 * 4, BYTES = KW > 1 ? 4 * SLOT + 4 * 2 * 64 * 4 : 0; };
+template <int DT, int KW> struct XaMeet { static constexpr int SLOT = DT * 16 * 64 * 4, BYTES = KW > 1 ? 4 * SLOT : 0; };
 template <int DT, int KW, typename F>
 __device__ __forceinline__ void xa_gather(const f32x16 (&acc)[DT], const float (&weight)[KW], uint8_t* lds, int wave, F f) {
   const int lane = threadIdx.x & 63, kw = wave % KW;
@@ -334,6 +334,7 @@ __device__ __forceinline__ void xa_gather(const f32x16 (&acc)[DT], const float (
     }
   } else {
     constexpr int SLOT = XaMeet<DT, KW>::SLOT / 4;
+    __syncthreads();             // the weights have been read from the same place
     float* mine = (float*)lds + wave * SLOT + lane;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
@@ -470,8 +471,9 @@ __device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigne
 
 // ------------------------------------------------------------------------------------------------ forward
 // waves for each SIMD that LDS allows and the registers are shared by (backward of few rows, 8 x 8 heads x 20480 keys x 64 with three: 81 us, with two,
-// which LDS allows, and no spills: 69.5; heads of 128: two 129, one 72.5)
-template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3, FEW = DT == 1 ? 3 : DT == 2 ? 2 : 1; };
+// which LDS allows, and no spills: 69.5; heads of 128: two 129, one 72.5; dk and
+// dv of 4 x 8 heads of 128, 2560 rows x 5120 keys: two with spills 640, one 572)
+template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3, FEW = DT == 1 ? 3 : DT == 2 ? 2 : 1, DKV = DT == 4 ? 1 : BWD; };
 
 template <typename T, int DT, int KW>
 __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaParams p) {
@@ -558,7 +560,7 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaPara
   float weight[KW];              // of the waves that share these rows
   if constexpr (KW > 1) {
     __syncthreads();             // nobody reads the tiles any more
-    float* st = (float*)(lds + 4 * XaMeet<DT, KW>::SLOT);
+    float* st = (float*)lds;
     st[wave * 128 + lane] = m;
     st[wave * 128 + 64 + lane] = l;
     __syncthreads();
@@ -726,7 +728,7 @@ __device__ __forceinline__ void xa_store_dq(const XaParams& p, const f32x16 (&ac
   float weight[KW];
   if constexpr (KW > 1) {        // fp16: each wave has a factor of its own
     __syncthreads();
-    float* st = (float*)(lds + 4 * XaMeet<DT, KW>::SLOT);
+    float* st = (float*)lds;
     st[wave * 64 + (threadIdx.x & 63)] = out;
     __syncthreads();
 #pragma unroll
@@ -856,7 +858,7 @@ template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane o
   static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, BYTES = 2 * BUF;
 };
 template <typename T, int DT>
-__global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dkv_kernel(XaParams p) {
+__global__ __launch_bounds__(256, XaWaves<DT>::DKV) void xattn_dkv_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
   typedef XaRows<DT> R;
   constexpr int BR = R::BR, IMG = R::IMG, BUF = R::BUF;
