@@ -362,9 +362,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
 template <typename O, bool SQUARE>
 static int mm8_launch(Mm8Params p, hipStream_t st) {
   const long tiles128 = (long)rtp_div_up(p.m, 128) * rtp_div_up(p.n, 128);
-  // Up to 64 rows, or where 128 x 128 tiles would leave most CUs without one.  m x 4096 x 4096: m = 128 (32 tiles) 17.9 us against 23.4 in tiles,
-  // m = 300 (96 tiles) 39.4 against 23.6; 64 x 8192 x 8192 32.5 against 46.
-  if (p.m <= 64 || tiles128 < 48) {
+  // Up to 64 rows, or so few tiles that their sums are better shared by more waves.  m x 4096 x 4096: m = 128 (32 tiles of 128 x 128) 18.4 us against
+  // 17.3 in tiles, fp32 19.1 against 26.7; 128 x 2048 x 4096 (16) 15.3 against 17.4; 64 x 8192 x 8192 32.5 against 46.
+  if (p.m <= 64 || tiles128 < (sizeof(O) == 4 ? 48 : 32)) {
     // as many n per workgroup as leave one for each CU: b is then read once, a from L2 less often
     const int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
     const long rows = rtp_div_up(p.m, 16 * mt);
@@ -393,7 +393,7 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     RTP_CHECK_LAUNCH();
     return RTP_OK;
   };
-  static bool once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES];
+  static bool once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES], once64[RTP_MAX_DEVICES];
   // 256 x 256 halves what is staged per product and wins where the sum is long and its tiles fill whole rounds of the 256 CUs (8192^3: 505 us
   // against 580, 4096^3: 72 against 77); 128 x 128, two workgroups to a CU, where one's start and end hide behind the other's sum
   // (163840 x 256 x 384: 40 us against 57, x 1024: 71 against 87).  The exact road needs the registers of the small tile.
@@ -401,6 +401,9 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     const long rounds = (tiles256 + 255) / 256;
     if (p.kb >= 16 && tiles256 >= 256 && tiles256 * 5 >= rounds * 256 * 4) return go(mm8_tile_kernel<O, 256, 256, 64, 128, SQUARE>, 256, 256, 512, once256);
   }
+  // half a tile of n where whole ones would not give every CU one, or where there is no more (m x 4096 x 4096: m = 300 18.1 us against 23.6, fp32 27.9
+  // against 41.3, m = 1500 40.0 against 33.9; 40000 x 64 x 256 4.5 against 6.2)
+  if (tiles128 <= 256 || p.n <= 64) return go(mm8_tile_kernel<O, 128, 64, 64, 32, SQUARE>, 128, 64, 256, once64);
   return go(mm8_tile_kernel<O, 128, 128, 64, 64, SQUARE>, 128, 128, 256, once128);
 }
 

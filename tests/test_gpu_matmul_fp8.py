@@ -160,3 +160,12 @@ def test_far_rows_and_sizes_beyond():
         kb = -(-k // 128)
         with pytest.raises(ValueError):
             matmul_fp8(byte.expand(m, k), one.expand(m, kb), byte.expand(n, k), one.expand(n, kb))
+
+
+@pytest.mark.parametrize("m,n,k", [(4200, 50, 300), (6200, 64, 129), (130, 4200, 390), (1000, 700, 640), (4000, 1000, 130), (520, 1090, 1111)])
+@pytest.mark.parametrize("square", [True, False])
+def test_tiles_of_half_the_width(m, n, k, square):
+    from rt_pose_amd.fp8 import matmul_fp8
+    (a, sa), (b, sb) = operand(m, k, False, m + n), operand(n, k, square, m + n + 1)
+    for t in OUT:
+        check(matmul_fp8(a, sa, b, sb, t), a, sa, b, sb, square)
