@@ -470,7 +470,13 @@ __device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigne
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// waves for each SIMD that LDS allows and the registers are shared by (backward of few rows, 8 x 8 heads x 20480 keys x 64 with three: 81 us, with two,
+// Many rows are bound by the matrix and vector units together: 32 x 32 scores of a head of 64 are 8 matrix instructions (256 cycles) and a dozen vector
+// instructions a score, the exponential at a quarter of their rate.  8 x 8 heads of 64, 2048 x 2048: 84 us, 0.82 PFLOP/s; left out one at a time,
+// staging, exponentials, masks or either product give about a tenth each.  4 x 8 heads of 64, 2560 rows x 0 to 5120 keys: 90 us, 0.51 PFLOP/s: all
+// workgroups with keys are resident at once, four to a CU, and the CU with two long ones ends last.
+// Few rows are bound by memory and latency: one row, 8 entries of 0 to 2560 keys x 8 heads of 128: 15 us and 4.5 for the join (42 MB, 8.5 us at a large
+// copy's rate); one tile of keys alone takes 7.4 us, further ones 2.1 each.
+// Waves for each SIMD that LDS allows and the registers are shared by (backward of few rows, 8 x 8 heads x 20480 keys x 64 with three: 81 us, with two,
 // which LDS allows, and no spills: 69.5; heads of 128: two 129, one 72.5; dk and
 // dv of 4 x 8 heads of 128, 2560 rows x 5120 keys: two with spills 640, one 572)
 template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3, FEW = DT == 1 ? 3 : DT == 2 ? 2 : 1, DKV = DT == 4 ? 1 : BWD; };
@@ -743,7 +749,8 @@ __device__ __forceinline__ void xa_store_dq(const XaParams& p, const f32x16 (&ac
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dq
-// the forward kernel's shape: s^T and dp^T with a lane per row, dq^T = k^T ds^T, k read from LDS both ways
+// the forward kernel's shape: s^T and dp^T with a lane per row, dq^T = k^T ds^T, k read from LDS both ways.  Three products for the forward pass's two:
+// 4 x 8 heads of 64, 2560 rows x 0 to 5120 keys 107 us, 0.64 PFLOP/s.
 template <typename T, int DT, int KW>
 __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
@@ -853,7 +860,8 @@ __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
 // ------------------------------------------------------------------------------------------------ backward: dk, dv
 // Each wave keeps 32 keys (k, v as second operands in registers, dk^T and dv^T as accumulators) and walks the rows: s = q k^T and
 // dp = do v^T with a lane per key, then dv^T += do^T p and dk^T += q^T ds with q and do read from LDS both ways.  A lane's key touches its own
-// column of the products alone, so a masked key needs nothing inside the loop: zeros are written for it at the end.
+// column of the products alone, so a masked key needs nothing inside the loop: zeros are written for it at the end.  Four products: at the same sizes
+// 135 us, 0.68 PFLOP/s; 640 workgroups with keys, of one length, two or three to a CU.
 template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane of the wave that brings their L or delta; two buffers
   static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, BYTES = 2 * BUF;
 };
@@ -985,7 +993,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::DKV) void xattn_dkv_kernel(XaPara
 
 // ------------------------------------------------------------------------------------------------ backward, up to 32 rows
 // All rows are one tile, so a tile of keys is done with once read: its dk and dv are complete, and dq is summed on.  One pass over k and v, which
-// are the work (8 x 8 heads of 32, 15 rows x 20480 keys: dq and dk / dv one after the other 105 us, here 67).  Each wave takes 32 keys of a tile both
+// are the work (8 x 8 heads of 32, 15 rows x 0 to 20480 keys: dq and dk / dv one after the other 105 us, here 67: 252 MB with the zeros of keys that
+// do not count, 3.8 TB/s; a large copy's rate would be 51 us for forward and backward together).  Each wave takes 32 keys of a tile both
 // ways round from the same fragments, operands exchanged: a lane per row for ds^T and dq, a lane per key for p, ds and dk / dv.
 template <int DT> struct XaFew {       // key tiles, then the images of do and q, then L and delta of the rows
   static constexpr int ROWS_IMG = 32 * XaImg<DT>::PITCH, AT = XaKeys<DT, 4>::BYTES, BYTES = AT + 2 * ROWS_IMG + 2 * 32 * 4;

@@ -83,7 +83,8 @@ __device__ __forceinline__ void store4(O* p, f32x4 v, int n) {
 // ------------------------------------------------------------------------------------------------ few rows
 // The eight waves of a workgroup share one tile of 16 * NT n x 16 * MT m and split the blocks of k; their sums meet in LDS in wave order.
 // Operands go from memory straight to registers, DEPTH blocks in flight.  Nothing is staged: a row of b is used by this workgroup alone, and the
-// rows of a are few enough to come from L2.
+// rows of a are few enough to come from L2.  4 x 4096 x 4096: 6.0 us for 17 MB of b, 2.8 TB/s: the launch, one trip to memory of four blocks a wave
+// and the meeting of the waves.
 #define MM8_FEW_WAVES 8
 template <typename O, int MT, int NT, int DEPTH, bool SQUARE>
 __global__ __launch_bounds__(64 * MM8_FEW_WAVES) void mm8_few_kernel(Mm8Params p) {
@@ -401,9 +402,9 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     const long rounds = (tiles256 + 255) / 256;
     if (p.kb >= 16 && tiles256 >= 256 && tiles256 * 5 >= rounds * 256 * 4) return go(mm8_tile_kernel<O, 256, 256, 64, 128, SQUARE>, 256, 256, 512, once256);
   }
-  // half a tile of n where whole ones would not give every CU one, or where there is no more (m x 4096 x 4096: m = 300 18.1 us against 23.6, fp32 27.9
-  // against 41.3, m = 1500 40.0 against 33.9; 40000 x 64 x 256 4.5 against 6.2)
-  if (tiles128 <= 256 || p.n <= 64) return go(mm8_tile_kernel<O, 128, 64, 64, 32, SQUARE>, 128, 64, 256, once64);
+  // half a tile of n where whole ones would not give every CU one (m x 4096 x 4096: m = 300 18.1 us against 23.6, fp32 27.9 against 41.3, m = 1500
+  // 40.0 against 33.9), or where a large part of them would be empty (40000 x 64 x 256 4.5 against 6.2, 163840 x 192 x 300 30.9 against 33.5)
+  if (tiles128 <= 256 || p.n <= 64 || (p.n > 128 && p.n <= 192)) return go(mm8_tile_kernel<O, 128, 64, 64, 32, SQUARE>, 128, 64, 256, once64);
   return go(mm8_tile_kernel<O, 128, 128, 64, 64, SQUARE>, 128, 128, 256, once128);
 }
 

