@@ -557,7 +557,8 @@ int rtp_modulated_deform_conv_backward(const float* input, const float* weight, 
 #define RTP_DT_BF16 2
 /* "8 bits" is OCP e4m3 (largest value 448), held in rows of at least the length rounded up to 16 bytes, 16-byte aligned.  Row strides
  * (`*_rs`) are in elements; rows of the other types need no alignment.  An operand is q * scale with one fp32 scale for each 128 columns
- * of a row (scale[rows][ceil(cols / 128)]) or for each 128 x 128 block ([ceil(rows / 128)][ceil(cols / 128)]).
+ * of a row (scale[rows][ceil(cols / 128)]) or for each 128 x 128 block ([ceil(rows / 128)][ceil(cols / 128)]).  What a launch cannot count
+ * (rows of up to 2^28 for the narrowest norm) is refused with RTP_ERR_SHAPE.
  *
  * Root-mean-square norm (csrc/token_norm.hip): s = round(x + res), y = s / sqrt(mean(s^2) + eps) * w.  res may be NULL (s = x); s may be
  * NULL when res is.  w_dtype: the values' type or RTP_DT_F32.  h <= 16384.  s, y, dx: contiguous rows of h.
@@ -572,20 +573,21 @@ int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int w_dtype, c
                          void* dw, float* part, long rows, int h, int dtype, float eps, void* stream);
 /* x -> q, scale with blocks of 1 x 128 (square = 0) or 128 x 128 (square = 1): a = max(largest magnitude, 2^-100), q = e4m3(x * (448 / a)),
  * scale = a / 448.  turned = 1: x is given by columns, x[r][c] at c * x_rs + r (a transpose that is never written out).  The bytes between
- * cols and cols rounded up to 16 are written too. */
+ * cols and cols rounded up to 16 may be written too.  cols <= 2^30. */
 int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, float* scale, long rows, int cols, int square, int dtype,
                      void* stream);
 
 /* out[m][n] = the product of a [m][k] and the transpose of b [n][k], both in 8 bits with scales (csrc/matmul_fp8.hip).  sa: [m][ceil(k / 128)];
  * sb: [ceil(n / 128)][ceil(k / 128)] (b_square = 1) or [n][ceil(k / 128)].  Rows of a and b are readable up to k rounded up to 16; what stands
- * there does not count.  out: row stride n, out_dtype any of the three. */
+ * there does not count.  out: row stride n, out_dtype any of the three.  lda, ldb <= 2^22 (and so k); m, n <= 2^30. */
 int rtp_matmul_fp8(const void* a, long lda, const float* sa, const void* b, long ldb, const float* sb, int b_square, void* out, int m, int n,
                    int k, int out_dtype, void* stream);
 
 /* Cross attention (csrc/cross_attn.hip): o[b][i][h] = sum_j softmax_j(scale q[b][i][h] . k[b][j][h / (hq / hkv)]) v[b][j][...] over the keys j that
  * count in batch entry b: j < key_lens[b] (clamped to 0 .. sk; NULL: all) and key_mask[b][j] (bytes, strides m_bs and m_ss; NULL: all).  Keys that
  * do not count are not read, whatever they hold; a row without keys gives zeros and takes part in no gradient.  fp16 or bf16, d a multiple of 8
- * up to 128, scale > 0.  Strides in elements, of batch, token and head; the columns of a head are contiguous; every row 16-byte aligned.
+ * up to 128, 0 < scale <= 2e38.  Strides in elements, of batch, token and head; the columns of a head are contiguous; every row 16-byte aligned;
+ * token strides of 0 to 2^23, head stride of q and d_o times hq / hkv up to 2^28.
  * o, dq: contiguous [b][sq][hq][d]; dk, dv: contiguous [b][sk][hkv][d], zeros at keys that do not count.  dq, or dk and dv, may be NULL.
  * For a backward pass the forward pass also leaves o_lo (what o's rounding left over, o's type and shape) and lse ([b][hkv][sq * hq / hkv] fp32:
  * base-2 logarithm of the sum of exponentials); both NULL otherwise.  o_bs, o_ss, o_hs: of d_o.  ws: rtp_xattn_workspace_bytes(a, backward) bytes,

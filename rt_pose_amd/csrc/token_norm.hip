@@ -181,14 +181,17 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
   }
 }
 
-// dw[c] = sum of the partial rows: 16 columns (one 64-byte line) x 64 row slots per workgroup, so that few columns still make enough loads
+// dw[c] = sum of the partial rows: 16 columns (one 64-byte line) x 64 row slots per workgroup, so that few columns still make enough loads,
+// eight of a thread's at once (1024 rows of 1024: 4.1 us, one after the other 6.4)
 template <typename W>
 __global__ __launch_bounds__(1024) void rmsnorm_dw_kernel(const float* part, int slots, int h, W* dw) {
   __shared__ float red[64][17];
   const int cl = threadIdx.x & 15, k = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
   float t = 0.f;
-  if (c < h)
+  if (c < h) {
+#pragma unroll 8
     for (int i = k; i < slots; i += 64) t += part[(long)i * h + c];
+  }
   red[k][cl] = t;
   __syncthreads();
   for (int o = 32; o > 0; o >>= 1) {
