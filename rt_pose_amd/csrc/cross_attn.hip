@@ -471,7 +471,7 @@ __device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigne
 
 // ------------------------------------------------------------------------------------------------ forward
 // Many rows are bound by the matrix and vector units together: 32 x 32 scores of a head of 64 are 8 matrix instructions (256 cycles) and a dozen vector
-// instructions a score, the exponential at a quarter of their rate.  8 x 8 heads of 64, 2048 x 2048: 84 us, 0.82 PFLOP/s; left out one at a time,
+// instructions a score, the exponential at a quarter of the others' rate.  8 x 8 heads of 64, 2048 x 2048: 84 us, 0.82 PFLOP/s; left out one at a time,
 // staging, exponentials, masks or either product give about a tenth each.  4 x 8 heads of 64, 2560 rows x 0 to 5120 keys: 90 us, 0.51 PFLOP/s: all
 // workgroups with keys are resident at once, four to a CU, and the CU with two long ones ends last.
 // Few rows are bound by memory and latency: one row, 8 entries of 0 to 2560 keys x 8 heads of 128: 15 us and 4.5 for the join (42 MB, 8.5 us at a large
@@ -479,7 +479,9 @@ __device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigne
 // Waves for each SIMD that LDS allows and the registers are shared by (backward of few rows, 8 x 8 heads x 20480 keys x 64 with three: 81 us, with two,
 // which LDS allows, and no spills: 69.5; heads of 128: two 129, one 72.5; dk and
 // dv of 4 x 8 heads of 128, 2560 rows x 5120 keys: two with spills 640, one 572)
-template <int DT> struct XaWaves { static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3, FEW = DT == 1 ? 3 : DT == 2 ? 2 : 1, DKV = DT == 4 ? 1 : BWD; };
+template <int DT> struct XaWaves {
+  static constexpr int FWD = DT == 1 ? 4 : DT == 2 ? 3 : 2, BWD = DT > 2 ? 2 : 3, FEW = DT == 1 ? 3 : DT == 2 ? 2 : 1, DKV = DT == 4 ? 1 : BWD;
+};
 
 template <typename T, int DT, int KW>
 __global__ __launch_bounds__(256, XaWaves<DT>::FWD) void xattn_fwd_kernel(XaParams p) {
@@ -777,7 +779,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParam
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
   const int nt = (xa_len(p, b) + XaKeys<DT, KW>::BK - 1) / XaKeys<DT, KW>::BK;
-  xa_over_keys<T, DT, KW>(p, lds, b, hk, (int)((long)nt * split / p.nsplit), (int)((long)nt * (split + 1) / p.nsplit), r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  const int t0 = (int)((long)nt * split / p.nsplit), t1 = (int)((long)nt * (split + 1) / p.nsplit);
+  xa_over_keys<T, DT, KW>(p, lds, b, hk, t0, t1, r0 < p.rows, [&](int, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[SUB], any = 0;
     xa_mine<KW, NW>(words, kw, w);
 #pragma unroll
@@ -1037,7 +1040,8 @@ __global__ __launch_bounds__(256, XaWaves<DT>::FEW) void xattn_bwd_few_kernel(Xa
     for (int i = 0; i < 16; ++i) acc[t][i] = 0.f;
 
   const int nt = (p.sk + XaKeys<DT, 4>::BK - 1) / XaKeys<DT, 4>::BK;       // tiles without a key that counts too: every key gets its gradient
-  xa_over_keys<T, DT, 4>(p, lds, b, hk, (int)((long)nt * split / p.nsplit), (int)((long)nt * (split + 1) / p.nsplit), true, [&](int t, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
+  const int t0 = (int)((long)nt * split / p.nsplit), t1 = (int)((long)nt * (split + 1) / p.nsplit);
+  xa_over_keys<T, DT, 4>(p, lds, b, hk, t0, t1, true, [&](int t, const uint8_t* ki, const uint8_t* vi, const unsigned (&words)[NW]) {
     unsigned w[1];
     xa_mine<4, NW>(words, wave, w);
     const int key = t * 128 + wave * 32 + r;
