@@ -590,7 +590,8 @@ int rtp_matmul_fp8(const void* a, long lda, const float* sa, const void* b, long
  * token strides of 0 to 2^23, head stride of q and d_o times hq / hkv up to 2^28.
  * o, dq: contiguous [b][sq][hq][d]; dk, dv: contiguous [b][sk][hkv][d], zeros at keys that do not count.  dq, or dk and dv, may be NULL.
  * For a backward pass the forward pass also leaves o_lo (what o's rounding left over, o's type and shape) and lse ([b][hkv][sq * hq / hkv] fp32:
- * base-2 logarithm of the sum of exponentials); both NULL otherwise.  o_bs, o_ss, o_hs: of d_o.  ws: rtp_xattn_workspace_bytes(a, backward) bytes,
+ * base-2 logarithm of the sum of exponentials, with a key_mask followed, from the next multiple of 64 on, by the masks' bits: b * 4 * ceil(sk / 128)
+ * words); both NULL otherwise.  o_bs, o_ss, o_hs: of d_o.  ws: rtp_xattn_workspace_bytes(a, backward) bytes,
  * 256-byte aligned; -1 for what the entries refuse.  No atomics: results do not depend on scheduling. */
 typedef struct RtpXattn {
   const void *q, *k, *v;

@@ -88,7 +88,10 @@ class CrossAttentionFunction(Function):
     @staticmethod
     def forward(ctx, q, k, v, key_lens, key_mask, scale):
         a = _operands(q, k, v, key_lens, key_mask, scale)
-        o_lo, lse = like(q), q.new_empty(q.shape[:3].numel(), dtype=torch.float32)
+        n = q.shape[:3].numel()
+        if key_mask is not None:                    # room for its bits behind
+            n = -(-n // 64) * 64 + q.shape[0] * 4 * -(-k.shape[1] // 128)
+        o_lo, lse = like(q), q.new_empty(n, dtype=torch.float32)
         o = _forward(a, q, o_lo, lse)
         ctx.operands, ctx.scale, ctx.layout = a, scale, (q.stride(), k.stride(), v.stride())
         ctx.save_for_backward(q, k, v, key_lens, key_mask, o, o_lo, lse)

@@ -1239,17 +1239,20 @@ extern "C" long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward) {
   if (xa_check(a) != RTP_OK) return -1;
   const XaPlan pl = xa_plan(a);
   const long rows = (long)a->b * a->sq * a->hq;
-  long n = a->key_mask ? xa_round((long)a->b * xa_words(a->sk) * 4) : 0;
+  const long n = a->key_mask && !backward ? xa_round((long)a->b * xa_words(a->sk) * 4) : 0;
   const long parts = (long)pl.pairs * a->sq * a->hq;
   if (!backward) return n + xa_round(parts * a->d * 4) + xa_round(parts * 4);
   const long q = pl.nsplit > 1 ? rows * pl.nsplit * a->d * 4 : 0;
   const long kv = pl.ksplit > 1 ? 2L * pl.ksplit * a->b * a->sk * a->hkv * a->d * 4 : 0;
-  return n + xa_round(rows * 4) + xa_round(q > kv ? q : kv);   // dq and dk / dv run one after the other
+  return xa_round(rows * 4) + xa_round(q > kv ? q : kv);   // dq and dk / dv run one after the other
 }
 
-static int xa_bits(const RtpXattn* a, XaParams& p, uint8_t*& ws, hipStream_t st) {
+// where the masks' bits stand behind lse, for the backward pass
+static unsigned* xa_kept(const RtpXattn* a, const float* lse) { return (unsigned*)lse + (((long)a->b * a->sq * a->hq + 63) & ~63L); }
+
+static int xa_bits(const RtpXattn* a, XaParams& p, float* lse, uint8_t*& ws, hipStream_t st) {
   if (!a->key_mask) return RTP_OK;
-  p.bits = (unsigned*)ws;
+  p.bits = lse ? xa_kept(a, lse) : (unsigned*)ws;
   ws += xa_round((long)a->b * p.words * 4);
   hipLaunchKernelGGL(xattn_bits_kernel, dim3((unsigned)rtp_div_up(p.words, 8) * a->b), dim3(256), 0, st, (const uint8_t*)a->key_mask, a->m_bs, a->m_ss, a->key_lens,
                      (unsigned*)p.bits, a->sk, p.words);
@@ -1314,7 +1317,7 @@ extern "C" int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* 
   RtpProfScope prof(RTP_FAM_POINTWISE, st);
   XaParams p = xa_params(a);
   uint8_t* at = (uint8_t*)ws;
-  const int rb = xa_bits(a, p, at, st);
+  const int rb = xa_bits(a, p, lse, at, st);
   if (rb != RTP_OK) return rb;
   p.o = o; p.o_lo = o_lo; p.lse = lse;
   const XaPlan pl = xa_plan(a);
@@ -1353,8 +1356,7 @@ extern "C" int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* 
   RtpProfScope prof(RTP_FAM_POINTWISE, st);
   XaParams p = xa_params(a);
   uint8_t* at = (uint8_t*)ws;
-  const int rb = xa_bits(a, p, at, st);
-  if (rb != RTP_OK) return rb;
+  if (a->key_mask) p.bits = xa_kept(a, lse);
   const long rows = (long)a->b * a->sq * a->hq;
   p.d_o = d_o; p.o_bs = o_bs; p.o_ss = o_ss; p.o_hs = o_hs;
   p.o = (void*)o; p.o_lo = (void*)o_lo; p.lse_in = lse;
