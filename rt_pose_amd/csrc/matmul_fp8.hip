@@ -23,6 +23,7 @@ struct Mm8Params {
   long lda, ldb, ldo;
   int m, n, k, kb;          // kb = ceil(k / 128)
   int tiles_m, tiles_n;
+  bool far;                 // out is larger than the last-level cache
 };
 
 // one lane's 32 values of an operand, as the instruction takes them
@@ -353,7 +354,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
       for (int i = 0; i < NT; i += 2) {
         const int nc = n0 + wn + i * 16 + g * 8;
         const float v[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
-        store8(o + nc, v, p.n - nc);
+        if (p.far) store8_far(o + nc, v, p.n - nc);
+        else store8(o + nc, v, p.n - nc);
       }
     }
   }
@@ -418,7 +420,10 @@ extern "C" int rtp_matmul_fp8(const void* a, long lda, const float* sa, const vo
   if (((size_t)a & 15) || ((size_t)b & 15) || (lda & 15) || (ldb & 15)) return RTP_ERR_ALIGN;
   hipStream_t st = (hipStream_t)stream;
   RtpProfScope prof(RTP_FAM_CONV, st);
-  Mm8Params p{(const uint8_t*)a, (const uint8_t*)b, sa, sb, out, lda, ldb, n, m, n, k, (k + 127) >> 7, 0, 0};
+  Mm8Params p{(const uint8_t*)a, (const uint8_t*)b, sa, sb, out, lda, ldb, n, m, n, k, (k + 127) >> 7, 0, 0, false};
+  // 163840 x 1024 x 384 134 us, 147 without, in fp32 215 and 238; 65536 x 4096 x 512 236 and 244; but 8192 x 8192 x 512 (134 MB), done always, 61
+  // against 55
+  p.far = (long)m * n * (out_dtype == RTP_DT_F32 ? 4 : 2) > RTP_FAR_BYTES;
   auto go = [&](auto o) {
     typedef decltype(o) O;
     return b_square ? mm8_launch<O, true>(p, st) : mm8_launch<O, false>(p, st);

@@ -43,6 +43,22 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
   }
 }
 
+// Outputs of more than the last-level cache drive each other out of it before the next pass reads them: they are stored past it.
+#define RTP_FAR_BYTES (256L << 20)
+// as store8, marked to leave the caches first
+template <typename T>
+__device__ __forceinline__ void store8_far(T* p, const float (&v)[8], int n) {
+  typedef T tv8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (n >= 8) {
+    tv8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
+    __builtin_nontemporal_store(r, (tv8*)p);
+  } else {
+    store8(p, v, n);
+  }
+}
+
 // eight values times `up` -> eight e4m3 bytes, round to nearest even (|v * up| <= 448 up to one fp32 rounding: never out of range)
 __device__ __forceinline__ i32x2 to_fp8x8(const float (&v)[8], float up) {
   i32x2 r = {0, 0};

@@ -39,10 +39,11 @@ struct NormParams {
   float* scale;
   long x_rs, res_rs, q_rs, rows;
   int h;
+  bool far;                  // s and y are larger than the last-level cache
   float eps;
 };
 
-// Bound by HBM: 20480 x 1024 bf16 with the residual 34 us for 168 MB, 4.9 TB/s; 16384 x 8192 to 8 bits 187 us for 944 MB, 5.05 TB/s (a large copy
+// Bound by HBM: 20480 x 1024 bf16 with the residual 34 us for 168 MB, 4.9 TB/s; 16384 x 8192 to 8 bits 174 us for 944 MB, 5.4 TB/s (a large copy
 // moves 4.96).  8 x 4096, a token's rows: 4.3 us, one trip to memory and the launch.
 template <typename T, typename W, int LPR, int NV, bool OUT8>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(NormParams p) {
@@ -71,7 +72,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(Norm
   for (int i = 0; i < NV; ++i) load8(wv[i], (const W*)p.w + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
   if (so) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) store8(so + (lane + i * LPR) * 8, v[i], p.h - (lane + i * LPR) * 8);
+    for (int i = 0; i < NV; ++i) {
+      if (p.far) store8_far(so + (lane + i * LPR) * 8, v[i], p.h - (lane + i * LPR) * 8);
+      else store8(so + (lane + i * LPR) * 8, v[i], p.h - (lane + i * LPR) * 8);
+    }
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -84,7 +88,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(Norm
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rho * wv[i][j];
     if constexpr (!OUT8) {
-      store8((T*)p.y + row * p.h + c, v[i], n);
+      if (p.far) store8_far((T*)p.y + row * p.h + c, v[i], n);
+      else store8((T*)p.y + row * p.h + c, v[i], n);
     } else {
       // a block of 128 columns = 16 neighbouring lanes; columns behind the row's end are zeros and change nothing
       float a = amax8(v[i]);
@@ -229,12 +234,16 @@ static int norm_types(int dtype, int w_dtype, F f) {
 }
 
 template <bool OUT8>
-static int norm_forward(const NormParams& p, int dtype, int w_dtype, hipStream_t st) {
+static int norm_forward(NormParams p, int dtype, int w_dtype, hipStream_t st) {
   if (p.rows < 0 || p.h < 1 || p.rows >= (1L << 31)) return RTP_ERR_SHAPE;
   if (p.h > NORM_MAX_H) return RTP_ERR_UNSUPPORTED;
   if (p.rows == 0) return RTP_OK;
   if (!p.x || !p.w || (p.res && !p.s)) return RTP_ERR_SHAPE;
   RtpProfScope prof(RTP_FAM_NORM, st);
+  // 16384 x 8192 to 8 bits (s of 268 MB) 174 us, 187 without; 40960 x 2048 ten times in a row, each on the last one's outputs (2 x 168 MB), 118
+  // against 124; but 20480 x 1024 (2 x 42 MB), done always, 31.4 against 27.9.
+  const long size = dtype == RTP_DT_F32 ? 4 : 2;
+  p.far = p.rows * p.h * ((p.s ? size : 0) + (OUT8 ? 1 : size)) > RTP_FAR_BYTES;
   return norm_types(dtype, w_dtype, [&](auto t, auto w) {
     return norm_shape(p.h, [&](auto lpr, auto nv) {
       constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, THREADS = LPR > 256 ? LPR : 256;
@@ -250,7 +259,7 @@ static int norm_forward(const NormParams& p, int dtype, int w_dtype, hipStream_t
 extern "C" int rtp_rmsnorm_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* y, void* s,
                                    long rows, int h, int dtype, float eps, void* stream) {
   if (rows > 0 && !y) return RTP_ERR_SHAPE;
-  NormParams p{x, res, w, y, s, nullptr, nullptr, x_rs, res_rs, 0, rows, h, eps};
+  NormParams p{x, res, w, y, s, nullptr, nullptr, x_rs, res_rs, 0, rows, h, false, eps};
   return norm_forward<false>(p, dtype, w_dtype, (hipStream_t)stream);
 }
 
@@ -259,7 +268,7 @@ extern "C" int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res
   if (rows > 0 && (!q || !scale)) return RTP_ERR_SHAPE;
   if (q_rs < ((h + 15) & ~15)) return RTP_ERR_SHAPE;
   if (((size_t)q & 15) || (q_rs & 15)) return RTP_ERR_ALIGN;
-  NormParams p{x, res, w, nullptr, s, (uint8_t*)q, scale, x_rs, res_rs, q_rs, rows, h, eps};
+  NormParams p{x, res, w, nullptr, s, (uint8_t*)q, scale, x_rs, res_rs, q_rs, rows, h, false, eps};
   return norm_forward<true>(p, dtype, w_dtype, (hipStream_t)stream);
 }
 

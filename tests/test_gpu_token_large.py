@@ -114,3 +114,16 @@ def test_gradients_behind_the_32nd_bit():
         assert bool(((dk[:, -200:].double() - total).abs() <= tol + t2 + 2.0 ** -8 * (total.abs() + tol + t2)).all())
         assert not bool(dk[:, :-200].any())
         del o, dq, dk, big
+
+
+@pytest.mark.parametrize("dtype,h", [(torch.float16, 777), (torch.float32, 1031), (BF, 136)])
+def test_outputs_larger_than_the_caches_hold(dtype, h):
+    from rt_pose_amd.rmsnorm import add_rms_norm, add_rms_norm_fp8, rms_norm
+    rows = (2 ** 28 + 2 ** 20) // (h * torch.finfo(dtype).bits // 8)
+    x = torch.randn(rows, h, device="cuda", generator=torch.Generator(device="cuda").manual_seed(h)).to(dtype)
+    w = torch.rand(h, device="cuda")
+    some = torch.cat((x[:33], x[rows // 2:rows // 2 + 40], x[-41:]))
+    pick = lambda t: torch.cat((t[:33], t[rows // 2:rows // 2 + 40], t[-41:]))
+    for a, b in ((rms_norm(x, w), rms_norm(some, w)), *zip(add_rms_norm(x, x, w), add_rms_norm(some, some, w)),
+                 *zip(add_rms_norm_fp8(x, x, w), add_rms_norm_fp8(some, some, w))):
+        assert torch.equal(pick(a.view(torch.uint8) if a.dtype.itemsize == 1 else a), b.view(torch.uint8) if b.dtype.itemsize == 1 else b)
