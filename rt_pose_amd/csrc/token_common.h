@@ -28,6 +28,24 @@ __device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
     for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.f;
   }
 }
+// as load8, marked to leave the caches first
+template <typename T>
+__device__ __forceinline__ void load8_once(float (&v)[8], const T* p, int n) {
+  typedef T tv8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (n >= 8) {
+    const tv8 r = __builtin_nontemporal_load((const tv8*)p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
+  } else {
+    load8(v, p, n);
+  }
+}
+// load8 or load8_once, by a condition that all lanes share
+template <typename T>
+__device__ __forceinline__ void load8_if(bool once, float (&v)[8], const T* p, int n) {
+  if (once) load8_once(v, p, n);
+  else load8(v, p, n);
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
   typedef T tv8 __attribute__((ext_vector_type(8)));

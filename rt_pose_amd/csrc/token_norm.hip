@@ -40,10 +40,11 @@ struct NormParams {
   long x_rs, res_rs, q_rs, rows;
   int h;
   bool far;                  // s and y are larger than the last-level cache
+  bool once;                 // x and res are far larger than the L2s
   float eps;
 };
 
-// Bound by HBM: 20480 x 1024 bf16 with the residual 34 us for 168 MB, 4.9 TB/s; 16384 x 8192 to 8 bits 174 us for 944 MB, 5.4 TB/s (a large copy
+// Bound by HBM: 20480 x 1024 bf16 with the residual 34 us for 168 MB, 4.9 TB/s; 16384 x 8192 to 8 bits 167 us for 944 MB, 5.65 TB/s (a large copy
 // moves 4.96).  8 x 4096, a token's rows: 4.3 us, one trip to memory and the launch.
 template <typename T, typename W, int LPR, int NV, bool OUT8>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(NormParams p) {
@@ -58,11 +59,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(Norm
   float v[NV][8], wv[NV][8];
   float sq = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) load8(v[i], x + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+  for (int i = 0; i < NV; ++i) load8_if(p.once, v[i], x + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
   if (r) {
     float rv[NV][8];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8(rv[i], r + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+    for (int i = 0; i < NV; ++i) load8_if(p.once, rv[i], r + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -243,6 +244,9 @@ static int norm_forward(NormParams p, int dtype, int w_dtype, hipStream_t st) {
   // 16384 x 8192 to 8 bits (s of 268 MB) 174 us, 187 without; 40960 x 2048 ten times in a row, each on the last one's outputs (2 x 168 MB), 118
   // against 124; but 20480 x 1024 (2 x 42 MB), done always, 31.4 against 27.9.
   const long size = dtype == RTP_DT_F32 ? 4 : 2;
+  // Rows of x and res that are read and done with, past the caches too: 8192 x 8192 91 us, 106 without; 2500 x 16384 (78 MB) 57 and 64; but 16384 x 1024
+  // (32 MB) 27 and 23.  (The backward pass gains nothing by either.)
+  p.once = p.rows * p.h * size > (64L << 20);
   p.far = p.rows * p.h * ((p.s ? size : 0) + (OUT8 ? 1 : size)) > RTP_FAR_BYTES;
   return norm_types(dtype, w_dtype, [&](auto t, auto w) {
     return norm_shape(p.h, [&](auto lpr, auto nv) {
@@ -259,7 +263,7 @@ static int norm_forward(NormParams p, int dtype, int w_dtype, hipStream_t st) {
 extern "C" int rtp_rmsnorm_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* y, void* s,
                                    long rows, int h, int dtype, float eps, void* stream) {
   if (rows > 0 && !y) return RTP_ERR_SHAPE;
-  NormParams p{x, res, w, y, s, nullptr, nullptr, x_rs, res_rs, 0, rows, h, false, eps};
+  NormParams p{x, res, w, y, s, nullptr, nullptr, x_rs, res_rs, 0, rows, h, false, false, eps};
   return norm_forward<false>(p, dtype, w_dtype, (hipStream_t)stream);
 }
 
@@ -268,7 +272,7 @@ extern "C" int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res
   if (rows > 0 && (!q || !scale)) return RTP_ERR_SHAPE;
   if (q_rs < ((h + 15) & ~15)) return RTP_ERR_SHAPE;
   if (((size_t)q & 15) || (q_rs & 15)) return RTP_ERR_ALIGN;
-  NormParams p{x, res, w, nullptr, s, (uint8_t*)q, scale, x_rs, res_rs, q_rs, rows, h, false, eps};
+  NormParams p{x, res, w, nullptr, s, (uint8_t*)q, scale, x_rs, res_rs, q_rs, rows, h, false, false, eps};
   return norm_forward<true>(p, dtype, w_dtype, (hipStream_t)stream);
 }
 
