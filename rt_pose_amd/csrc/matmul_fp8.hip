@@ -354,7 +354,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
       for (int i = 0; i < NT; i += 2) {
         const int nc = n0 + wn + i * 16 + g * 8;
         const float v[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
-        if (p.far) store8_far(o + nc, v, p.n - nc);
+        if (p.far && nc + 8 <= p.n) put8(o + nc, v, true);
         else store8(o + nc, v, p.n - nc);
       }
     }

@@ -28,23 +28,39 @@ __device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
     for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.f;
   }
 }
-// as load8, marked to leave the caches first
-template <typename T>
-__device__ __forceinline__ void load8_once(float (&v)[8], const T* p, int n) {
-  typedef T tv8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  if (n >= 8) {
-    const tv8 r = __builtin_nontemporal_load((const tv8*)p);
+// Rows in chunks of eight columns, by what their length n allows: a multiple of 8, any from 8 on, fewer.
+enum RowKind { ROW_WHOLE, ROW_RAGGED, ROW_SHORT };
+template <typename T> using vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+// Columns c .. c + 7, zeros behind the row's end, in two steps: all loads of a row first, then their values.  A ragged row's last chunk is read as the
+// row's last eight columns and moved into place in registers: element by element it is another trip to memory for the whole wave (bf16, 20480 x 1023:
+// norm 47 us, so 31, its gradients 72 and 40; 8192 x 4094 quantised in blocks of 128 x 128: 41 and 21).  `once`: marked to leave the caches first.
+template <RowKind KIND, typename T>
+__device__ __forceinline__ vec8<T> fetch8(const T* row, int c, int n, bool once = false) {
+  vec8<T> r;
+  if constexpr (KIND == ROW_SHORT) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
+    for (int j = 0; j < 8; ++j) r[j] = c + j < n ? row[c + j] : (T)0.f;
   } else {
-    load8(v, p, n);
+    const vec8<T>* p = (const vec8<T>*)(row + (c + 8 > n ? n - 8 : c));
+    r = once ? __builtin_nontemporal_load(p) : *p;
   }
+  return r;
 }
-// load8 or load8_once, by a condition that all lanes share
-template <typename T>
-__device__ __forceinline__ void load8_if(bool once, float (&v)[8], const T* p, int n) {
-  if (once) load8_once(v, p, n);
-  else load8(v, p, n);
+template <RowKind KIND, typename T>
+__device__ __forceinline__ void settle8(float (&v)[8], const vec8<T>& r, int c, int n) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
+  if constexpr (KIND != ROW_SHORT) {
+    const int over = c + 8 > n ? c + 8 - n : 0;
+    if (KIND == ROW_RAGGED && __any(over)) {
+#pragma unroll
+      for (int s = 1; s < 8; s *= 2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = over & s ? (j + s < 8 ? v[j + s] : 0.f) : v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = over > 7 ? 0.f : v[j];
+  }
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
@@ -60,20 +76,26 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
       if (j < n) p[j] = (T)v[j];
   }
 }
-
 // Outputs of more than the last-level cache drive each other out of it before the next pass reads them: they are stored past it.
 #define RTP_FAR_BYTES (256L << 20)
-// as store8, marked to leave the caches first
+// eight values, `far`: marked to leave the caches first
 template <typename T>
-__device__ __forceinline__ void store8_far(T* p, const float (&v)[8], int n) {
-  typedef T tv8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  if (n >= 8) {
-    tv8 r;
+__device__ __forceinline__ void put8(T* p, const float (&v)[8], bool far) {
+  vec8<T> r;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
-    __builtin_nontemporal_store(r, (tv8*)p);
-  } else {
-    store8(p, v, n);
+  for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
+  if (far) __builtin_nontemporal_store(r, (vec8<T>*)p);
+  else *(vec8<T>*)p = r;
+}
+// columns c .. c + 7 of a row of n
+template <RowKind KIND, typename T>
+__device__ __forceinline__ void put_row8(T* row, const float (&v)[8], int c, int n, bool far = false) {
+  if (KIND != ROW_SHORT && c + 8 <= n) {
+    put8(row + c, v, far);
+  } else if constexpr (KIND != ROW_WHOLE) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < n) row[c + j] = (T)v[j];
   }
 }
 

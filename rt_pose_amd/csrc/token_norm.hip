@@ -44,9 +44,9 @@ struct NormParams {
   float eps;
 };
 
-// Bound by HBM: 20480 x 1024 bf16 with the residual 34 us for 168 MB, 4.9 TB/s; 16384 x 8192 to 8 bits 167 us for 944 MB, 5.65 TB/s (a large copy
+// Bound by HBM: 20480 x 1024 bf16 with the residual 32 us for 168 MB, 5.2 TB/s; 16384 x 8192 to 8 bits 167 us for 944 MB, 5.65 TB/s (a large copy
 // moves 4.96).  8 x 4096, a token's rows: 4.3 us, one trip to memory and the launch.
-template <typename T, typename W, int LPR, int NV, bool OUT8>
+template <typename T, typename W, int LPR, int NV, bool OUT8, RowKind KIND>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(NormParams p) {
   constexpr int THREADS = LPR > 256 ? LPR : 256;
   __shared__ float red[THREADS / 64];
@@ -58,25 +58,33 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(Norm
   T* so = p.s ? (T*)p.s + row * p.h : nullptr;
   float v[NV][8], wv[NV][8];
   float sq = 0.f;
+  vec8<T> xr[NV];
+  vec8<W> wr[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) load8_if(p.once, v[i], x + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+  for (int i = 0; i < NV; ++i) xr[i] = fetch8<KIND>(x, (lane + i * LPR) * 8, p.h, p.once);
   if (r) {
-    float rv[NV][8];
+    vec8<T> rr[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load8_if(p.once, rv[i], r + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + rv[i][j]);   // the stream as it is written is what is normed
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) load8(wv[i], (const W*)p.w + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
-  if (so) {
+    for (int i = 0; i < NV; ++i) rr[i] = fetch8<KIND>(r, (lane + i * LPR) * 8, p.h, p.once);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (p.far) store8_far(so + (lane + i * LPR) * 8, v[i], p.h - (lane + i * LPR) * 8);
-      else store8(so + (lane + i * LPR) * 8, v[i], p.h - (lane + i * LPR) * 8);
+      float rv[8];
+      settle8<KIND, T>(v[i], xr[i], (lane + i * LPR) * 8, p.h);
+      settle8<KIND, T>(rv, rr[i], (lane + i * LPR) * 8, p.h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + rv[j]);   // the stream as it is written is what is normed
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) settle8<KIND, T>(v[i], xr[i], (lane + i * LPR) * 8, p.h);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) wr[i] = fetch8<KIND>((const W*)p.w, (lane + i * LPR) * 8, p.h);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) settle8<KIND, W>(wv[i], wr[i], (lane + i * LPR) * 8, p.h);
+  if (so) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put_row8<KIND>(so, v[i], (lane + i * LPR) * 8, p.h, p.far);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -89,8 +97,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(Norm
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rho * wv[i][j];
     if constexpr (!OUT8) {
-      if (p.far) store8_far((T*)p.y + row * p.h + c, v[i], n);
-      else store8((T*)p.y + row * p.h + c, v[i], n);
+      put_row8<KIND>((T*)p.y + row * p.h, v[i], c, p.h, p.far);
     } else {
       // a block of 128 columns = 16 neighbouring lanes; columns behind the row's end are zeros and change nothing
       float a = amax8(v[i]);
@@ -116,7 +123,7 @@ struct NormBwdParams {
 
 // Workgroups walk the rows with a stride; each lane keeps its columns' share of dw in registers over all its rows, a workgroup leaves one
 // partial row, and rmsnorm_dw_kernel adds those in fixed order: no atomics.  20480 x 1024 bf16: 34.5 us for 168 MB, 4.9 TB/s, and 4 for dw.
-template <typename T, typename W, int LPR, int NV>
+template <typename T, typename W, int LPR, int NV, RowKind KIND>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(NormBwdParams p) {
   constexpr int THREADS = LPR > 256 ? LPR : 256, GROUPS = THREADS / LPR;
   __shared__ float red[THREADS / 64];
@@ -125,22 +132,31 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
   float wv[NV][8], dw[NV][8];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load8(wv[i], (const W*)p.w + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+    settle8<KIND, W>(wv[i], fetch8<KIND>((const W*)p.w, (lane + i * LPR) * 8, p.h), (lane + i * LPR) * 8, p.h);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
   }
   for (long row = (long)blockIdx.x * GROUPS + grp; row < p.rows; row += (long)gridDim.x * GROUPS) {
     float s[NV][8], g[NV][8], d[NV][8];      // all of a row's loads at once: one trip to memory for it
     float sq = 0.f, gs = 0.f;
+    vec8<T> sr[NV], gr[NV], dr[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (lane + i * LPR) * 8;
-      load8(s[i], (const T*)p.s + row * p.s_rs + c, p.h - c);
-      load8(g[i], (const T*)p.dy + row * p.dy_rs + c, p.h - c);
+      sr[i] = fetch8<KIND>((const T*)p.s + row * p.s_rs, (lane + i * LPR) * 8, p.h);
+      gr[i] = fetch8<KIND>((const T*)p.dy + row * p.dy_rs, (lane + i * LPR) * 8, p.h);
     }
     if (p.ds) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) load8(d[i], (const T*)p.ds + row * p.ds_rs + (lane + i * LPR) * 8, p.h - (lane + i * LPR) * 8);
+      for (int i = 0; i < NV; ++i) dr[i] = fetch8<KIND>((const T*)p.ds + row * p.ds_rs, (lane + i * LPR) * 8, p.h);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      settle8<KIND, T>(s[i], sr[i], (lane + i * LPR) * 8, p.h);
+      settle8<KIND, T>(g[i], gr[i], (lane + i * LPR) * 8, p.h);
+    }
+    if (p.ds) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) settle8<KIND, T>(d[i], dr[i], (lane + i * LPR) * 8, p.h);
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -164,7 +180,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
         dw[i][j] += g[i][j] * s[i][j] * rho;
         d[i][j] += rho * (g[i][j] * wv[i][j] - s[i][j] * back);
       }
-      store8((T*)p.dx + row * p.h + c, d[i], n);
+      put_row8<KIND>((T*)p.dx + row * p.h, d[i], c, p.h);
     }
   }
   if constexpr (GROUPS > 1) {
@@ -182,7 +198,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (lane + i * LPR) * 8;
-      store8(p.part + (long)blockIdx.x * p.h + c, dw[i], p.h - c);
+      put_row8<KIND>(p.part + (long)blockIdx.x * p.h, dw[i], c, p.h);
     }
   }
 }
@@ -209,18 +225,27 @@ __global__ __launch_bounds__(1024) void rmsnorm_dw_kernel(const float* part, int
 
 // ------------------------------------------------------------------------------------------------ launches
 // lanes per row and chunks per lane by the row's length: 16 lanes up to 128 columns (four rows a wave), a wave up to 2048, a workgroup of
-// 256 up to 8192, of 1024 up to 16384 (its 128 registers a lane end there)
+// 256 up to 8192, of 512 up to 16384, where its registers end (2500 x 16384 bf16: gradients 89 us, with 1024 threads of half as many registers 119)
 #define NORM_MAX_H 16384
 
 template <typename F>
-static int norm_shape(int h, F f) {
+static int norm_lanes(int h, F f) {
   if (h <= 128) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
   if (h <= 512) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
   if (h <= 1024) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
   if (h <= 2048) return f(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
   if (h <= 4096) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
   if (h <= 8192) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-  return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
+}
+
+// f(lanes, chunks, kind of rows)
+template <typename F>
+static int norm_shape(int h, F f) {
+  if (h < 8) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{}, std::integral_constant<RowKind, ROW_SHORT>{});
+  return norm_lanes(h, [&](auto lpr, auto nv) {
+    return h % 8 ? f(lpr, nv, std::integral_constant<RowKind, ROW_RAGGED>{}) : f(lpr, nv, std::integral_constant<RowKind, ROW_WHOLE>{});
+  });
 }
 
 // value type x weight type (fp32 weights beside half values, or the values' own type)
@@ -249,10 +274,10 @@ static int norm_forward(NormParams p, int dtype, int w_dtype, hipStream_t st) {
   p.once = p.rows * p.h * size > (64L << 20);
   p.far = p.rows * p.h * ((p.s ? size : 0) + (OUT8 ? 1 : size)) > RTP_FAR_BYTES;
   return norm_types(dtype, w_dtype, [&](auto t, auto w) {
-    return norm_shape(p.h, [&](auto lpr, auto nv) {
+    return norm_shape(p.h, [&](auto lpr, auto nv, auto kind) {
       constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, THREADS = LPR > 256 ? LPR : 256;
       if (!rtp_launchable(rtp_div_up(p.rows, THREADS / LPR), THREADS)) return RTP_ERR_SHAPE;
-      hipLaunchKernelGGL((rmsnorm_fwd_kernel<decltype(t), decltype(w), LPR, NV, OUT8>), dim3(rtp_div_up(p.rows, THREADS / LPR)), dim3(THREADS), 0,
+      hipLaunchKernelGGL((rmsnorm_fwd_kernel<decltype(t), decltype(w), LPR, NV, OUT8, decltype(kind)::value>), dim3(rtp_div_up(p.rows, THREADS / LPR)), dim3(THREADS), 0,
                          st, p);
       RTP_CHECK_LAUNCH();
       return RTP_OK;
@@ -296,10 +321,10 @@ extern "C" int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int
   NormBwdParams p{s, w, dy, ds, dx, part, s_rs, dy_rs, ds_rs, rows, h, eps};
   const int slots = rtp_rmsnorm_backward_slots(rows, h);
   return norm_types(dtype, w_dtype, [&](auto t, auto wt) {
-    return norm_shape(h, [&](auto lpr, auto nv) {
+    return norm_shape(h, [&](auto lpr, auto nv, auto kind) {
       constexpr int LPR = decltype(lpr)::value, NV = decltype(nv)::value, THREADS = LPR > 256 ? LPR : 256;
       typedef decltype(wt) W;
-      hipLaunchKernelGGL((rmsnorm_bwd_kernel<decltype(t), W, LPR, NV>), dim3(slots), dim3(THREADS), 0, st, p);
+      hipLaunchKernelGGL((rmsnorm_bwd_kernel<decltype(t), W, LPR, NV, decltype(kind)::value>), dim3(slots), dim3(THREADS), 0, st, p);
       RTP_CHECK_LAUNCH();
       hipLaunchKernelGGL((rmsnorm_dw_kernel<W>), dim3(rtp_div_up(h, 16)), dim3(1024), 0, st, part, slots, h, (W*)dw);
       RTP_CHECK_LAUNCH();
@@ -319,16 +344,18 @@ struct QuantParams {
 
 // blocks of 1 x 128, rows in memory order: 16 lanes a block, four rows a lane so that four loads are in flight
 #define QUANT_ROWS 4
-template <typename T>
+template <typename T, RowKind KIND>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
   const unsigned g = blockIdx.x * 16u + (threadIdx.x >> 4);
   const int lane = threadIdx.x & 15;
   const long row0 = (long)(g / (unsigned)p.kb) * QUANT_ROWS;
   const int b = (int)(g % (unsigned)p.kb), c = b * 128 + lane * 8, n = p.cols - c;
   float v[QUANT_ROWS][8];
+  vec8<T> r[QUANT_ROWS];
 #pragma unroll
-  for (int u = 0; u < QUANT_ROWS; ++u)
-    load8(v[u], (const T*)p.x + (row0 + u) * p.x_rs + c, row0 + u < p.rows ? n : 0);
+  for (int u = 0; u < QUANT_ROWS; ++u) r[u] = fetch8<KIND>((const T*)p.x + (row0 + u < p.rows ? row0 + u : p.rows - 1) * p.x_rs, c, p.cols);
+#pragma unroll
+  for (int u = 0; u < QUANT_ROWS; ++u) settle8<KIND, T>(v[u], r[u], c, p.cols);
 #pragma unroll
   for (int u = 0; u < QUANT_ROWS; ++u) {
     float a = amax8(v[u]);
@@ -344,16 +371,19 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
 
 // blocks of 128 x 128, rows in memory order: one workgroup a block, held in registers between its maximum and the output.  8192 x 4096 bf16: 18 us for
 // 101 MB, 5.6 TB/s.
-template <typename T>
+template <typename T, RowKind KIND>
 __global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
   __shared__ float red[4];
   const int lane = threadIdx.x & 15, b = blockIdx.x % (unsigned)p.kb;
   const long row0 = (long)(blockIdx.x / (unsigned)p.kb) * 128 + (threadIdx.x >> 4);
   const int c = b * 128 + lane * 8, n = p.cols - c;
   float v[8][8];
+  vec8<T> r[8];
   float a = 0.f;
 #pragma unroll
-  for (int u = 0; u < 8; ++u) load8(v[u], (const T*)p.x + (row0 + u * 16) * p.x_rs + c, row0 + u * 16 < p.rows ? n : 0);
+  for (int u = 0; u < 8; ++u) r[u] = fetch8<KIND>((const T*)p.x + (row0 + u * 16 < p.rows ? row0 + u * 16 : p.rows - 1) * p.x_rs, c, p.cols);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) settle8<KIND, T>(v[u], r[u], c, p.cols);     // a row behind the last one repeats it: the block's maximum stays
 #pragma unroll
   for (int u = 0; u < 8; ++u) a = fmaxf(a, amax8(v[u]));
 #pragma unroll
@@ -472,9 +502,11 @@ extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, l
     else if (turned)
       hipLaunchKernelGGL((quant_turned_kernel<T, false>), dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
     else if (square)
-      hipLaunchKernelGGL((quant_square_kernel<T>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((cols < 8 ? quant_square_kernel<T, ROW_SHORT> : cols % 8 ? quant_square_kernel<T, ROW_RAGGED> : quant_square_kernel<T, ROW_WHOLE>),
+                         dim3((unsigned)tiles), dim3(256), 0, st, p);
     else
-      hipLaunchKernelGGL((quant_rows_kernel<T>), dim3(rtp_div_up(groups, 16)), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((cols < 8 ? quant_rows_kernel<T, ROW_SHORT> : cols % 8 ? quant_rows_kernel<T, ROW_RAGGED> : quant_rows_kernel<T, ROW_WHOLE>),
+                         dim3(rtp_div_up(groups, 16)), dim3(256), 0, st, p);
     RTP_CHECK_LAUNCH();
     return RTP_OK;
   };

@@ -279,3 +279,19 @@ def test_the_same_rows_twice_broadcast_rows_and_widths_beyond():
     for n in (2 ** 30 + 1, 2 ** 32 + 8):
         with pytest.raises(ValueError):
             quantize_fp8(wide[:, :1].expand(1, n))
+
+
+@pytest.mark.parametrize("h", [2, 8, 9, 15, 16, 121, 127, 505, 520, 1000, 1023, 1025, 2047, 2056, 4090, 8191, 8200, 12345, 16383])
+def test_every_kind_of_width(h):
+    """Whole, ragged and short rows at each of the kernels' widths, odd strides and an odd start among them."""
+    from rt_pose_amd.fp8 import quantize_fp8
+    for dtype in TYPES:
+        test_forward_backward(6, h, dtype, dtype != torch.float32)
+        test_norm_fp8(5, h, True, dtype)
+    for square in (False, True):
+        test_quantize(130, h, square, False, torch.bfloat16)
+        test_quantize(3, h, square, False, torch.float32)
+        wide = rnd(4, h + 3, seed=h, dtype=torch.float16)
+        block = (128, 128) if square else (1, 128)
+        for a, b in zip(quantize_fp8(wide[:, 1:-2], block), quantize_fp8(wide[:, 1:-2].clone(), block)):
+            assert torch.equal(a.float(), b.float())
