@@ -651,7 +651,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XaParams p, int bk) {
     for (int s = lane / L; s < n; s += 64 / L) {
       const float lse = p.part_lse[at + s * step], w = exp2f(lse - mx);
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (c < p.d) load8(v, p.part + (at + s * step) * p.d + c, 8);
+      if (c < p.d) load8(v, p.part + (at + s * step) * p.d + c);
       sum += w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) acc[j] += lse == -INFINITY ? 0.f : v[j] * w;      // a run without keys has left nothing
@@ -698,9 +698,9 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XaParams p) {
     const int bh = (int)(row / p.rows), r = (int)(row % p.rows), s = r / p.grp, g = r % p.grp, b = bh / p.hkv, hq = (bh % p.hkv) * p.grp + g;
     const long oo = (((long)b * p.sq + s) * p.hq + hq) * p.d + c;
     float hi[8], lo[8], d[8];
-    load8(hi, (const T*)p.o + oo, 8);
-    load8(lo, (const T*)p.o_lo + oo, 8);
-    load8(d, (const T*)p.d_o + (long)b * p.o_bs + (long)s * p.o_ss + (long)hq * p.o_hs + c, 8);
+    load8(hi, (const T*)p.o + oo);
+    load8(lo, (const T*)p.o_lo + oo);
+    load8(d, (const T*)p.d_o + (long)b * p.o_bs + (long)s * p.o_ss + (long)hq * p.o_hs + c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) t += (hi[j] + lo[j]) * d[j];
   }
@@ -849,7 +849,7 @@ __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
 #pragma unroll 4
   for (int s = lane / L; s < p.nsplit; s += 64 / L) {
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < p.d) load8(v, p.part + (s * rows + row) * p.d + c, 8);
+    if (c < p.d) load8(v, p.part + (s * rows + row) * p.d + c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] += v[j];
   }
@@ -1142,7 +1142,7 @@ __global__ __launch_bounds__(256) void xattn_dkv_join_kernel(XaParams p, long al
   if (i >= 2 * all) return;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8];
   for (int s = 0; s < p.nsplit; ++s) {
-    load8(v, p.part + 2L * s * all + i, 8);
+    load8(v, p.part + 2L * s * all + i);
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] += v[j];
   }

@@ -13,24 +13,17 @@ static inline bool rtp_launchable(long blocks, long threads) { return blocks * t
 
 #define RTP_FP8_AMAX_FLOOR 0x1p-100f   // keeps 448 / amax finite; a block of zeros gets the floor's scale
 
-// Eight consecutive values at any address (rows of odd length or odd stride start anywhere): one unaligned 16- or 32-byte access,
-// which global memory takes at every alignment of the element; element by element only where the row ends inside the chunk.
+// Eight consecutive values at any address (rows of odd length or odd stride start anywhere): one unaligned 16- or 32-byte access, which global memory
+// takes at every alignment of the element.
+template <typename T> using vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 template <typename T>
-__device__ __forceinline__ void load8(float (&v)[8], const T* p, int n) {
-  typedef T tv8 __attribute__((ext_vector_type(8)));
-  if (n >= 8) {
-    tv8 r;
-    __builtin_memcpy(&r, p, sizeof(r));
+__device__ __forceinline__ void load8(float (&v)[8], const T* p) {
+  const vec8<T> r = *(const vec8<T>*)p;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? (float)p[j] : 0.f;
-  }
+  for (int j = 0; j < 8; ++j) v[j] = (float)r[j];
 }
 // Rows in chunks of eight columns, by what their length n allows: a multiple of 8, any from 8 on, fewer.
 enum RowKind { ROW_WHOLE, ROW_RAGGED, ROW_SHORT };
-template <typename T> using vec8 = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 // Columns c .. c + 7, zeros behind the row's end, in two steps: all loads of a row first, then their values.  A ragged row's last chunk is read as the
 // row's last eight columns and moved into place in registers: element by element it is another trip to memory for the whole wave (bf16, 20480 x 1023:
 // norm 47 us, so 31, its gradients 72 and 40; 8192 x 4094 quantised in blocks of 128 x 128: 41 and 21).  `once`: marked to leave the caches first.
@@ -62,14 +55,14 @@ __device__ __forceinline__ void settle8(float (&v)[8], const vec8<T>& r, int c, 
     for (int j = 0; j < 8; ++j) v[j] = over > 7 ? 0.f : v[j];
   }
 }
+// eight values, or the first n of them
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], int n) {
-  typedef T tv8 __attribute__((ext_vector_type(8)));
   if (n >= 8) {
-    tv8 r;
+    vec8<T> r;
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = (T)v[j];
-    __builtin_memcpy(p, &r, sizeof(r));
+    *(vec8<T>*)p = r;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)

@@ -369,8 +369,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(QuantParams p) {
   }
 }
 
-// blocks of 128 x 128, rows in memory order: one workgroup a block, held in registers between its maximum and the output.  8192 x 4096 bf16: 18 us for
-// 101 MB, 5.6 TB/s.
+// blocks of 128 x 128, rows in memory order: one workgroup a block, held in registers between its maximum and the output.  8192 x 4096 bf16: 17 us for
+// 101 MB, 6.0 TB/s.
 template <typename T, RowKind KIND>
 __global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
   __shared__ float red[4];
@@ -400,9 +400,9 @@ __global__ __launch_bounds__(256) void quant_square_kernel(QuantParams p) {
 
 // Either block, x given by columns (a transpose's view: x[r][c] at c * x_rs + r).  A tile of 128 rows x 128 columns goes through LDS twice: read
 // along the columns' memory order, taken by each thread as 32 columns of two neighbouring rows (one LDS word a column for 16-bit types, held in
-// registers from the maximum to the output), and the bytes once more so that they leave as whole rows.  1000 x 20481 bf16: 17 us for 62 MB, 3.7 TB/s:
-// rows of an odd length start inside a line, which two tiles then read.
-template <typename T, bool SQUARE>
+// registers from the maximum to the output), and the bytes once more so that they leave as whole rows.  1000 x 20481 bf16: 14 us for 62 MB, 4.4 TB/s
+// (a chunk's loads one after the other: 17).
+template <typename T, bool SQUARE, RowKind KIND>
 __global__ __launch_bounds__(256) void quant_turned_kernel(QuantParams p) {
   constexpr int PITCH = 128 + 16 / sizeof(T), QPITCH = 144;     // keep 16-byte accesses aligned and rows apart
   typedef T tv2 __attribute__((ext_vector_type(2)));
@@ -415,16 +415,22 @@ __global__ __launch_bounds__(256) void quant_turned_kernel(QuantParams p) {
   if (b >= p.kb) return;
   {
     const int ch = (threadIdx.x & 15) * 8;
-    const long left = p.rows - row0 - ch;
-    const int n = left < 0 ? 0 : left > 8 ? 8 : (int)left;
-    float v[8][8];
+    vec8<T> r[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const int c = (threadIdx.x >> 4) + u * 16;
-      load8(v[u], (const T*)p.x + (long)(b * 128 + c) * p.x_rs + row0 + ch, b * 128 + c < p.cols ? n : 0);
+      const int c = b * 128 + (threadIdx.x >> 4) + u * 16;
+      r[u] = fetch8<KIND>((const T*)p.x + (long)(c < p.cols ? c : p.cols - 1) * p.x_rs, (int)row0 + ch, (int)p.rows);
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) store8(tile + ((threadIdx.x >> 4) + u * 16) * PITCH + ch, v[u], 8);
+    for (int u = 0; u < 8; ++u) {
+      float v[8];
+      settle8<KIND, T>(v, r[u], (int)row0 + ch, (int)p.rows);
+      if (b * 128 + (threadIdx.x >> 4) + u * 16 >= p.cols) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      }
+      store8(tile + ((threadIdx.x >> 4) + u * 16) * PITCH + ch, v, 8);
+    }
   }
   __syncthreads();
   float v[2][32], a[2] = {0.f, 0.f};
@@ -498,9 +504,15 @@ extern "C" int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, l
   auto go = [&](auto t) {
     typedef decltype(t) T;
     if (turned && square)
-      hipLaunchKernelGGL((quant_turned_kernel<T, true>), dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((rows < 8   ? quant_turned_kernel<T, true, ROW_SHORT>
+                          : rows % 8 ? quant_turned_kernel<T, true, ROW_RAGGED>
+                                     : quant_turned_kernel<T, true, ROW_WHOLE>),
+                         dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
     else if (turned)
-      hipLaunchKernelGGL((quant_turned_kernel<T, false>), dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
+      hipLaunchKernelGGL((rows < 8   ? quant_turned_kernel<T, false, ROW_SHORT>
+                          : rows % 8 ? quant_turned_kernel<T, false, ROW_RAGGED>
+                                     : quant_turned_kernel<T, false, ROW_WHOLE>),
+                         dim3((unsigned)turned_tiles), dim3(256), 0, st, p);
     else if (square)
       hipLaunchKernelGGL((cols < 8 ? quant_square_kernel<T, ROW_SHORT> : cols % 8 ? quant_square_kernel<T, ROW_RAGGED> : quant_square_kernel<T, ROW_WHOLE>),
                          dim3((unsigned)tiles), dim3(256), 0, st, p);
