@@ -201,6 +201,7 @@ __global__ __launch_bounds__(64 * MM8_FEW_WAVES) void mm8_few_kernel(Mm8Params p
 // of group g = lane / 16 read chunks g and g + 4.  A 16-byte LDS read goes by the lanes {0-3, 12-15, 20-27}, {4-11, 16-19, 28-31} and the same of
 // the upper half: each of these sets then touches 16 different slots of the 256-byte bank row (chunks 2 g and 2 g + 1 instead: every read
 // two-way, half of the LDS cycles, 637 -> 621 us at 8192^3).
+template <typename O, int BN> struct Mm8Out { static constexpr int PITCH = BN * sizeof(O) + 16; };      // of a row of results in LDS
 template <typename O, int BM, int BN, int WM, int WN, bool SQUARE>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel(Mm8Params p) {
   constexpr int WAVES = (BM / WM) * (BN / WN), THREADS = WAVES * 64, MT = WM / 16, NT = WN / 16;
@@ -345,17 +346,37 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
   if (p.k & 127) compute(kb, kb & 1, true, false);
   else compute(kb, kb & 1, false, false);
 
+  // The results leave as whole rows of the tile, by way of LDS: 128 bytes or more of a row together, not 64 or 128 a lane group (163840 x 255 x 384:
+  // 36 us, straight from the registers 53; x 256: 30.7 and 31.5, fp32 48 and 53; 8192^3 493 and 505).
+  __syncthreads();
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int mr = m0 + wm + j * 16 + col;
-    if (mr < p.m) {
-      O* o = (O*)p.out + mr * p.ldo;
+  for (int j = 0; j < MT; ++j)
 #pragma unroll
-      for (int i = 0; i < NT; i += 2) {
-        const int nc = n0 + wn + i * 16 + g * 8;
-        const float v[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
-        if (p.far && nc + 8 <= p.n) put8(o + nc, v, true);
-        else store8(o + nc, v, p.n - nc);
+    for (int i = 0; i < NT; i += 2) {
+      const float v[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
+      typedef O ov8 __attribute__((ext_vector_type(8), aligned(16)));
+      ov8 r;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = (O)v[e];
+      *(ov8*)(lds + (wm + j * 16 + col) * Mm8Out<O, BN>::PITCH + (wn + i * 16 + g * 8) * sizeof(O)) = r;
+    }
+  __syncthreads();
+  constexpr int E = 16 / sizeof(O), CH = BN / E;
+#pragma unroll
+  for (int u = 0; u < BM * CH / THREADS; ++u) {
+    const int at = u * THREADS + threadIdx.x, row = at / CH, c = at % CH * E;
+    if (m0 + row < p.m) {
+      typedef O lds16 __attribute__((ext_vector_type(E), aligned(16)));
+      typedef O out16 __attribute__((ext_vector_type(E), aligned(sizeof(O))));
+      const out16 r = *(const lds16*)(lds + row * Mm8Out<O, BN>::PITCH + c * sizeof(O));
+      O* o = (O*)p.out + (m0 + row) * p.ldo + n0 + c;
+      if (n0 + c + E <= p.n) {
+        if (p.far) __builtin_nontemporal_store(r, (out16*)o);
+        else *(out16*)o = r;
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (n0 + c + e < p.n) o[e] = r[e];
       }
     }
   }
@@ -389,7 +410,7 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     p.tiles_m = rtp_div_up(p.m, bm);
     p.tiles_n = rtp_div_up(p.n, bn);
     if (!rtp_launchable((long)p.tiles_m * p.tiles_n, threads)) return RTP_ERR_SHAPE;
-    const int bytes = 2 * ((bm + bn) * 128 + (bm + (SQUARE ? 64 : bn)) * 4);
+    const int ring = 2 * ((bm + bn) * 128 + (bm + (SQUARE ? 64 : bn)) * 4), out = bm * (bn * (int)sizeof(O) + 16), bytes = ring > out ? ring : out;
     if (rtp_once_per_device(once) && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
       return RTP_ERR_LAUNCH;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((long)p.tiles_m * p.tiles_n)), dim3(threads), bytes, st, p);
@@ -397,7 +418,7 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     return RTP_OK;
   };
   static bool once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES], once64[RTP_MAX_DEVICES];
-  // 256 x 256 halves what is staged per product and wins where the sum is long and its tiles fill whole rounds of the 256 CUs (8192^3: 505 us
+  // 256 x 256 halves what is staged per product and wins where the sum is long and its tiles fill whole rounds of the 256 CUs (8192^3: 493 us
   // against 580, 4096^3: 72 against 77); 128 x 128, two workgroups to a CU, where one's start and end hide behind the other's sum
   // (163840 x 256 x 384: 40 us against 57, x 1024: 71 against 87).  The exact road needs the registers of the small tile.
   if constexpr (sizeof(O) == 2) {

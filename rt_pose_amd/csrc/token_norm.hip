@@ -44,7 +44,7 @@ struct NormParams {
   float eps;
 };
 
-// Bound by HBM: 20480 x 1024 bf16 with the residual 32 us for 168 MB, 5.2 TB/s; 16384 x 8192 to 8 bits 167 us for 944 MB, 5.65 TB/s (a large copy
+// Bound by HBM: 20480 x 1024 bf16 with the residual 32 us for 168 MB, 5.2 TB/s; 16384 x 8192 to 8 bits 163 us for 944 MB, 5.8 TB/s (a large copy
 // moves 4.96).  8 x 4096, a token's rows: 4.3 us, one trip to memory and the launch.
 template <typename T, typename W, int LPR, int NV, bool OUT8, RowKind KIND>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(NormParams p) {
