@@ -225,7 +225,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_dw_kernel(const float* part, int
 
 // ------------------------------------------------------------------------------------------------ launches
 // lanes per row and chunks per lane by the row's length: 16 lanes up to 128 columns (four rows a wave), a wave up to 2048, a workgroup of
-// 256 up to 8192, of 512 up to 16384, where its registers end (2500 x 16384 bf16: gradients 89 us, with 1024 threads of half as many registers 119)
+// 256 up to 8192, of 512 up to 16384, where its registers end (2500 x 16384 bf16: gradients 80 us, with 1024 threads of half as many registers 119)
 #define NORM_MAX_H 16384
 
 template <typename F>
@@ -301,13 +301,14 @@ extern "C" int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res
   return norm_forward<true>(p, dtype, w_dtype, (hipStream_t)stream);
 }
 
-// partial rows of dw: four workgroups per CU walk the rows where a wave takes one (20480 x 1024: 34.5 us, with two 39.4), two where a workgroup does
-// (their partial rows are longer: 2048 x 8192 37.4 us, with four 46.2), fewer where there are fewer rows
+// partial rows of dw: four workgroups per CU walk the rows where a wave takes one (20480 x 1024: 34.5 us, with two 39.4), two where a workgroup of 256
+// does (their partial rows are longer: 2048 x 8192 34 us, with four 45, with one 38), one of 512 (as many fit: 2500 x 16384 80 us, with two 88), fewer
+// where there are fewer rows
 extern "C" int rtp_rmsnorm_backward_slots(long rows, int h) {
   if (rows < 1 || h < 1 || h > NORM_MAX_H) return 0;
   const int groups = h <= 128 ? 16 : h <= 2048 ? 4 : 1;
   const long need = (rows + groups - 1) / groups;
-  const long most = h <= 2048 ? 1024 : 512;
+  const long most = h <= 2048 ? 1024 : h <= 8192 ? 512 : 256;
   return (int)(need < most ? need : most);
 }
 
