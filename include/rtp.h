@@ -558,7 +558,7 @@ int rtp_modulated_deform_conv_backward(const float* input, const float* weight, 
 /* "8 bits" is OCP e4m3 (largest value 448), held in rows of at least the length rounded up to 16 bytes, 16-byte aligned.  Row strides
  * (`*_rs`) are in elements; rows of the other types need no alignment.  An operand is q * scale with one fp32 scale for each 128 columns
  * of a row (scale[rows][ceil(cols / 128)]) or for each 128 x 128 block ([ceil(rows / 128)][ceil(cols / 128)]).  What a launch cannot count
- * (rows of up to 2^28 for the narrowest norm) is refused with RTP_ERR_SHAPE.
+ * (rows of up to 2^28 for the narrowest norm) is refused with RTP_ERR_SHAPE.  Outputs overlap no input.
  *
  * Root-mean-square norm (csrc/token_norm.hip): s = round(x + res), y = s / sqrt(mean(s^2) + eps) * w.  res may be NULL (s = x); s may be
  * NULL when res is.  w_dtype: the values' type or RTP_DT_F32.  h <= 16384.  s, y, dx: contiguous rows of h.
