@@ -1,6 +1,7 @@
 """Marshalling shared by the token operators (rmsnorm.py, fp8.py, attention.py).  Small calls are bound by the host: one native call, no
 context manager and no stream object where the tensor's device is already the current one."""
 import torch
+from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -27,6 +28,16 @@ def call(name, t, *args):
             rc = getattr(_lib.load(), name)(*args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc, name)
+
+
+class TokenFunction(Function):
+    """What every token operator's call goes through, where nothing asks for a gradient too: only a Function's call is seen by forward mode, whose
+    tangents would be dropped without a word, and by a trace, which would hold the output's allocation and not the operator.  Arguments are checked and
+    laid out inside `forward`: a trace repeats that, and nothing else, with the tensors of its later calls."""
+
+    @staticmethod
+    def jvp(ctx, *tangents):
+        raise NotImplementedError("rt_pose_amd: the token operators have no forward-mode derivatives")
 
 
 def once(backward):

@@ -5,17 +5,17 @@
 q: [b, sq, hq, d]; k, v: [b, sk, hkv, d] with hq a multiple of hkv (head h reads k and v of head h // (hq // hkv)).  Of batch entry i the keys j
 with j < key_lens[i] and key_mask[i, j] count.  Keys that do not count -- an encoder's padding -- are never multiplied, whatever they hold (NaN
 too), and get zero gradients; a row without keys gives zeros, and so does one whose every score is minus infinity.  bf16 or fp16, d a multiple of 8 up to 128; any strides (a tensor whose rows
-are not 16-byte aligned is copied).  Sums and softmax are fp32; the result does not depend on scheduling.  Differentiable in q, k and v.
+are not 16-byte aligned is copied).  Sums and softmax are fp32; the result does not depend on scheduling.  Differentiable in q, k and v
+(backward; a forward-mode tangent is refused with NotImplementedError).  A trace holds the operator as one node, which checks its arguments at every call.
 With few queries (single tokens while serving, key-point queries) the keys are split over the GPU and joined.
 Errors as in rt_pose_amd.rmsnorm.
 """
 import ctypes as C
 
 import torch
-from torch.autograd import Function
 
 from . import _lib
-from ._tokens import DTYPES, call, like, once, p, same_device
+from ._tokens import DTYPES, TokenFunction, call, like, once, p, same_device
 
 
 def _check(q, k, v, key_lens, key_mask, scale):
@@ -84,10 +84,19 @@ def _forward(a, q, o_lo=None, lse=None):
     return o
 
 
-class CrossAttentionFunction(Function):
+class CrossAttentionFunction(TokenFunction):
     @staticmethod
-    def forward(ctx, q, k, v, key_lens, key_mask, scale):
+    def forward(ctx, q, k, v, key_lens, key_mask, scale, keep):
+        """keep: whether a backward pass may follow, if an input asks for its gradient."""
+        scale = float(q.shape[-1]) ** -0.5 if scale is None and q.dim() == 4 and q.shape[-1] else 1.0 if scale is None else float(scale)
+        _check(q, k, v, key_lens, key_mask, scale)
+        q, k, v = _aligned(q, q.shape[2] // k.shape[2]), _aligned(k), _aligned(v)
+        if key_lens is not None:
+            key_lens = (key_lens if key_lens.dtype == torch.int32 else key_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
         a = _operands(q, k, v, key_lens, key_mask, scale)
+        need = ctx.needs_input_grad
+        if not (keep and (need[0] or need[1] or need[2])):
+            return _forward(a, q)
         n = q.shape[:3].numel()
         if key_mask is not None:                    # room for its bits behind
             n = -(-n // 64) * 64 + q.shape[0] * 4 * -(-k.shape[1] // 128)
@@ -105,7 +114,7 @@ class CrossAttentionFunction(Function):
         dq = like(q) if need_q else None
         dk, dv = (like(k), like(v)) if need_k or need_v else (None, None)
         if q.numel() == 0 or k.numel() == 0:
-            return tuple(None if t is None else t.zero_() for t in (dq, dk, dv)) + (None, None, None)
+            return tuple(None if t is None else t.zero_() for t in (dq, dk, dv)) + (None,) * 4
         a, do = ctx.operands, _aligned(do, q.shape[2] // k.shape[2])
         if a.q != q.data_ptr() or a.k != k.data_ptr() or a.v != v.data_ptr() or a.key_lens != p(key_lens) or a.key_mask != p(key_mask) or ctx.layout != (
                 q.stride(), k.stride(), v.stride()):
@@ -113,16 +122,9 @@ class CrossAttentionFunction(Function):
             a = _operands(q, k, v, key_lens, key_mask, ctx.scale)
         ws, n = _workspace(a, 1, q)
         call("rtp_xattn_backward", q, C.byref(a), p(o), p(o_lo), p(lse), p(do), *_strides(do), p(dq), p(dk), p(dv), p(ws), n)
-        return dq, dk, dv, None, None, None
+        return dq, dk, dv, None, None, None, None
 
 
 def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     """scale: 1 / sqrt(d) by default.  key_lens: [b] int32 or int64 (taken between 0 and sk); key_mask: [b, sk], True where a key counts."""
-    scale = q.shape[-1] ** -0.5 if scale is None and q.dim() == 4 and q.shape[-1] else 1.0 if scale is None else float(scale)
-    _check(q, k, v, key_lens, key_mask, scale)
-    q, k, v = _aligned(q, q.shape[2] // k.shape[2]), _aligned(k), _aligned(v)
-    if key_lens is not None:
-        key_lens = (key_lens if key_lens.dtype == torch.int32 else key_lens.clamp(0, k.shape[1]).to(torch.int32)).contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return CrossAttentionFunction.apply(q, k, v, key_lens, key_mask, scale)
-    return _forward(_operands(q, k, v, key_lens, key_mask, scale), q)
+    return CrossAttentionFunction.apply(q, k, v, key_lens, key_mask, scale, torch.is_grad_enabled() or torch.jit.is_tracing())
