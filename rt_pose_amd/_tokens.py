@@ -40,6 +40,13 @@ class TokenFunction(Function):
         raise NotImplementedError("rt_pose_amd: the token operators have no forward-mode derivatives")
 
 
+def without_gradient(ctx, *outputs):
+    """A Function's outputs that carry no gradient, whatever the inputs ask for."""
+    if True in ctx.needs_input_grad:
+        ctx.mark_non_differentiable(*outputs)
+    return outputs
+
+
 def once(backward):
     """A Function's backward that cannot be differentiated again (autograd says so if one tries).  The guard is put on only where a graph of the
     backward pass is asked for: a backward pass runs in a thread of its own, where every line of Python costs twice."""

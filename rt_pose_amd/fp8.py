@@ -7,34 +7,41 @@
 An operand stands for q * scale; q is float8_e4m3fn, scale fp32 of shape [rows, ceil(cols / 128)] or [ceil(rows / 128), ceil(cols / 128)].
 The three products of a linear layer y = x w.T are matmul_fp8 of operands quantised along what is summed over:
     y  = matmul(q(x), q(w));    dx = matmul(q(dy), q(w.T));    dw = matmul(q(dy.T), q(x.T))      (quantize_fp8 takes transposed views as they are)
-Neither function is differentiable.  Errors as in rt_pose_amd.rmsnorm.
+Neither function is differentiable: outputs carry no gradient, a forward-mode tangent is refused with NotImplementedError.  A trace holds each call as
+one node, which checks its arguments every time.  Errors as in rt_pose_amd.rmsnorm.
 """
 import torch
 
-from ._tokens import DTYPES, FP8, call, fp8_rows, p, rows_of, same_device
+from ._tokens import DTYPES, FP8, TokenFunction, call, fp8_rows, p, rows_of, same_device, without_gradient
+
+
+class QuantizeFp8Function(TokenFunction):
+    @staticmethod
+    def forward(ctx, x, block):
+        same_device(x)
+        if x.dtype not in DTYPES:
+            raise NotImplementedError("quantize_fp8: fp32, fp16 or bf16 only (got %s)" % x.dtype)
+        if tuple(block) not in ((1, 128), (128, 128)):
+            raise NotImplementedError("quantize_fp8: blocks of (1, 128) or (128, 128) (got %s)" % (block,))
+        square = tuple(block) == (128, 128)
+        if x.dim() < 1 or x.shape[-1] < 1 or (square and x.dim() != 2):
+            raise ValueError("quantize_fp8: [..., cols] expected, [rows, cols] for blocks of 128 x 128 (got %s)" % (tuple(x.shape),))
+        if x.shape[-1] > 1 << 30:
+            raise ValueError("quantize_fp8: rows of up to 2^30 columns (got %d)" % x.shape[-1])
+        turned = x.dim() == 2 and x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1
+        x2 = x if turned else rows_of(x)
+        rows, cols = x2.shape
+        q, scale = fp8_rows(x.shape, x.device, -(-rows // 128) if square else None)
+        call("rtp_quantize_fp8", x, p(x2), x2.stride(1) if turned else x2.stride(0), int(turned), p(q), -(-cols // 16) * 16, p(scale), rows, cols,
+             int(square), DTYPES[x.dtype])
+        return without_gradient(ctx, q, scale)
 
 
 def quantize_fp8(x, block=(1, 128)):
     """x: [..., cols] of fp32, fp16 or bf16 (block (1, 128)), or [rows, cols] (block (128, 128)) -> q, scale.  Per block a = max(largest
     magnitude, 2^-100): q = e4m3(x * (448 / a)) rounded to nearest even, scale = a / 448.  NaN stay NaN and do not move the scale; a block
     that holds an infinity reads back as NaN.  A 2-D x whose columns are contiguous (x.t() of a row-major tensor) is read in place."""
-    same_device(x)
-    if x.dtype not in DTYPES:
-        raise NotImplementedError("quantize_fp8: fp32, fp16 or bf16 only (got %s)" % x.dtype)
-    if tuple(block) not in ((1, 128), (128, 128)):
-        raise NotImplementedError("quantize_fp8: blocks of (1, 128) or (128, 128) (got %s)" % (block,))
-    square = tuple(block) == (128, 128)
-    if x.dim() < 1 or x.shape[-1] < 1 or (square and x.dim() != 2):
-        raise ValueError("quantize_fp8: [..., cols] expected, [rows, cols] for blocks of 128 x 128 (got %s)" % (tuple(x.shape),))
-    if x.shape[-1] > 1 << 30:
-        raise ValueError("quantize_fp8: rows of up to 2^30 columns (got %d)" % x.shape[-1])
-    turned = x.dim() == 2 and x.stride(0) == 1 and x.stride(1) != 1 and x.shape[0] > 1
-    x2 = x if turned else rows_of(x)
-    rows, cols = x2.shape
-    q, scale = fp8_rows(x.shape, x.device, -(-rows // 128) if square else None)
-    call("rtp_quantize_fp8", x, p(x2), x2.stride(1) if turned else x2.stride(0), int(turned), p(q), -(-cols // 16) * 16, p(scale), rows, cols,
-         int(square), DTYPES[x.dtype])
-    return q, scale
+    return QuantizeFp8Function.apply(x, block)
 
 
 def _operand(q, what):
@@ -49,36 +56,42 @@ def _operand(q, what):
     if (step == 1 or cols == 1) and ld % 16 == 0 and wide <= ld <= 1 << 22 and q.data_ptr() % 16 == 0 and (
             wide == cols or q.storage_offset() + (rows - 1) * ld + wide <= q.untyped_storage().nbytes()):
         return q, ld
-    own = torch.empty(rows, wide, dtype=torch.uint8, device=q.device)
-    own[:, :cols].copy_((q if step == 1 or cols == 1 else q.contiguous()).view(torch.uint8))
+    own = torch.empty(rows, wide, dtype=FP8, device=q.device)
+    own[:, :cols].copy_(q)          # between one type: bytes
     return own, wide
+
+
+class MatmulFp8Function(TokenFunction):
+    @staticmethod
+    def forward(ctx, a, a_scale, b, b_scale, out_dtype):
+        same_device(a, a_scale, b, b_scale)
+        if out_dtype not in DTYPES:
+            raise NotImplementedError("matmul_fp8: out_dtype bf16, fp16 or fp32 (got %s)" % out_dtype)
+        if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
+            raise NotImplementedError("matmul_fp8: fp32 scales (got %s and %s)" % (a_scale.dtype, b_scale.dtype))
+        lead = a.shape[:-1]
+        if len(lead) < 1 or b.dim() != 2 or a.shape[-1] != b.shape[-1] or b.shape[-1] < 1:
+            raise ValueError("matmul_fp8: [..., m, k] and [n, k] expected (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
+        k, n = b.shape[1], b.shape[0]
+        kb, nb = -(-k // 128), -(-n // 128)
+        if k > 1 << 22 or max(n, lead.numel()) > 1 << 30:
+            raise ValueError("matmul_fp8: up to 2^22 columns and 2^30 rows (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
+        if a_scale.shape != (*lead, kb):
+            raise ValueError("matmul_fp8: a_scale of shape %s expected (got %s)" % ((*lead, kb), tuple(a_scale.shape)))
+        if b_scale.shape not in ((nb, kb), (n, kb)):
+            raise ValueError("matmul_fp8: b_scale of shape %s or %s expected (got %s)" % ((nb, kb), (n, kb), tuple(b_scale.shape)))
+        out = torch.empty((*lead, n), dtype=out_dtype, device=a.device)
+        if out.numel() == 0:
+            return without_gradient(ctx, out)[0]
+        a2, lda = _operand(a if len(lead) == 1 else a.reshape(-1, k), "a")
+        b2, ldb = _operand(b, "b")
+        sa, sb = a_scale.contiguous(), b_scale.contiguous()
+        call("rtp_matmul_fp8", a, p(a2), lda, p(sa), p(b2), ldb, p(sb), int(b_scale.shape[0] == nb), p(out), a2.shape[0], n, k, DTYPES[out_dtype])
+        return without_gradient(ctx, out)[0]
 
 
 def matmul_fp8(a, a_scale, b, b_scale, out_dtype=torch.bfloat16):
     """a: [..., m, k] and b: [n, k] in float8_e4m3fn -> [..., m, n]: the sum over k of (a * a_scale) * (b * b_scale) in fp32, rounded once to
     out_dtype (bf16, fp16 or fp32).  a_scale: [..., m, ceil(k / 128)]; b_scale: [ceil(n / 128), ceil(k / 128)] or [n, ceil(k / 128)]; both fp32.
     (For n = 1 the two say the same.)"""
-    same_device(a, a_scale, b, b_scale)
-    if out_dtype not in DTYPES:
-        raise NotImplementedError("matmul_fp8: out_dtype bf16, fp16 or fp32 (got %s)" % out_dtype)
-    if a_scale.dtype != torch.float32 or b_scale.dtype != torch.float32:
-        raise NotImplementedError("matmul_fp8: fp32 scales (got %s and %s)" % (a_scale.dtype, b_scale.dtype))
-    lead = a.shape[:-1]
-    if len(lead) < 1 or b.dim() != 2 or a.shape[-1] != b.shape[-1] or b.shape[-1] < 1:
-        raise ValueError("matmul_fp8: [..., m, k] and [n, k] expected (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
-    k, n = b.shape[1], b.shape[0]
-    kb, nb = -(-k // 128), -(-n // 128)
-    if k > 1 << 22 or max(n, lead.numel()) > 1 << 30:
-        raise ValueError("matmul_fp8: up to 2^22 columns and 2^30 rows (got %s and %s)" % (tuple(a.shape), tuple(b.shape)))
-    if a_scale.shape != (*lead, kb):
-        raise ValueError("matmul_fp8: a_scale of shape %s expected (got %s)" % ((*lead, kb), tuple(a_scale.shape)))
-    if b_scale.shape not in ((nb, kb), (n, kb)):
-        raise ValueError("matmul_fp8: b_scale of shape %s or %s expected (got %s)" % ((nb, kb), (n, kb), tuple(b_scale.shape)))
-    out = torch.empty((*lead, n), dtype=out_dtype, device=a.device)
-    if out.numel() == 0:
-        return out
-    a2, lda = _operand(a if len(lead) == 1 else a.reshape(-1, k), "a")
-    b2, ldb = _operand(b, "b")
-    sa, sb = a_scale.contiguous(), b_scale.contiguous()
-    call("rtp_matmul_fp8", a, p(a2), lda, p(sa), p(b2), ldb, p(sb), int(b_scale.shape[0] == nb), p(out), a2.shape[0], n, k, DTYPES[out_dtype])
-    return out
+    return MatmulFp8Function.apply(a, a_scale, b, b_scale, out_dtype)

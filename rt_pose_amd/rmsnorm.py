@@ -15,7 +15,7 @@ import torch.nn as nn
 from torch.autograd import Function
 
 from . import _lib
-from ._tokens import DTYPES, call, fp8_rows, like, once, p, rows_of, same_device
+from ._tokens import DTYPES, TokenFunction, call, fp8_rows, like, once, p, rows_of, same_device, without_gradient
 
 
 def _check(x, residual, weight):
@@ -94,6 +94,19 @@ class AddRMSNormFunction(Function):
         return dx, dx, dw, None
 
 
+class AddRMSNormFp8Function(TokenFunction):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps):
+        _check(x, residual, weight)
+        x2, w = rows_of(x), weight.contiguous()
+        r2 = rows_of(residual) if residual is not None else None
+        q, scale = fp8_rows(x.shape, x.device)
+        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+        call("rtp_rmsnorm_fp8_forward", x, p(x2), x2.stride(0), p(r2), 0 if r2 is None else r2.stride(0), p(w), DTYPES[w.dtype], p(q),
+             -(-x.shape[-1] // 16) * 16, p(scale), p(s), *x2.shape, DTYPES[x.dtype], float(eps))
+        return without_gradient(ctx, q, scale) if s is None else without_gradient(ctx, q, scale, s)
+
+
 def rms_norm(x, weight, eps=1e-6):
     _check(x, None, weight)
     return RMSNormFunction.apply(x, weight, float(eps))
@@ -108,15 +121,10 @@ def add_rms_norm(x, residual, weight, eps=1e-6):
 
 def add_rms_norm_fp8(x, residual, weight, eps=1e-6):
     """For serving: the normed rows in 8 bits and their scales, as rt_pose_amd.fp8.matmul_fp8 reads them, and the stream.  residual may be
-    None (the stream is x itself).  The value that is quantised is the fp32 one.  Not differentiable: the outputs carry no gradient."""
-    _check(x, residual, weight)
-    x2, w = rows_of(x), weight.contiguous()
-    r2 = rows_of(residual) if residual is not None else None
-    q, scale = fp8_rows(x.shape, x.device)
-    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
-    call("rtp_rmsnorm_fp8_forward", x, p(x2), x2.stride(0), p(r2), 0 if r2 is None else r2.stride(0), p(w), DTYPES[w.dtype], p(q),
-         -(-x.shape[-1] // 16) * 16, p(scale), p(s), *x2.shape, DTYPES[x.dtype], float(eps))
-    return q, scale, x if s is None else s
+    None (the stream is x itself).  The value that is quantised is the fp32 one.  Not differentiable: the outputs carry no gradient, a
+    forward-mode tangent is refused with NotImplementedError."""
+    out = AddRMSNormFp8Function.apply(x, residual, weight, float(eps))
+    return out if residual is not None else (*out, x)
 
 
 class RMSNorm(nn.Module):

@@ -28,3 +28,33 @@ def test_cross_attention():
         leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
         grads = [torch.autograd.grad(g(*leaves, lens[:b], m), leaves, q) for g in (f, call)]
         assert all(torch.equal(a, c) for a, c in zip(*grads))
+
+
+def test_8_bit_serving():
+    from rt_pose_amd.fp8 import matmul_fp8, quantize_fp8
+    from rt_pose_amd.rmsnorm import add_rms_norm_fp8
+    w, g = rnd(90, 200, seed=1), rnd(200, seed=2, dtype=torch.float32)
+    b, sb = quantize_fp8(w, (128, 128))
+
+    def call(x, r):
+        q, scale, s = add_rms_norm_fp8(x, r, g)
+        return matmul_fp8(q, scale, b, sb), s, *quantize_fp8(x)
+    f = traced(call, rnd(3, 200, seed=3), rnd(3, 200, seed=4))
+    for rows in (1, 8, 300):
+        x, r = rnd(rows, 200, seed=rows), rnd(200, rows, seed=rows + 1).t()
+        for u, v in zip(f(x, r), call(x, r)):
+            assert torch.equal(u.float(), v.float())
+
+
+def test_8_bit_operands_that_are_copied():
+    from rt_pose_amd.fp8 import _operand, matmul_fp8
+    every = torch.arange(256, dtype=torch.uint8, device="cuda").repeat(3, 2).view(torch.float8_e4m3fn)     # every byte, NaN too
+    for q in (every[:, 1:300], every[:, ::3], every.t()):
+        own, wide = _operand(q, "a")
+        assert own.data_ptr() != q.data_ptr() and torch.equal(own[:, :q.shape[1]].contiguous().view(torch.uint8), q.contiguous().view(torch.uint8))
+    some = rnd(6, 400, seed=5, dtype=torch.float32).to(torch.float8_e4m3fn)
+    scale = lambda n, k: torch.rand(n, -(-k // 128), generator=torch.Generator().manual_seed(k)).cuda()
+    f = traced(matmul_fp8, some[:2, :40], scale(2, 40), some[:, :40], scale(6, 40))
+    for a, b in ((some[:, 3:333], some[:4, 1:331]), (some[:, ::3][:, :133], some[:, 1::3])):
+        args = a, scale(a.shape[0], a.shape[1]), b, scale(b.shape[0], b.shape[1])
+        assert torch.equal(f(*args), matmul_fp8(*args))

@@ -12,9 +12,12 @@ pytestmark = pytest.mark.filterwarnings("ignore")      # a trace warns of every 
 @pytest.fixture
 def native(monkeypatch):
     """The native calls made; each fills its first output with the byte 0x40."""
-    from rt_pose_amd import _lib, attention
+    from rt_pose_amd import _lib, attention, fp8, rmsnorm
     made = []
-    entries = {"rtp_xattn_forward": lambda a, o, *_: (o, a._obj.b * a._obj.sq * a._obj.hq * a._obj.d * 2)}
+    entries = {"rtp_xattn_forward": lambda a, o, *_: (o, a._obj.b * a._obj.sq * a._obj.hq * a._obj.d * 2),
+               "rtp_quantize_fp8": lambda x, x_rs, turned, q, q_rs, scale, rows, *_: (q, rows * q_rs),
+               "rtp_matmul_fp8": lambda a, lda, sa, b, ldb, sb, square, out, m, n, k, t: (out, m * n * (4 if t == 0 else 2)),
+               "rtp_rmsnorm_fp8_forward": lambda x, x_rs, r, r_rs, w, wt, q, q_rs, scale, s, rows, *_: (q, rows * q_rs)}
 
     def call(name, t, *args):
         made.append(name)
@@ -24,7 +27,7 @@ def native(monkeypatch):
         if n:
             C.memset(at, 0x40, n)
 
-    for module in (attention,):
+    for module in (attention, fp8, rmsnorm):
         monkeypatch.setattr(module, "same_device", lambda *a: None)
         monkeypatch.setattr(module, "call", call)
     return made
@@ -81,3 +84,55 @@ def test_cross_attention_keeps_nothing_where_no_gradient_is_asked_for(native):
         assert not cross_attention(q, k, v).requires_grad
     o = cross_attention(q, k, v)
     assert o.requires_grad and o.grad_fn.saved_tensors[0].data_ptr() == q.data_ptr()
+
+
+def eight(rows, cols, square):
+    return torch.zeros(rows, cols).to(torch.float8_e4m3fn), torch.ones(-(-rows // 128) if square else rows, -(-cols // 128))
+
+
+def test_the_8_bit_entries_refuse_tangents(native):
+    from rt_pose_amd.fp8 import matmul_fp8, quantize_fp8
+    from rt_pose_amd.rmsnorm import add_rms_norm_fp8
+    x, w = torch.ones(3, 40, dtype=torch.bfloat16), torch.ones(40)
+    tangents_are_refused(quantize_fp8, x)
+    tangents_are_refused(add_rms_norm_fp8, x, x, w)
+    tangents_are_refused(lambda x, w: add_rms_norm_fp8(x, None, w), x, w)
+    (a, sa), (b, sb) = eight(3, 40, False), eight(5, 40, True)
+    tangents_are_refused(lambda sa, sb: matmul_fp8(a, sa, b, sb), sa, sb)
+
+
+def test_the_8_bit_entries_carry_no_gradient(native):
+    from rt_pose_amd.fp8 import matmul_fp8, quantize_fp8
+    from rt_pose_amd.rmsnorm import add_rms_norm_fp8
+    x, w = torch.ones(3, 40, requires_grad=True), torch.ones(40, requires_grad=True)
+    (a, sa), (b, sb) = eight(3, 40, False), eight(5, 40, True)
+    outs = [*quantize_fp8(x), *add_rms_norm_fp8(x, x, w), *add_rms_norm_fp8(x, None, w)[:2], matmul_fp8(a, sa.requires_grad_(True), b, sb),
+            matmul_fp8(a[:0], sa[:0], b, sb)]
+    assert not any(t.requires_grad for t in outs) and add_rms_norm_fp8(x, None, w)[2] is x
+    for t in outs:
+        t.copy_(torch.zeros_like(t))                               # the caller's own, to overwrite as well
+
+
+def test_the_8_bit_entries_are_nodes_of_a_trace(native):
+    from rt_pose_amd.fp8 import matmul_fp8, quantize_fp8
+    from rt_pose_amd.rmsnorm import add_rms_norm_fp8
+    x, w = torch.ones(3, 40), torch.ones(40)
+    f = traced(lambda x: quantize_fp8(x, (128, 128)), x)
+    q, scale = f(torch.ones(150, 300))
+    assert native[-1] == "rtp_quantize_fp8" and q.shape == (150, 300) and scale.shape == (2, 3) and filled(q)
+    f = traced(add_rms_norm_fp8, x, x, w)
+    q, scale, s = f(torch.ones(2, 7, 40), torch.ones(2, 7, 40), w)
+    assert native[-1] == "rtp_rmsnorm_fp8_forward" and q.shape == s.shape == (2, 7, 40) and scale.shape == (2, 7, 1) and filled(q)
+    with pytest.raises(Exception, match="expected"):               # rows that the weight does not have
+        f(torch.ones(3, 41), torch.ones(3, 41), w)
+    f = traced(lambda x, w: add_rms_norm_fp8(x, None, w), x, w)
+    z = torch.ones(5, 40)
+    q, scale, s = f(z, w)
+    assert q.shape == (5, 40) and filled(q) and torch.equal(s, z)
+    (a, sa), (b, sb) = eight(3, 40, False), eight(5, 40, True)
+    f = traced(lambda a, sa, b, sb: matmul_fp8(a, sa, b, sb, torch.float16), a, sa, b, sb)
+    (a, sa), (b, sb) = eight(4, 300, False), eight(200, 300, True)
+    out = f(a, sa, b, sb)
+    assert native[-1] == "rtp_matmul_fp8" and out.shape == (4, 200) and out.dtype == torch.float16 and filled(out)
+    with pytest.raises(Exception, match="expected"):
+        f(a, sa[:3], b, sb)
