@@ -6,13 +6,13 @@
     RMSNorm(dim)                                   module over the first two
 
 x, residual: [..., dim] of one type (fp32, fp16, bf16), any strides; weight: [dim], of that type or fp32.  Differentiable in x, residual
-and weight (not in the 8-bit form); the sums are fp32 and the gradients do not depend on scheduling.  Error behaviour as in
+and weight (not in the 8-bit form; forward-mode tangents are refused with NotImplementedError); the sums are fp32 and the gradients do not
+depend on scheduling.  A trace holds each call as one node, which checks its arguments every time.  Error behaviour as in
 rt_pose_amd.dcn: CPU tensors -> NotImplementedError, a wrong type -> NotImplementedError, shapes that do not fit -> ValueError,
 a failing native call -> RtpError.
 """
 import torch
 import torch.nn as nn
-from torch.autograd import Function
 
 from . import _lib
 from ._tokens import DTYPES, TokenFunction, call, fp8_rows, like, once, p, rows_of, same_device, without_gradient
@@ -60,9 +60,10 @@ def _backward(s, weight, eps, dy, ds, need_w):
     return dx, dw if need_w else None
 
 
-class RMSNormFunction(Function):
+class RMSNormFunction(TokenFunction):
     @staticmethod
     def forward(ctx, x, weight, eps):
+        _check(x, None, weight)
         ctx.eps = eps
         ctx.save_for_backward(x, weight)
         return _forward(x, None, weight, eps)[0]
@@ -75,9 +76,10 @@ class RMSNormFunction(Function):
         return dx, dw, None
 
 
-class AddRMSNormFunction(Function):
+class AddRMSNormFunction(TokenFunction):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
+        _check(x, residual, weight)
         y, s = _forward(x, residual, weight, eps)
         ctx.eps = eps
         ctx.set_materialize_grads(False)
@@ -108,14 +110,12 @@ class AddRMSNormFp8Function(TokenFunction):
 
 
 def rms_norm(x, weight, eps=1e-6):
-    _check(x, None, weight)
     return RMSNormFunction.apply(x, weight, float(eps))
 
 
 def add_rms_norm(x, residual, weight, eps=1e-6):
     if residual is None:
         raise ValueError("add_rms_norm: a residual is expected (rms_norm has none)")
-    _check(x, residual, weight)
     return AddRMSNormFunction.apply(x, residual, weight, float(eps))
 
 

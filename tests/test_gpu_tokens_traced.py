@@ -58,3 +58,14 @@ def test_8_bit_operands_that_are_copied():
     for a, b in ((some[:, 3:333], some[:4, 1:331]), (some[:, ::3][:, :133], some[:, 1::3])):
         args = a, scale(a.shape[0], a.shape[1]), b, scale(b.shape[0], b.shape[1])
         assert torch.equal(f(*args), matmul_fp8(*args))
+
+
+def test_norms():
+    from rt_pose_amd.rmsnorm import add_rms_norm, rms_norm
+    w = rnd(200, seed=1).requires_grad_(True)
+    f, g = traced(rms_norm, rnd(3, 200, seed=2), w), traced(add_rms_norm, rnd(3, 200, seed=2), rnd(3, 200, seed=3), w)
+    for rows in (1, 300):
+        x, r = rnd(rows, 200, seed=rows).requires_grad_(True), rnd(200, rows, seed=rows + 1).t().requires_grad_(True)
+        for a, b in ((torch.autograd.grad(f(x, w), (x, w), r), torch.autograd.grad(rms_norm(x, w), (x, w), r)),
+                     (torch.autograd.grad(g(x, r, w), (x, r, w), (r, x)), torch.autograd.grad(add_rms_norm(x, r, w), (x, r, w), (r, x)))):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))

@@ -17,6 +17,7 @@ def native(monkeypatch):
     entries = {"rtp_xattn_forward": lambda a, o, *_: (o, a._obj.b * a._obj.sq * a._obj.hq * a._obj.d * 2),
                "rtp_quantize_fp8": lambda x, x_rs, turned, q, q_rs, scale, rows, *_: (q, rows * q_rs),
                "rtp_matmul_fp8": lambda a, lda, sa, b, ldb, sb, square, out, m, n, k, t: (out, m * n * (4 if t == 0 else 2)),
+               "rtp_rmsnorm_forward": lambda x, x_rs, r, r_rs, w, wt, y, s, rows, h, t, eps: (y, rows * h * (4 if t == 0 else 2)),
                "rtp_rmsnorm_fp8_forward": lambda x, x_rs, r, r_rs, w, wt, q, q_rs, scale, s, rows, *_: (q, rows * q_rs)}
 
     def call(name, t, *args):
@@ -136,3 +137,24 @@ def test_the_8_bit_entries_are_nodes_of_a_trace(native):
     assert native[-1] == "rtp_matmul_fp8" and out.shape == (4, 200) and out.dtype == torch.float16 and filled(out)
     with pytest.raises(Exception, match="expected"):
         f(a, sa[:3], b, sb)
+
+
+def test_the_norms_refuse_tangents(native):
+    from rt_pose_amd.rmsnorm import add_rms_norm, rms_norm
+    x, w = torch.ones(3, 40, dtype=torch.bfloat16), torch.ones(40)
+    tangents_are_refused(rms_norm, x, w)
+    tangents_are_refused(add_rms_norm, x, x, w)
+
+
+def test_the_norms_check_at_every_call_of_a_trace(native):
+    from rt_pose_amd.rmsnorm import RMSNorm, add_rms_norm, rms_norm
+    x, w = torch.ones(3, 40), torch.ones(40)
+    f, g, m = traced(rms_norm, x, w), traced(add_rms_norm, x, x, w), traced(RMSNorm(40), x)
+    z = torch.ones(2, 7, 40)
+    assert filled(f(z, w)) and filled(g(z, z, w)[0]) and filled(m(z))
+    wide = torch.ones(3, 41)
+    for call in (lambda: f(wide, w), lambda: g(wide, wide, w), lambda: g(x, wide, w), lambda: m(wide)):
+        done = len(native)
+        with pytest.raises(Exception, match="rms norm"):
+            call()
+        assert len(native) == done                                 # nothing is read that is not there
