@@ -320,11 +320,12 @@ static int c64_launch(C64Params& p, const RtpConvGeom* g, int wgs, hipStream_t s
   p.wgs_per_sample = wgs;
   const long vox = (long)p.D * p.H * p.W;
   if (vox * p.x_cs[0] >= (1L << 31) || vox * p.x_cs[1] >= (1L << 31) || (long)p.tiles_per_sample * (wgs + 1) >= (1L << 31)) return RTP_ERR_SHAPE;
-  static bool attr_done[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr_done)) {
-    (void)hipFuncSetAttribute((const void*)conv64_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, C64_LDS_B);
-    (void)hipFuncSetAttribute((const void*)conv64_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, C64_LDS_B);
-  }
+  static std::atomic<bool> attr_done[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr_done, [&] {
+        return hipFuncSetAttribute((const void*)conv64_kernel<false>, hipFuncAttributeMaxDynamicSharedMemorySize, C64_LDS_B) == hipSuccess &&
+               hipFuncSetAttribute((const void*)conv64_kernel<true>, hipFuncAttributeMaxDynamicSharedMemorySize, C64_LDS_B) == hipSuccess;
+      }))
+    return RTP_ERR_LAUNCH;
   RtpProfScope prof(RTP_FAM_CONV64, s);
   if (p.acc_in || p.acc_out) hipLaunchKernelGGL(conv64_kernel<true>, dim3(p.N * wgs), dim3(512), C64_LDS_B, s, p);
   else hipLaunchKernelGGL(conv64_kernel<false>, dim3(p.N * wgs), dim3(512), C64_LDS_B, s, p);

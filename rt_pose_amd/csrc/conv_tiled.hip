@@ -1151,8 +1151,9 @@ int rtp_conv_tiled_try(const RtpAct* x, const void* wf, int w_per_sample, const 
                                             {RTP_TILED_ROW(2, false), RTP_TILED_ROW(2, true)}};   // [nt][class bias][aux][statistics][fp32 in/out]
 #undef RTP_TILED_ROW
 #undef RTP_TILED_CELL
-  static bool attr_done[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr_done)) {
+  static std::atomic<bool> attr_done[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr_done, [&] {
+    bool ok = true;
     const int big = (int)(sizeof(bf16_t) * (27 * (size_t)32 * 32 + 2 * (size_t)HALO_VOX * 32) + 27 * 32 * sizeof(float) + 64);
     for (int a = 0; a < 2; ++a)
       for (int b = 0; b < 2; ++b)
@@ -1160,18 +1161,23 @@ int rtp_conv_tiled_try(const RtpAct* x, const void* wf, int w_per_sample, const 
           for (int d = 0; d < 2; ++d)
             for (int e = 0; e < 2; ++e)
               if (table[a][b][c][d][e])
-                (void)hipFuncSetAttribute((const void*)table[a][b][c][d][e], hipFuncAttributeMaxDynamicSharedMemorySize, big);
-  }
+                ok = ok && hipFuncSetAttribute((const void*)table[a][b][c][d][e], hipFuncAttributeMaxDynamicSharedMemorySize, big) == hipSuccess;
+    return ok;
+  }))
+    return RTP_ERR_LAUNCH;
   const int aux = stat_x ? 2 : (res ? 1 : 0);
   if (fuse) {
     static const Kern ftab[4] = {conv_tiled_kernel<2, false, 2, false, 1>, conv_tiled_kernel<2, false, 2, false, 2>,
                                  conv_tiled_kernel<2, false, 2, false, 3>, conv_tiled_kernel<2, false, 2, false, 4>};
-    static bool fattr[RTP_MAX_DEVICES] = {};
-    if (rtp_once_per_device(fattr)) {
+    static std::atomic<bool> fattr[RTP_MAX_DEVICES];
+    if (!rtp_once_per_device(fattr, [&] {
+      bool ok = true;
       for (int e = 0; e < 4; ++e)
-        (void)hipFuncSetAttribute((const void*)ftab[e], hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  (int)(sizeof(bf16_t) * (27 * (size_t)32 * 32 + 2 * (size_t)HALO_VOX * 32) + 27 * 32 * sizeof(float) + 64));
-    }
+        ok = ok && hipFuncSetAttribute((const void*)ftab[e], hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)(sizeof(bf16_t) * (27 * (size_t)32 * 32 + 2 * (size_t)HALO_VOX * 32) + 27 * 32 * sizeof(float) + 64)) == hipSuccess;
+      return ok;
+    }))
+      return RTP_ERR_LAUNCH;
     hipLaunchKernelGGL(ftab[p.nextra], dim3(p.N * wgs), dim3(512), shm, s, p);
     RTP_CHECK_LAUNCH();
     return RTP_OK;

@@ -1272,9 +1272,9 @@ static int xa_types(const RtpXattn* a, F f) {
   return a->dtype == RTP_DT_BF16 ? width(bf16_t{}) : width(_Float16{});
 }
 template <typename K>
-static int xa_launch(K kernel, int grid, int bytes, bool* once, hipStream_t st, const XaParams& p) {
-  if (bytes > 65536 && rtp_once_per_device(once) &&
-      hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+static int xa_launch(K kernel, int grid, int bytes, std::atomic<bool>* once, hipStream_t st, const XaParams& p) {
+  if (bytes > 65536 &&
+      !rtp_once_per_device(once, [&] { return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; }))
     return RTP_ERR_LAUNCH;
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), bytes, st, p);
   RTP_CHECK_LAUNCH();
@@ -1283,22 +1283,22 @@ static int xa_launch(K kernel, int grid, int bytes, bool* once, hipStream_t st, 
 
 template <typename T, int DT, int KW>
 static int xa_fwd(int grid, hipStream_t st, const XaParams& p) {
-  static bool once[RTP_MAX_DEVICES];
+  static std::atomic<bool> once[RTP_MAX_DEVICES];
   return xa_launch(xattn_fwd_kernel<T, DT, KW>, grid, XaKeys<DT, KW>::BYTES, once, st, p);
 }
 template <typename T, int DT, int KW>
 static int xa_dq(int grid, hipStream_t st, const XaParams& p) {
-  static bool once[RTP_MAX_DEVICES];
+  static std::atomic<bool> once[RTP_MAX_DEVICES];
   return xa_launch(xattn_dq_kernel<T, DT, KW>, grid, XaKeys<DT, KW>::BYTES, once, st, p);
 }
 template <typename T, int DT>
 static int xa_dkv(int grid, hipStream_t st, const XaParams& p) {
-  static bool once[RTP_MAX_DEVICES];
+  static std::atomic<bool> once[RTP_MAX_DEVICES];
   return xa_launch(xattn_dkv_kernel<T, DT>, grid, XaRows<DT>::BYTES, once, st, p);
 }
 template <typename T, int DT>
 static int xa_bwd_few(int grid, hipStream_t st, const XaParams& p) {
-  static bool once[RTP_MAX_DEVICES];
+  static std::atomic<bool> once[RTP_MAX_DEVICES];
   return xa_launch(xattn_bwd_few_kernel<T, DT>, grid, XaFew<DT>::BYTES, once, st, p);
 }
 

@@ -1598,13 +1598,9 @@ static int dcn_gradw_fused_launch(const float* input, const float* offset, const
   int tpb = (int)((tiles + 511) / 512);   // two 4-wave blocks per CU
   if (tpb < 1) tpb = 1;
   const size_t lds = sizeof(float) * 4 * 72 * DCN_GF_ROW;
-  static bool attr[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr)) {
-    if (hipFuncSetAttribute((const void*)dcn_gradw_fused_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
-      attr[rtp_device_index()] = false;
-      return RTP_ERR_LAUNCH;
-    }
-  }
+  static std::atomic<bool> attr[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr, [&] { return hipFuncSetAttribute((const void*)dcn_gradw_fused_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess; }))
+    return RTP_ERR_LAUNCH;
   hipLaunchKernelGGL(dcn_gradw_fused_kernel, dim3((unsigned)((tiles + tpb - 1) / tpb)), dim3(256), lds, s, input, offset, mask,
                      gradOutput, gradWeight, g, scale, tpb);
   return RTP_OK;
@@ -2177,14 +2173,15 @@ static int dcn_backward_fused(const float* input, const float* offset, const flo
   unsigned* rec = (unsigned*)ws;
   if (hipMemsetAsync(rec, 0, 8, s) != hipSuccess) return RTP_ERR_LAUNCH;
   const size_t lds = sizeof(float) * 4 * (72 * DCN_FB_ROW + 8 * 7 * 64);   // tiles + rings: 135 680 B, one block per CU
-  static bool attr[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr)) {   // 135 KB of LDS: above the default limit, the launch fails without the attribute
+  static std::atomic<bool> attr[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr, [&] {   // 135 KB of LDS: above the default limit, the launch fails without the attribute
     bool ok = hipFuncSetAttribute((const void*)dcn_bwd_fused_kernel<true, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
     ok = ok && hipFuncSetAttribute((const void*)dcn_bwd_fused_kernel<false, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
     ok = ok && hipFuncSetAttribute((const void*)dcn_bwd_fused_kernel<true, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
     ok = ok && hipFuncSetAttribute((const void*)dcn_bwd_fused_kernel<false, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) == hipSuccess;
-    if (!ok) { attr[rtp_device_index()] = false; return RTP_ERR_LAUNCH; }
-  }
+    return ok;
+  }))
+    return RTP_ERR_LAUNCH;
   const bool split = false;   // (weight gradient by dcn_gradw_fused_kernel, a gather pass of its own: measured slower, round 3)
   float* gwk = split ? nullptr : gradWeight;
   const char* fe = getenv("RTP_DCN_FP32_MFMA");  // the two products on the fp32 matrix instruction (exact products, 3x the cycles)

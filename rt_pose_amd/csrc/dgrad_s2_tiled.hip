@@ -424,10 +424,13 @@ int rtp_dgrad_s2_try(const RtpAct* gy, const void* wd, const RtpAct* dx, const R
   const size_t shm = sizeof(bf16_t) * (27 * 32 * 32 + 2 * GVOX * 32) + 864 * sizeof(float);
   using Kern = void (*)(S2Params);
   static const Kern tab[5] = {dgrad_s2_kernel<0>, dgrad_s2_kernel<1>, dgrad_s2_kernel<2>, dgrad_s2_kernel<3>, dgrad_s2_kernel<4>};
-  static bool attr[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr)) {
-    for (int i = 0; i < 5; ++i) (void)hipFuncSetAttribute((const void*)tab[i], hipFuncAttributeMaxDynamicSharedMemorySize, (int)shm);
-  }
+  static std::atomic<bool> attr[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr, [&] {
+        bool ok = true;
+        for (int i = 0; i < 5; ++i) ok = ok && hipFuncSetAttribute((const void*)tab[i], hipFuncAttributeMaxDynamicSharedMemorySize, (int)shm) == hipSuccess;
+        return ok;
+      }))
+    return RTP_ERR_LAUNCH;
   RtpProfScope prof(RTP_FAM_CONV_TILED, s);
   hipLaunchKernelGGL(tab[mode], dim3(p.N * p.wgs_per_sample), dim3(256), shm, s, p);
   RTP_CHECK_LAUNCH();

@@ -406,18 +406,18 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
     return nt == 4 ? few(mm8_few_kernel<O, 4, 4, 1, SQUARE>) : nt == 2 ? few(mm8_few_kernel<O, 4, 2, 2, SQUARE>) : few(mm8_few_kernel<O, 4, 1, 2, SQUARE>);
   }
   const long tiles256 = (long)rtp_div_up(p.m, 256) * rtp_div_up(p.n, 256);
-  auto go = [&](auto kernel, int bm, int bn, int threads, bool* once) {
+  auto go = [&](auto kernel, int bm, int bn, int threads, std::atomic<bool>* once) {
     p.tiles_m = rtp_div_up(p.m, bm);
     p.tiles_n = rtp_div_up(p.n, bn);
     if (!rtp_launchable((long)p.tiles_m * p.tiles_n, threads)) return RTP_ERR_SHAPE;
     const int ring = 2 * ((bm + bn) * 128 + (bm + (SQUARE ? 64 : bn)) * 4), out = bm * (bn * (int)sizeof(O) + 16), bytes = ring > out ? ring : out;
-    if (rtp_once_per_device(once) && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+    if (!rtp_once_per_device(once, [&] { return hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; }))
       return RTP_ERR_LAUNCH;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((long)p.tiles_m * p.tiles_n)), dim3(threads), bytes, st, p);
     RTP_CHECK_LAUNCH();
     return RTP_OK;
   };
-  static bool once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES], once64[RTP_MAX_DEVICES];
+  static std::atomic<bool> once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES], once64[RTP_MAX_DEVICES];
   // 256 x 256 halves what is staged per product and wins where the sum is long and its tiles fill whole rounds of the 256 CUs (8192^3: 493 us
   // against 580, 4096^3: 72 against 77); 128 x 128, two workgroups to a CU, where one's start and end hide behind the other's sum
   // (163840 x 256 x 384: 40 us against 57, x 1024: 71 against 87).  The exact road needs the registers of the small tile.

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "../../include/rtp.h"
+#include "rtp_once.h"
 
 typedef __bf16 bf16_t;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
@@ -77,18 +78,15 @@ __host__ __device__ __forceinline__ bool tap_inb_1d(int k, int first, int last, 
 
 static inline int rtp_div_up(long a, long b) { return (int)((a + b - 1) / b); }
 
-// One-time per-DEVICE set-up (hipFuncSetAttribute and cached device properties are per device: a process-wide `static bool`
-// would leave a second GPU of the same process without its LDS limit).  `flags` is a static bool[RTP_MAX_DEVICES]; true exactly
-// once per device.
-#define RTP_MAX_DEVICES 16
+// slot of the current device in a static array[RTP_MAX_DEVICES] of cached properties
 static inline int rtp_device_index() {
   int d = 0;
   if (hipGetDevice(&d) != hipSuccess || d < 0 || d >= RTP_MAX_DEVICES) d = 0;
   return d;
 }
-static inline bool rtp_once_per_device(bool* flags) {
-  const int d = rtp_device_index();
-  if (flags[d]) return false;
-  flags[d] = true;
-  return true;
+template <typename F>
+static inline bool rtp_once_per_device(std::atomic<bool>* done, F set) {
+  int d = 0;
+  if (hipGetDevice(&d) != hipSuccess) d = -1;
+  return rtp_once(done, d, set);
 }

@@ -286,10 +286,9 @@ extern "C" int rtp_wgrad(const RtpAct* gy, const RtpAct* x, const RtpConvGeom* g
   static const bool no_1x1 = false;
   if (!no_1x1 && p.ks == 1 && p.stride == 1 && p.pad == 0 && (p.co32 / 32) * p.citiles <= 16) {
     const size_t shm = sizeof(bf16_t) * (size_t)(p.co32 / 32 + p.citiles) * W1_VB * 32;
-    static bool attr[RTP_MAX_DEVICES] = {};
-    if (rtp_once_per_device(attr)) {
-      (void)hipFuncSetAttribute((const void*)wgrad_1x1_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-    }
+    static std::atomic<bool> attr[RTP_MAX_DEVICES];
+    if (!rtp_once_per_device(attr, [&] { return hipFuncSetAttribute((const void*)wgrad_1x1_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) == hipSuccess; }))
+      return RTP_ERR_LAUNCH;
     hipLaunchKernelGGL(wgrad_1x1_kernel, dim3(nsplit, p.N), dim3(256), shm, s, p);
     RTP_CHECK_LAUNCH();
     return RTP_OK;

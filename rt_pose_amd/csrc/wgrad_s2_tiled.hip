@@ -261,10 +261,9 @@ int rtp_wgrad_s2_try(const RtpAct* gy, const RtpAct* x, const RtpConvGeom* g, in
   p.wgs_per_sample = nsplit; p.part_stride = nsplit;
   const size_t shm = sizeof(bf16_t) * (size_t)W2_RING * W2_SLOT;
   RtpProfScope prof(RTP_FAM_WGRAD_TILED, s);
-  static bool attr[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr)) {
-    (void)hipFuncSetAttribute((const void*)wgrad_s2_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shm);
-  }
+  static std::atomic<bool> attr[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr, [&] { return hipFuncSetAttribute((const void*)wgrad_s2_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)shm) == hipSuccess; }))
+    return RTP_ERR_LAUNCH;
   hipLaunchKernelGGL(wgrad_s2_kernel, dim3(p.N * p.wgs_per_sample), dim3(512), shm, s, p);
   RTP_CHECK_LAUNCH();
   return RTP_OK;

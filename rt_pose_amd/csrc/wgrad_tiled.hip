@@ -578,11 +578,12 @@ int rtp_wgrad_tiled_try(const RtpAct* gy, const RtpAct* x, const RtpConvGeom* g,
     return RTP_OK;
   }
   RtpProfScope prof(RTP_FAM_WGRAD_TILED, s);
-  static bool attr[RTP_MAX_DEVICES] = {};
-  if (rtp_once_per_device(attr)) {
-    (void)hipFuncSetAttribute((const void*)wgrad_tiled_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              (int)(shm_base + 4 * 27 * 32 * sizeof(float) + 16));
-  }
+  static std::atomic<bool> attr[RTP_MAX_DEVICES];
+  if (!rtp_once_per_device(attr, [&] {
+        return hipFuncSetAttribute((const void*)wgrad_tiled_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)(shm_base + 4 * 27 * 32 * sizeof(float) + 16)) == hipSuccess;
+      }))
+    return RTP_ERR_LAUNCH;
   hipLaunchKernelGGL(wgrad_tiled_kernel, dim3(p.N * p.wgs_per_sample), dim3(WG_THREADS), shm, s, p);
   RTP_CHECK_LAUNCH();
   return RTP_OK;
