@@ -1,7 +1,7 @@
 """Build librtp_hip.so (all HIP kernels + the C ABI) for gfx950 with hipcc, in-tree.
 
-    python -m rt_pose_amd.build            # incremental
-    python -m rt_pose_amd.build --force
+    python -m rt_pose_amd.build            # what is older than its source or was made by another command (flags, compiler)
+    python -m rt_pose_amd.build --force    # everything
 
 hipcc cross-compiles without a GPU, so this also runs in the CPU-only authoring container.
 """
@@ -37,29 +37,50 @@ def _deps_mtime():
     return max(os.path.getmtime(h) for h in hdrs)
 
 
-def _compile(src, force, hdr_m):
-    obj = os.path.join(OBJ, src[:-4] + ".o")
-    srcp = os.path.join(CSRC, src)
-    if not force and os.path.exists(obj) and os.path.getmtime(obj) > max(os.path.getmtime(srcp), hdr_m):
-        return obj, False
-    cmd = [HIPCC, *FLAGS, "-c", srcp, "-o", obj]
+def _made_by(out, cmd):
+    """Whether `out` is there and this very command made it (recorded beside it once it had succeeded)."""
+    try:
+        with open(out + ".cmd") as f:
+            return os.path.exists(out) and f.read() == cmd
+    except OSError:
+        return False
+
+
+def _run(cmd, out, what):
+    if os.path.exists(out + ".cmd"):
+        os.remove(out + ".cmd")
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
-    return obj, True
+        raise RuntimeError("%s failed:\n%s\n%s" % (what, r.stdout, r.stderr))
+    with open(out + ".cmd", "w") as f:
+        f.write(_record(cmd))
+
+
+def _record(cmd):
+    """The command and the compiler that it stands for: another release, or another file at the same place, is another command."""
+    real = os.path.realpath(cmd[0])
+    return "\n".join([real, str(os.path.getmtime(real)) if os.path.exists(real) else "", *cmd])
+
+
+def _compile(src, force, hdr_m):
+    """An object is taken as it is if it is newer than its source and the headers and was made by the same command: other flags make other code."""
+    obj = os.path.join(OBJ, src[:-4] + ".o")
+    srcp = os.path.join(CSRC, src)
+    cmd = [HIPCC, *FLAGS, "-c", srcp, "-o", obj]
+    if not force and _made_by(obj, _record(cmd)) and os.path.getmtime(obj) > max(os.path.getmtime(srcp), hdr_m):
+        return obj
+    _run(cmd, obj, "hipcc for %s" % src)
+    return obj
 
 
 def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
     hdr_m = _deps_mtime()
     with ThreadPoolExecutor(max_workers=4) as ex:
-        res = list(ex.map(lambda s: _compile(s, force, hdr_m), sources()))
-    objs = [o for o, _ in res]
-    if force or any(ch for _, ch in res) or not os.path.exists(LIB):
-        cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError("link failed:\n%s\n%s" % (r.stdout, r.stderr))
+        objs = list(ex.map(lambda s: _compile(s, force, hdr_m), sources()))
+    cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB, *objs]
+    if force or not _made_by(LIB, _record(cmd)) or os.path.getmtime(LIB) < max(os.path.getmtime(o) for o in objs):
+        _run(cmd, LIB, "link")
         if verbose:
             print("built", LIB)
     elif verbose:
