@@ -1251,7 +1251,7 @@ extern "C" long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward) {
 static unsigned* xa_kept(const RtpXattn* a, const float* lse) { return (unsigned*)lse + (((long)a->b * a->sq * a->hq + 63) & ~63L); }
 
 static int xa_bits(const RtpXattn* a, XaParams& p, float* lse, uint8_t*& ws, hipStream_t st) {
-  if (!a->key_mask) return RTP_OK;
+  if (!a->key_mask || a->sk == 0) return RTP_OK;      // no keys: a launch of no workgroups would be an error
   p.bits = lse ? xa_kept(a, lse) : (unsigned*)ws;
   ws += xa_round((long)a->b * p.words * 4);
   hipLaunchKernelGGL(xattn_bits_kernel, dim3((unsigned)rtp_div_up(p.words, 8) * a->b), dim3(256), 0, st, (const uint8_t*)a->key_mask, a->m_bs, a->m_ss, a->key_lens,
