@@ -603,6 +603,8 @@ typedef struct RtpXattn {
   float scale;
 } RtpXattn;
 long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward);
+/* How a call of these sizes is cut: the waves of a workgroup (4, 2 or 1 of four) that share its query rows and split each tile of keys. -1: refused. */
+int rtp_xattn_row_waves(const RtpXattn* a);
 int rtp_xattn_forward(const RtpXattn* a, void* o, void* o_lo, float* lse, void* ws, long ws_bytes, void* stream);
 int rtp_xattn_backward(const RtpXattn* a, const void* o, const void* o_lo, const float* lse, const void* d_o, long o_bs, long o_ss, long o_hs,
                        void* dq, void* dk, void* dv, void* ws, long ws_bytes, void* stream);

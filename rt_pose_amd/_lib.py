@@ -167,6 +167,7 @@ PROTOTYPES = {
     "rtp_quantize_fp8": [_P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _P],
     "rtp_matmul_fp8": [_P, _L, _P, _P, _L, _P, _I, _P, _I, _I, _I, _I, _P],
     "rtp_xattn_workspace_bytes": [C.POINTER(RtpXattn), _I],
+    "rtp_xattn_row_waves": [C.POINTER(RtpXattn)],
     "rtp_xattn_forward": [C.POINTER(RtpXattn), _P, _P, _P, _P, _L, _P],
     "rtp_xattn_backward": [C.POINTER(RtpXattn), _P, _P, _P, _P, _L, _L, _L, _P, _P, _P, _P, _L, _P],
     "rtp_prof_enable": [_I, _I],

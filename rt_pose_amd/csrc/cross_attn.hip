@@ -1247,6 +1247,8 @@ extern "C" long rtp_xattn_workspace_bytes(const RtpXattn* a, int backward) {
   return xa_round(rows * 4) + xa_round(q > kv ? q : kv);   // dq and dk / dv run one after the other
 }
 
+extern "C" int rtp_xattn_row_waves(const RtpXattn* a) { return xa_check(a) == RTP_OK ? xa_plan(a).kw : -1; }
+
 // where the masks' bits stand behind lse, for the backward pass
 static unsigned* xa_kept(const RtpXattn* a, const float* lse) { return (unsigned*)lse + (((long)a->b * a->sq * a->hq + 63) & ~63L); }
 
