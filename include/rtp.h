@@ -563,7 +563,7 @@ int rtp_modulated_deform_conv_backward(const float* input, const float* weight, 
  * Root-mean-square norm (csrc/token_norm.hip): s = round(x + res), y = s / sqrt(mean(s^2) + eps) * w.  res may be NULL (s = x); s may be
  * NULL when res is.  w_dtype: the values' type or RTP_DT_F32.  h <= 16384.  s, y, dx: contiguous rows of h.
  * Backward: dx (= the residual's gradient too) = rho (g - xhat mean(g xhat)) + ds with g = dy w; ds may be NULL; dw of w's type.
- * part: rtp_rmsnorm_backward_slots(rows, h) * h floats of scratch.  Deterministic. */
+ * part: rtp_rmsnorm_backward_slots(rows, h) * h floats of scratch.  dw may be NULL (a weight that is not trained), part then too.  Deterministic. */
 int rtp_rmsnorm_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* y, void* s, long rows, int h,
                         int dtype, float eps, void* stream);
 int rtp_rmsnorm_fp8_forward(const void* x, long x_rs, const void* res, long res_rs, const void* w, int w_dtype, void* q, long q_rs,

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_fwd_kernel(Norm
 struct NormBwdParams {
   const void *s, *w, *dy, *ds;
   void* dx;
-  float* part;   // [gridDim.x][h]
+  float* part;   // [gridDim.x][h], or null: dw is not wanted
   long s_rs, dy_rs, ds_rs, rows;
   int h;
   float eps;
@@ -183,6 +183,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rmsnorm_bwd_kernel(Norm
       put_row8<KIND>((T*)p.dx + row * p.h, d[i], c, p.h);
     }
   }
+  if (!p.part) return;
   if constexpr (GROUPS > 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -316,10 +317,10 @@ extern "C" int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int
                                     void* dx, void* dw, float* part, long rows, int h, int dtype, float eps, void* stream) {
   if (rows < 1 || h < 1 || rows >= (1L << 31)) return RTP_ERR_SHAPE;
   if (h > NORM_MAX_H) return RTP_ERR_UNSUPPORTED;
-  if (!s || !w || !dy || !dx || !dw || !part) return RTP_ERR_SHAPE;
+  if (!s || !w || !dy || !dx || (dw && !part)) return RTP_ERR_SHAPE;
   hipStream_t st = (hipStream_t)stream;
   RtpProfScope prof(RTP_FAM_NORM, st);
-  NormBwdParams p{s, w, dy, ds, dx, part, s_rs, dy_rs, ds_rs, rows, h, eps};
+  NormBwdParams p{s, w, dy, ds, dx, dw ? part : nullptr, s_rs, dy_rs, ds_rs, rows, h, eps};
   const int slots = rtp_rmsnorm_backward_slots(rows, h);
   return norm_types(dtype, w_dtype, [&](auto t, auto wt) {
     return norm_shape(h, [&](auto lpr, auto nv, auto kind) {
@@ -327,6 +328,7 @@ extern "C" int rtp_rmsnorm_backward(const void* s, long s_rs, const void* w, int
       typedef decltype(wt) W;
       hipLaunchKernelGGL((rmsnorm_bwd_kernel<decltype(t), W, LPR, NV, decltype(kind)::value>), dim3(slots), dim3(THREADS), 0, st, p);
       RTP_CHECK_LAUNCH();
+      if (!dw) return RTP_OK;
       hipLaunchKernelGGL((rmsnorm_dw_kernel<W>), dim3(rtp_div_up(h, 16)), dim3(1024), 0, st, part, slots, h, (W*)dw);
       RTP_CHECK_LAUNCH();
       return RTP_OK;

@@ -47,17 +47,17 @@ def _forward(x, residual, weight, eps):
 
 
 def _backward(s, weight, eps, dy, ds, need_w):
-    """dx (also the residual's gradient) and dw of the rows `s` that were normed."""
+    """dx (also the residual's gradient) and, if need_w, dw of the rows `s` that were normed."""
     s2, w = rows_of(s), weight.contiguous()
     rows, h = s2.shape
-    dx, dw = like(s), torch.empty_like(w)
+    dx, dw = like(s), torch.empty_like(w) if need_w else None
     if rows == 0:
         return dx, dw.zero_() if need_w else None
     dy2, ds2 = rows_of(dy), rows_of(ds) if ds is not None else None
-    part = s.new_empty(_lib.load().rtp_rmsnorm_backward_slots(rows, h) * h, dtype=torch.float32)
+    part = s.new_empty(_lib.load().rtp_rmsnorm_backward_slots(rows, h) * h, dtype=torch.float32) if need_w else None
     call("rtp_rmsnorm_backward", s, p(s2), s2.stride(0), p(w), DTYPES[w.dtype], p(dy2), dy2.stride(0), p(ds2), 0 if ds2 is None else ds2.stride(0),
          p(dx), p(dw), p(part), rows, h, DTYPES[s.dtype], eps)
-    return dx, dw if need_w else None
+    return dx, dw
 
 
 class RMSNormFunction(TokenFunction):

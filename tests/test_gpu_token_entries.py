@@ -26,3 +26,22 @@ def test_cross_attention_without_keys_beside_a_mask(sq, lse):
     assert float(o.abs().sum()) == 0
     if lse:
         assert float(lo.abs().sum()) == 0 and bool((stat[:q.shape[:3].numel()] == float("inf")).all())
+
+
+@pytest.mark.parametrize("rows,h", [(3, 7), (5000, 100), (4200, 777), (600, 4100), (300, 12345)])
+def test_norm_gradients_with_a_weight_that_is_not_trained(rows, h):
+    """dx alone, by Python and by the C entry without dw and its scratch: the same dx; a dw without its scratch is refused."""
+    from rt_pose_amd import _lib
+    from rt_pose_amd.rmsnorm import add_rms_norm, rms_norm
+    g = torch.Generator().manual_seed(rows)
+    x, r, dy, ds = (torch.randn(rows, h, generator=g).to(torch.bfloat16).cuda() for _ in range(4))
+    w = torch.rand(h, generator=g).cuda()
+    x.requires_grad_(True)
+    both = torch.autograd.grad(add_rms_norm(x, r, w.clone().requires_grad_(True)), x, (dy, ds))[0]
+    assert torch.equal(torch.autograd.grad(add_rms_norm(x, r, w), x, (dy, ds))[0], both)
+    want = torch.autograd.grad(rms_norm(x, w.clone().requires_grad_(True)), x, dy)[0]
+    assert torch.equal(torch.autograd.grad(rms_norm(x, w), x, dy)[0], want)
+    dx, p, s = torch.empty_like(dy), x.data_ptr, torch.cuda.current_stream().cuda_stream
+    entry = lambda dw, part: _lib.load().rtp_rmsnorm_backward(p(), h, w.data_ptr(), 0, dy.data_ptr(), h, None, 0, dx.data_ptr(), dw, part, rows, h, 2, 1e-6, s)
+    assert entry(w.data_ptr(), None) == -1
+    assert entry(None, None) == 0 and torch.equal(dx, want)

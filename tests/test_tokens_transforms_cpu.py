@@ -158,3 +158,17 @@ def test_the_norms_check_at_every_call_of_a_trace(native):
         with pytest.raises(Exception, match="rms norm"):
             call()
         assert len(native) == done                                 # nothing is read that is not there
+
+
+def test_a_weight_that_is_not_trained_costs_no_gradient(monkeypatch):
+    """Neither the weight's gradient nor its partial rows are asked for."""
+    from rt_pose_amd import rmsnorm
+    made = []
+    monkeypatch.setattr(rmsnorm, "same_device", lambda *a: None)
+    monkeypatch.setattr(rmsnorm, "call", lambda name, t, *args: made.append((name, args)))
+    for trained in (False, True):
+        x, w = torch.ones(3, 40, requires_grad=True), torch.ones(40, requires_grad=trained)
+        for f in (lambda: rmsnorm.rms_norm(x, w), lambda: rmsnorm.add_rms_norm(x, x, w)[0]):
+            f().sum().backward()
+            name, args = made[-1]
+            assert name == "rtp_rmsnorm_backward" and (args[9] is not None) == (args[10] is not None) == trained
