@@ -579,14 +579,16 @@ int rtp_quantize_fp8(const void* x, long x_rs, int turned, void* q, long q_rs, f
 
 /* out[m][n] = the product of a [m][k] and the transpose of b [n][k], both in 8 bits with scales (csrc/matmul_fp8.hip).  sa: [m][ceil(k / 128)];
  * sb: [ceil(n / 128)][ceil(k / 128)] (b_square = 1) or [n][ceil(k / 128)].  Rows of a and b are readable up to k rounded up to 16; what stands
- * there does not count.  out: row stride n, out_dtype any of the three.  lda, ldb <= 2^22 (and so k); m, n <= 2^30. */
+ * there does not count.  out: row stride n, out_dtype any of the three.  fp32: exact products, fp32 sums.  fp16 and bf16: groups of eight neighbouring
+ * products are added at 14 bits (each loses less than 2^-13 of its group's largest), then fp32.  lda, ldb <= 2^22 (and so k); m, n <= 2^30. */
 int rtp_matmul_fp8(const void* a, long lda, const float* sa, const void* b, long ldb, const float* sb, int b_square, void* out, int m, int n,
                    int k, int out_dtype, void* stream);
 
 /* Cross attention (csrc/cross_attn.hip): o[b][i][h] = sum_j softmax_j(scale q[b][i][h] . k[b][j][h / (hq / hkv)]) v[b][j][...] over the keys j that
  * count in batch entry b: j < key_lens[b] (clamped to 0 .. sk; NULL: all) and key_mask[b][j] (bytes, strides m_bs and m_ss; NULL: all).  Keys that
  * do not count are not read, whatever they hold; a row without keys gives zeros and takes part in no gradient.  fp16 or bf16, d a multiple of 8
- * up to 128, 0 < scale <= 2e38.  Strides in elements, of batch, token and head; the columns of a head are contiguous; every row 16-byte aligned;
+ * up to 128, 0 < scale <= 2e38.  Scores and sums are fp32; with more than 32 rows (sq * hq / hkv) the exponentials and the scores' gradients are rounded
+ * once to dtype for their second product.  Strides in elements, of batch, token and head; the columns of a head are contiguous; every row 16-byte aligned;
  * token strides of 0 to 2^23, head stride of q and d_o times hq / hkv up to 2^28.
  * o, dq: contiguous [b][sq][hq][d]; dk, dv: contiguous [b][sk][hkv][d], zeros at keys that do not count.  dq, or dk and dv, may be NULL.
  * For a backward pass the forward pass also leaves o_lo (what o's rounding left over, o's type and shape) and lse ([b][hkv][sq * hq / hkv] fp32:

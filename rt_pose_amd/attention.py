@@ -5,7 +5,9 @@
 q: [b, sq, hq, d]; k, v: [b, sk, hkv, d] with hq a multiple of hkv (head h reads k and v of head h // (hq // hkv)).  Of batch entry i the keys j
 with j < key_lens[i] and key_mask[i, j] count.  Keys that do not count -- an encoder's padding -- are never multiplied, whatever they hold (NaN
 too), and get zero gradients; a row without keys gives zeros, and so does one whose every score is minus infinity.  bf16 or fp16, d a multiple of 8 up to 128; any strides (a tensor whose rows
-are not 16-byte aligned is copied).  Sums and softmax are fp32; the result does not depend on scheduling.  Differentiable in q, k and v
+are not 16-byte aligned is copied).  Scores, softmax statistics and sums are fp32.  For the second products (with v; with k, q and o's gradient) the
+exponentials and the scores' gradients are rounded once to the operands' type with more than 32 query rows of a key head (sq * hq / hkv); with up to
+32 both halves of them are kept.  The result does not depend on scheduling.  Differentiable in q, k and v
 (backward; a forward-mode tangent is refused with NotImplementedError).  A trace holds the operator as one node, which checks its arguments at every call.
 With few queries (single tokens while serving, key-point queries) the keys are split over the GPU and joined.
 Errors as in rt_pose_amd.rmsnorm.

@@ -45,3 +45,24 @@ def test_norm_gradients_with_a_weight_that_is_not_trained(rows, h):
     entry = lambda dw, part: _lib.load().rtp_rmsnorm_backward(p(), h, w.data_ptr(), 0, dy.data_ptr(), h, None, 0, dx.data_ptr(), dw, part, rows, h, 2, 1e-6, s)
     assert entry(w.data_ptr(), None) == -1
     assert entry(None, None) == 0 and torch.equal(dx, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 40, 264), (300, 200, 520), (1400, 1300, 384)])
+def test_products_that_cancel(m, n, k):
+    """Large products of opposite sign beside a small one in each group of eight: an fp32 output is exact, the others within what the instruction
+    leaves out."""
+    from rt_pose_amd.fp8 import matmul_fp8
+    from tests.test_gpu_matmul_fp8 import check
+    g = torch.Generator().manual_seed(m)
+    a = torch.zeros(m, k)
+    a[:, 0::8], a[:, 3::8], a[:, 5::8] = 448.0, -448.0, torch.randint(1, 8, (m, len(range(5, k, 8))), generator=g).float()
+    b = torch.ones(n, k)
+    b[:, 0::8] = b[:, 3::8] = 448.0
+    a, b = (t.to(torch.float8_e4m3fn).cuda() for t in (a, b))
+    kb = -(-k // 128)
+    for square in (True, False):
+        sa, sb = torch.ones(m, kb, device="cuda"), torch.ones(-(-n // 128) if square else n, kb, device="cuda")
+        exact = a.double()[:, 5::8].sum(1, keepdim=True).expand(m, n)
+        assert torch.equal(matmul_fp8(a, sa, b, sb, torch.float32).double(), exact)
+        for t in (torch.bfloat16, torch.float16):
+            check(matmul_fp8(a, sa, b, sb, t), a, sa, b, sb, square)
