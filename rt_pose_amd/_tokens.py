@@ -18,8 +18,16 @@ def p(t):
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
+def _recorded_by_fx():
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
+
+
 def call(name, t, *args):
-    """The native entry `name` on the current stream of t's device, with that device current; RtpError if it fails."""
+    """The native entry `name` on the current stream of t's device, with that device current; RtpError if it fails.  Refused under make_fx, which sees
+    torch's operators alone: its graph would hold the output's allocation and not the call."""
+    if torch._C._len_torch_dispatch_stack() and _recorded_by_fx():
+        raise NotImplementedError("rt_pose_amd: the token operators cannot be recorded by make_fx")
     index = t.get_device()
     if index == _current_device():
         rc = getattr(_lib.load(), name)(*args, _raw_stream(index))

@@ -172,3 +172,26 @@ def test_a_weight_that_is_not_trained_costs_no_gradient(monkeypatch):
             f().sum().backward()
             name, args = made[-1]
             assert name == "rtp_rmsnorm_backward" and (args[9] is not None) == (args[10] is not None) == trained
+
+
+def test_a_graph_of_torch_operators_is_refused(monkeypatch):
+    """make_fx runs on real tensors and records torch's operators alone: its graph would return an output that nothing has written."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    from rt_pose_amd import _lib, _tokens, attention, fp8, rmsnorm
+    for module in (attention, fp8, rmsnorm):
+        monkeypatch.setattr(module, "same_device", lambda *a: None)
+    x, w, (q, k, v) = torch.ones(3, 40), torch.ones(40), qkv()
+    (a, sa), (b, sb) = eight(3, 48, False), eight(5, 48, True)
+    for f, args in ((rmsnorm.rms_norm, (x, w)), (rmsnorm.add_rms_norm, (x, x, w)), (rmsnorm.add_rms_norm_fp8, (x, x, w)), (fp8.quantize_fp8, (x,)),
+                    (lambda sa, sb: fp8.matmul_fp8(a, sa, b, sb), (sa, sb)), (attention.cross_attention, (q, k, v))):
+        with pytest.raises(NotImplementedError, match="make_fx"):
+            make_fx(lambda *t: f(*t))(*args)
+    made = []
+    monkeypatch.setattr(_tokens, "_current_device", lambda: -1)
+    monkeypatch.setattr(_tokens, "_raw_stream", lambda index: None)
+    monkeypatch.setattr(_lib, "load", lambda: type("Lib", (), {"rtp_rmsnorm_forward": staticmethod(lambda *a: made.append(1) or 0)}))
+    with FlopCounterMode(display=False):                           # other modes only look on
+        rmsnorm.rms_norm(x, w)
+    assert made
