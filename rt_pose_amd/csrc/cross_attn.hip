@@ -247,7 +247,9 @@ struct XaLoader {
       }
     }
   }
-  // query rows r0 .. r0 + BR - 1; `even`: the group divides a step's rows, so that a step is a whole number of tokens
+  // query rows r0 .. r0 + BR - 1; `even`: the group divides a step's rows, so that a step is a whole number of tokens.  Widths between the images' take
+  // the road that is not `whole` for every tile; with two steps of columns dk / dv's kernel keeps its addresses in scratch there (20 to 28 bytes a
+  // lane): heads of 40, 48 and 56 take 145, 143 and 143 us where heads of 64 take 136.
   template <int BR>
   __device__ __forceinline__ void rows(uint8_t* img, const XaParams& p, const T* src, long ss, long hs, unsigned off, bool even, bool whole, int r0) const {
 #pragma unroll
@@ -387,7 +389,8 @@ __device__ __forceinline__ bool xa_narrow(f32x16& x, f32x16 (&acc)[DT], float& e
 // Four waves: 4 / KW groups of 32 rows, and KW waves that share rows and split each tile of keys (few rows: the keys are the work).
 // Tiles of BK keys go round NBUF LDS buffers: while one is used, the next NBUF - 1 are on their way, and the barrier in front of a tile waits
 // for that tile's transfers alone (they complete in order, PER of them a wave and tile).  Two buffers leave room for more workgroups on a CU,
-// which hide more than a third one (heads of 64: forward 89 us with three, 81 with two); heads up to 32 columns have small tiles and three.
+// which hide more than a third one (heads of 64: forward 89 us with three, 81 with two); heads up to 32 columns have small tiles and three.  In the
+// backward pass of few rows the third hides nothing: its stores of dk and dv count among the newest accesses, so that the wait takes in the tile behind.
 // The mask's words are scalar loads, one tile further ahead, so that nothing else counts as a vector access.
 // (Forming the next tile's scores beside this one's exponentials in one wave takes half as many registers again: 81 -> 103 us.)
 template <int DT, int KW> struct XaKeys {
@@ -472,8 +475,8 @@ __device__ __forceinline__ void xa_mine(const unsigned (&w)[NW], int kw, unsigne
 // ------------------------------------------------------------------------------------------------ forward
 // Many rows are bound by the matrix and vector units together: 32 x 32 scores of a head of 64 are 8 matrix instructions (256 cycles) and a dozen vector
 // instructions a score, the exponential at a quarter of the others' rate.  8 x 8 heads of 64, 2048 x 2048: 84 us, 0.82 PFLOP/s; left out one at a time,
-// staging, exponentials, masks or either product give about a tenth each.  4 x 8 heads of 64, 2560 rows x 0 to 5120 keys: 90 us, 0.51 PFLOP/s: all
-// workgroups with keys are resident at once, four to a CU, and the CU with two long ones ends last.
+// staging, exponentials, masks or either product give about a tenth each.  4 x 8 heads of 64, 2560 rows x 0 to 5120 keys: 91 us, 0.59 PFLOP/s, and 85
+// with as many keys in entries of equal length: 640 workgroups of two and two waves, of which all with keys are resident at once.
 // Few rows are bound by memory and latency: one row, 8 entries of 0 to 2560 keys x 8 heads of 128: 15 us and 4.5 for the join (42 MB, 8.5 us at a large
 // copy's rate); one tile of keys alone takes 7.4 us, further ones 2.1 each.
 // Waves for each SIMD that LDS allows and the registers are shared by (backward of few rows, 8 x 8 heads x 20480 keys x 64 with three: 81 us, with two,
@@ -752,7 +755,8 @@ __device__ __forceinline__ void xa_store_dq(const XaParams& p, const f32x16 (&ac
 
 // ------------------------------------------------------------------------------------------------ backward: dq
 // the forward kernel's shape: s^T and dp^T with a lane per row, dq^T = k^T ds^T, k read from LDS both ways.  Three products for the forward pass's two:
-// 4 x 8 heads of 64, 2560 rows x 0 to 5120 keys 107 us, 0.64 PFLOP/s.
+// 4 x 8 heads of 64, 2560 rows x 0 to 5120 keys 108 us, 0.75 PFLOP/s (entries of equal length 103).  As in the forward pass every fragment that is read
+// from LDS feeds one matrix instruction: by count the two are as busy as each other.
 template <typename T, int DT, int KW>
 __global__ __launch_bounds__(256, XaWaves<DT>::BWD) void xattn_dq_kernel(XaParams p) {
   typedef typename Vec8<T>::type V;
@@ -864,7 +868,9 @@ __global__ __launch_bounds__(256) void xattn_dq_join_kernel(XaParams p) {
 // Each wave keeps 32 keys (k, v as second operands in registers, dk^T and dv^T as accumulators) and walks the rows: s = q k^T and
 // dp = do v^T with a lane per key, then dv^T += do^T p and dk^T += q^T ds with q and do read from LDS both ways.  A lane's key touches its own
 // column of the products alone, so a masked key needs nothing inside the loop: zeros are written for it at the end.  Four products: at the same sizes
-// 135 us, 0.68 PFLOP/s; 640 workgroups with keys, of one length, two or three to a CU.
+// 136 us, 0.79 PFLOP/s; 640 workgroups with keys, of one length, two or three to a CU.  Bound by LDS, by count: a step of 32 x 32 of 64 columns is 16
+// matrix instructions (512 cycles) beside 16 reads of 16 bytes a lane, half of them for L and delta, and 16 transposing ones of 8: 96 KB for the four
+// SIMDs, 768 cycles at 128 bytes a cycle.
 template <int DT> struct XaRows {      // tiles of rows: 64, one for each lane of the wave that brings their L or delta; two buffers
   static constexpr int BR = 64, IMG = BR * XaImg<DT>::PITCH, BUF = 2 * IMG + 2 * BR * 4, BYTES = 2 * BUF;
 };

@@ -346,8 +346,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) void mm8_tile_kernel
   if (p.k & 127) compute(kb, kb & 1, true, false);
   else compute(kb, kb & 1, false, false);
 
-  // The results leave as whole rows of the tile, by way of LDS: 128 bytes or more of a row together, not 64 or 128 a lane group (163840 x 255 x 384:
-  // 36 us, straight from the registers 53; x 256: 30.7 and 31.5, fp32 48 and 53; 8192^3 493 and 505).
+  // The results leave as whole rows of the tile, by way of LDS: 128 bytes or more of a row together, not 64 or 128 a lane group (the same
+  // operands again and again, out of the last-level cache: 163840 x 255 x 384 36 us, straight from the registers 53; x 256 30.7 and 31.5, fp32 48
+  // and 53; 8192^3 493 and 505).
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < MT; ++j)
@@ -419,8 +420,9 @@ static int mm8_launch(Mm8Params p, hipStream_t st) {
   };
   static std::atomic<bool> once256[RTP_MAX_DEVICES], once128[RTP_MAX_DEVICES], once64[RTP_MAX_DEVICES];
   // 256 x 256 halves what is staged per product and wins where the sum is long and its tiles fill whole rounds of the 256 CUs (8192^3: 493 us
-  // against 580, 4096^3: 72 against 77); 128 x 128, two workgroups to a CU, where one's start and end hide behind the other's sum
-  // (163840 x 256 x 384: 40 us against 57, x 1024: 71 against 87).  The exact road needs the registers of the small tile.
+  // against 580 in one run, 493 to 552 over the runs; 4096^3: 72 against 77); 128 x 128, two workgroups to a CU, where one's start and end hide
+  // behind the other's sum (163840 x 256 x 384: 40 us against 57, 39 to 42 over the runs; x 1024: 71 against 87).  The exact road needs the registers
+  // of the small tile: 8192^3 974 us, 163840 x 256 x 384 61.
   if constexpr (sizeof(O) == 2) {
     const long rounds = (tiles256 + 255) / 256;
     if (p.kb >= 16 && tiles256 >= 256 && tiles256 * 5 >= rounds * 256 * 4) return go(mm8_tile_kernel<O, 256, 256, 64, 128, SQUARE>, 256, 256, 512, once256);

@@ -226,7 +226,8 @@ __global__ __launch_bounds__(1024) void rmsnorm_dw_kernel(const float* part, int
 
 // ------------------------------------------------------------------------------------------------ launches
 // lanes per row and chunks per lane by the row's length: 16 lanes up to 128 columns (four rows a wave), a wave up to 2048, a workgroup of
-// 256 up to 8192, of 512 up to 16384, where its registers end (2500 x 16384 bf16: gradients 80 us, with 1024 threads of half as many registers 119)
+// 256 up to 8192, of 512 up to 16384, where its registers end (2500 x 16384 bf16: gradients 78 us, with 1024 threads of half as many registers 119;
+// ragged widths keep 108 bytes a lane in scratch, fp32 172, and read them back in the loop over rows: 2500 x 16383 108 us, in fp32 174 and 164 whole)
 #define NORM_MAX_H 16384
 
 template <typename F>
