@@ -1,7 +1,7 @@
 """Marshalling shared by the token operators (rmsnorm.py, fp8.py, attention.py).  Small calls are bound by the host: one native call, no
 context manager and no stream object where the tensor's device is already the current one."""
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -56,11 +56,14 @@ def without_gradient(ctx, *outputs):
 
 
 def once(backward):
-    """A Function's backward that cannot be differentiated again (autograd says so if one tries).  The guard is put on only where a graph of the
+    """A Function's backward that cannot be differentiated again: autograd says so if one tries, and tangents of the outputs' gradients are refused like
+    the inputs'.  The guard is put on only where a graph of the
     backward pass is asked for: a backward pass runs in a thread of its own, where every line of Python costs twice."""
     guarded = once_differentiable(backward)
 
     def run(ctx, *grads):
+        if forward_ad._current_level >= 0 and any(g is not None and forward_ad.unpack_dual(g).tangent is not None for g in grads):
+            TokenFunction.jvp(ctx)
         return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
     return run
 

@@ -195,3 +195,23 @@ def test_a_graph_of_torch_operators_is_refused(monkeypatch):
     with FlopCounterMode(display=False):                           # other modes only look on
         rmsnorm.rms_norm(x, w)
     assert made
+
+
+def test_tangents_of_the_gradients_are_refused(monkeypatch):
+    """Forward mode over a backward pass: the gradients' derivatives would be lost as the values' would be in the forward pass."""
+    from rt_pose_amd import attention, rmsnorm
+    made = []
+    for module in (attention, rmsnorm):
+        monkeypatch.setattr(module, "same_device", lambda *a: None)
+        monkeypatch.setattr(module, "call", lambda name, *a: made.append(name))
+    x, w, (q, k, v) = torch.ones(3, 40, requires_grad=True), torch.ones(40), qkv()
+    q.requires_grad_(True)
+    for f, t in ((lambda: rmsnorm.rms_norm(x, w), x), (lambda: rmsnorm.add_rms_norm(x, x.detach(), w)[0], x), (lambda: rmsnorm.add_rms_norm(x, x.detach(), w)[1], x),
+                 (lambda: attention.cross_attention(q, k, v), q)):
+        with fw.dual_level():
+            y = f()
+            one = torch.ones_like(y)
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, t, fw.make_dual(one, one))
+            y = f()
+            torch.autograd.grad(y, t, one)                         # a level alone is no tangent
